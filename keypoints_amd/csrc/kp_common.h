@@ -139,9 +139,9 @@ __device__ __forceinline__ float kp_bnin1(float y, float mu, float is, float ga,
     const float z = (y - mu) * is * ga + be;
     return fmaxf(z, z * slope);
 }
-// one 16-byte chunk = 8 consecutive channels of a pixel, raw conv output -> stored activation: kp_bnin1 on the eight elements,
-// written on channel PAIRS so that the four arithmetic steps are packed instructions (v_pk_add_f32 / v_pk_mul_f32: 28
-// instead of 48 VALU per chunk; the same IEEE operation per element, no contraction: -ffp-contract=off)
+// one 16-byte chunk = 8 consecutive channels of a pixel, raw conv output -> stored activation: kp_bnin1 on the eight elements, two
+// at a time as they are unpacked and packed (the same IEEE operation per element, no contraction: -ffp-contract=off; the packed fp32
+// instructions are switched off for the whole library, Makefile)
 __device__ __forceinline__ uint4 kp_bnin8(const uint4 raw, const float (&mu)[8], const float (&is)[8], const float (&ga)[8],
                                           const float (&be)[8], float slope) {
     const uint32_t w[4] = {raw.x, raw.y, raw.z, raw.w};
