@@ -536,6 +536,53 @@ int kp_warp_affine(const float* x, const float* mat, float* out, int N, int C, i
  * rotate_affine_grid_multi (tps.py:154-166) is formed in the kernel instead of on the host */
 int kp_warp_rotate(const float* x, const float* angle, float* out, int N, int C, int H, int W, void* stream);
 
+/* ---- the 8-bit block format -------------------------------------------------------------------------------------------------
+ * A matrix in rows; each row is cut into blocks of 128 consecutive elements (the last block may be short).  A block is e4m3 or e5m2
+ * bytes q and ONE exponent byte s + 127: element = value(q) * 2^s.  s = the smallest whole number >= -127 that brings the block's
+ * largest finite magnitude M to M * 2^-s <= 448 (e4m3) / 57344 (e5m2); s = 0 for a block of zeros.  q = x * 2^-s rounded to nearest, ties
+ * to even (x * 2^-s is exact): an element is off by at most 2^-4 (e4m3) / 2^-3 (e5m2) of itself, below the format's smallest normal number
+ * by at most 2^(s-10) / 2^(s-17).  Not-a-numbers stay; infinities stay in e5m2 and become not-a-numbers in e4m3.
+ * Strides: ldq bytes between rows of q, lds bytes between rows of exponent bytes, ld* of T matrices in elements. */
+#define KP_E4M3 1
+#define KP_E5M2 2
+/* x T [rows][cols] -> q, s.  ldq >= cols rounded up to whole blocks: the last block is written out with zeros (what kp_q8_matmul takes);
+ * ldq == cols: rows lie back to back.  A tensor of n elements in memory order is one row of n. */
+int kp_q8_pack(const void* x, long long ldx, unsigned char* q, long long ldq, unsigned char* s, long long lds, long long rows,
+               long long cols, int dtype, int fmt, void* stream);
+/* and back: y T [rows][cols] = value(q) * 2^s, rounded once; a finite element that the format rounded past T's range is T's largest number */
+int kp_q8_unpack(const unsigned char* q, long long ldq, const unsigned char* s, long long lds, void* y, long long ldy, long long rows,
+                 long long cols, int dtype, int fmt, void* stream);
+/* One read of x, up to three results, each left out with a NULL pointer: the row form (q, s: blocks along the columns, rows padded to whole
+ * blocks), the column form (qt, st: row c holds column c of x, blocks along the rows, padded alike; qt on a multiple of 16 bytes) and the
+ * fp32 column sums colsum[cols] (fixed order; ws: kp_q8_pack_both_ws_floats floats).  The forward of a linear layer packs its input both
+ * ways -- rows for its own product, columns for the weight gradient's, which is the activation checkpoint -- and the backward its output
+ * gradient, with the bias gradient as column sums. */
+int kp_q8_pack_both(const void* x, long long ldx, unsigned char* q, long long ldq, unsigned char* s, long long lds, unsigned char* qt,
+                    long long ldqt, unsigned char* st, long long ldst, float* ws, float* colsum, long long rows, long long cols, int dtype,
+                    int fmt, void* stream);
+long long kp_q8_pack_both_ws_floats(long long rows, long long cols);
+/* c T [M][N] = sum_k a[m][k] b[n][k] (+ bias[n], fp32, may be NULL), fp32 accumulation, rounded once.  a, b: row forms along k padded to
+ * whole blocks, rows on multiples of 16 bytes; rows of exponent bytes on multiples of 4 bytes with whole words readable (lds % 4 == 0).
+ * ws: kp_q8_matmul_ws_floats floats (0 for most shapes: then NULL), used when few tiles split the sum; joined in a fixed order. */
+int kp_q8_matmul(const unsigned char* a, long long lda, const unsigned char* sa, long long ldsa, int fmta, const unsigned char* b,
+                 long long ldb, const unsigned char* sb, long long ldsb, int fmtb, const float* bias, void* c, long long ldc, float* ws,
+                 long long M, long long N, long long K, int dtype, void* stream);
+long long kp_q8_matmul_ws_floats(long long M, long long N, long long K);
+
+/* ---- layer norm ----------------------------------------------------------------------------------------------------------------
+ * Per row of C elements: y = (x - mean) * rstd * w + b, rstd = 1 / sqrt(mean((x - mean)^2) + eps).  w, b fp32 or NULL (1, 0).  mean, rstd
+ * [rows] fp32 are written when not NULL (both or none).  q, s (both or none): x in the 8-bit format as well, q [rows][C] back to back,
+ * s [rows][ceil(C / 128)]: what the backward may read instead of x. */
+int kp_layer_norm_fwd(const void* x, long long ldx, const float* w, const float* b, float eps, void* y, long long ldy, float* mean,
+                      float* rstd, unsigned char* q, unsigned char* s, int fmt, long long rows, int C, int dtype, void* stream);
+/* dx = rstd (g - mean(g) - xh mean(g xh)) with g = dy w, xh = (x - mean) rstd (x, or the values q, s stand for); dw = sum dy xh, db = sum
+ * dy, fp32, overwritten; each of dx, dw, db may be NULL.  ws: kp_layer_norm_bwd_ws_floats floats when dw or db is asked for.  Sums are
+ * taken in a fixed order. */
+int kp_layer_norm_bwd(const void* dy, long long lddy, const void* x, long long ldx, const unsigned char* q, const unsigned char* s, int fmt,
+                      const float* w, const float* mean, const float* rstd, void* dx, long long lddx, float* ws, float* dw, float* db,
+                      long long rows, int C, int dtype, void* stream);
+long long kp_layer_norm_bwd_ws_floats(long long rows, int C);
+
 /* ---- loss and optimiser -------------------------------------------------- */
 /* l2_reconstruction_loss (transporter.py:56-60): loss_sum[0] += sum (x-t)^2*mask (fp64, zeroed by caller);
  * grad = 2*(x-t)*mask*scale  (scale = 1/numel).  mask may be NULL. */

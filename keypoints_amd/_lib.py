@@ -13,6 +13,7 @@ _HERE = os.path.dirname(os.path.abspath(__file__))
 LIB_PATH = os.path.join(_HERE, 'csrc', 'libkp_hip.so')
 
 KP_F32, KP_BF16, KP_F16 = 0, 1, 2
+KP_E4M3, KP_E5M2 = 1, 2
 TAIL_NONE, TAIL_MAXPOOL2, TAIL_UPSAMPLE2 = 0, 1, 2
 KP_CFG_CUS = 6   # kp_config key: CU budget of the persistent kernels (include/kp_hip.h)
 COMBINE = {'sum_and_clamp': 1, 'pretrained_network': 2, 'loop': 3}
@@ -75,6 +76,12 @@ SIGNATURES = {
     'kp_warp_tps': [_p, _p, _p, _p, _i, _i, _i, _i, _i, _i, _i, _p],
     'kp_warp_affine': [_p, _p, _p, _i, _i, _i, _i, _p],
     'kp_warp_rotate': [_p, _p, _p, _i, _i, _i, _i, _p],
+    'kp_q8_pack': [_p, _ll, _p, _ll, _p, _ll, _ll, _ll, _i, _i, _p],
+    'kp_q8_unpack': [_p, _ll, _p, _ll, _p, _ll, _ll, _ll, _i, _i, _p],
+    'kp_q8_pack_both': [_p, _ll, _p, _ll, _p, _ll, _p, _ll, _p, _ll, _p, _p, _ll, _ll, _i, _i, _p],
+    'kp_q8_matmul': [_p, _ll, _p, _ll, _i, _p, _ll, _p, _ll, _i, _p, _p, _ll, _p, _ll, _ll, _ll, _i, _p],
+    'kp_layer_norm_fwd': [_p, _ll, _p, _p, _f, _p, _ll, _p, _p, _p, _p, _i, _ll, _i, _i, _p],
+    'kp_layer_norm_bwd': [_p, _ll, _p, _ll, _p, _p, _i, _p, _p, _p, _p, _ll, _p, _p, _p, _ll, _i, _i, _p],
     'kp_l2_loss': [_p, _p, _p, _p, _p, _f, _z, _p],
     'kp_l2_loss_mean': [_p, _p, _p, _p, _p, _p, _z, _p],
     'kp_scale': [_p, _p, _p, _z, _p],
@@ -101,7 +108,7 @@ SIGNATURES = {
     'kp_prof_bytes': [_i, _p],
     'kp_prof_step_bytes': [_p, _p],
 }
-PLAIN = {'kp_config_get': ([_i], _i), 'kp_conv_fwd_act_supported': ([_i] * 6, _i), 'kp_conv_fwd_fin_folds': ([_i] * 7, _i), 'kp_comm_available': ([], _i), 'kp_conv_pair_supported': ([_i] * 7, _i), 'kp_head_pair_supported': ([_i] * 7, _i), 'kp_conv_wgrad_pad_hw': ([_i] * 7 + [_p, _p], _i), 'kp_conv_first_fused_supported': ([_i] * 6, _i), 'kp_conv_first_fused_rows': ([_i] * 6, _ll), 'kp_bn_finalize_pair_supported': ([_ll, _i], _i), 'kp_head_t_supported': ([_i] * 6, _i), 'kp_keypoint_bottleneck_t_supported': ([_i] * 6, _i), 'kp_conv_bnin_supported': ([_i] * 6, _i), 'kp_head_bnin_supported': ([_i] * 6, _i), 'kp_conv_dgrad_bnred_supported': ([_i] * 6, _i), 'kp_conv_dgrad_bnred_rows': ([_i] * 6, _ll), 'kp_unit_infer_param_floats': ([_i, _i, _p], _ll), 'kp_conv_wgrad_partials': ([_i] * 8, _i), 'kp_conv_fwd_stats_rows': ([_i] * 7, _ll), 'kp_bn_bwd_rows': ([_i] * 7, _ll), 'kp_head_bwd_ws_floats': ([_i] * 6, _ll), 'kp_last_rows': ([], _ll), 'kp_bn_ws_doubles': ([_i], _i), 'kp_version': ([], _i), 'kp_last_error': ([], C.c_char_p), 'kp_device_cus': ([], _i)}
+PLAIN = {'kp_q8_pack_both_ws_floats': ([_ll, _ll], _ll), 'kp_q8_matmul_ws_floats': ([_ll, _ll, _ll], _ll), 'kp_layer_norm_bwd_ws_floats': ([_ll, _i], _ll), 'kp_config_get': ([_i], _i), 'kp_conv_fwd_act_supported': ([_i] * 6, _i), 'kp_conv_fwd_fin_folds': ([_i] * 7, _i), 'kp_comm_available': ([], _i), 'kp_conv_pair_supported': ([_i] * 7, _i), 'kp_head_pair_supported': ([_i] * 7, _i), 'kp_conv_wgrad_pad_hw': ([_i] * 7 + [_p, _p], _i), 'kp_conv_first_fused_supported': ([_i] * 6, _i), 'kp_conv_first_fused_rows': ([_i] * 6, _ll), 'kp_bn_finalize_pair_supported': ([_ll, _i], _i), 'kp_head_t_supported': ([_i] * 6, _i), 'kp_keypoint_bottleneck_t_supported': ([_i] * 6, _i), 'kp_conv_bnin_supported': ([_i] * 6, _i), 'kp_head_bnin_supported': ([_i] * 6, _i), 'kp_conv_dgrad_bnred_supported': ([_i] * 6, _i), 'kp_conv_dgrad_bnred_rows': ([_i] * 6, _ll), 'kp_unit_infer_param_floats': ([_i, _i, _p], _ll), 'kp_conv_wgrad_partials': ([_i] * 8, _i), 'kp_conv_fwd_stats_rows': ([_i] * 7, _ll), 'kp_bn_bwd_rows': ([_i] * 7, _ll), 'kp_head_bwd_ws_floats': ([_i] * 6, _ll), 'kp_last_rows': ([], _ll), 'kp_bn_ws_doubles': ([_i], _i), 'kp_version': ([], _i), 'kp_last_error': ([], C.c_char_p), 'kp_device_cus': ([], _i)}
 
 _lib = None
 

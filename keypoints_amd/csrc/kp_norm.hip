@@ -1,0 +1,453 @@
+// Layer norm over the last dimension: y = (x - mean) * rstd * w + b per row of C elements, forward and backward, with the reduction of the
+// weight's and bias's gradients.  Statistics and sums in fp32, over registers: a row is read once, its variance is the mean of the squared
+// distances from its mean (no difference of large squares).
+//
+//   forward   reads x, writes y (and, for a backward, mean and rstd; with keep the row in the 8-bit block format of kp_q8_dev.h, taken from
+//             the registers the row is in anyway)
+//   backward  g = dy w, xh = (x - mean) rstd, dx = rstd (g - mean(g) - xh mean(g xh)); a thread's columns are the same for every row it
+//             meets, so dw += dy xh and db += dy stay in its registers; one partial row a workgroup, joined by a second launch in a fixed
+//             order (fp64), so equal calls give equal bits
+//
+// Both are bound by memory.  A row is spread over G lanes, 8 consecutive elements (16 bytes of a 16-bit type) each, NJ times: the smallest
+// power of two that holds it up to a wave (rows of 64 elements: eight rows a wave), then a workgroup of 256 or 1024 threads with sums
+// through LDS, and beyond 16384 elements a workgroup that walks the row and reads it again.
+#include "kp_q8_dev.h"
+
+namespace {
+
+// ---- sums and maxima over a row's G lanes (G <= 64: lanes of a wave, aligned; more: the whole workgroup) ---------------------------------
+template <int CTRL> __device__ __forceinline__ float ln_dpp(float v) { return __uint_as_float(q8_dpp<CTRL>(__float_as_uint(v))); }
+template <int G> __device__ __forceinline__ float ln_wave_sum(float v) {
+    if constexpr (G >= 2) v += ln_dpp<0xB1>(v);      // lane ^ 1
+    if constexpr (G >= 4) v += ln_dpp<0x4E>(v);      // lane ^ 2
+    if constexpr (G >= 8) v += ln_dpp<0x141>(v);     // lane ^ 7
+    if constexpr (G >= 16) v += ln_dpp<0x128>(v);    // lane + 8 of 16
+    if constexpr (G >= 32) v += __shfl_xor(v, 16, 64);
+    if constexpr (G >= 64) v += __shfl_xor(v, 32, 64);
+    return v;
+}
+template <int G> __device__ __forceinline__ uint32_t ln_block_max(uint32_t m) {   // over the lanes of one 128-block: min(G, 16)
+    if constexpr (G >= 2) m = q8_umax(m, q8_dpp<0xB1>(m));
+    if constexpr (G >= 4) m = q8_umax(m, q8_dpp<0x4E>(m));
+    if constexpr (G >= 8) m = q8_umax(m, q8_dpp<0x141>(m));
+    if constexpr (G >= 16) m = q8_umax(m, q8_dpp<0x128>(m));
+    return m;
+}
+// `red`: one float a wave and call slot; every thread of the workgroup calls it
+template <int G> __device__ __forceinline__ float ln_sum(float v, float* red) {
+    v = ln_wave_sum<(G < 64 ? G : 64)>(v);
+    if constexpr (G > 64) {
+        if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = v;
+        __syncthreads();
+        v = 0.f;
+#pragma unroll
+        for (int w = 0; w < G / 64; ++w) v += red[w];
+    }
+    return v;
+}
+
+struct LnFwd {
+    const void* x; const float *w, *b; void* y; float *mean, *rstd; uint8_t *q, *s;
+    long long ldx, ldy, rows; int C, nb; float eps; bool vec;   // vec: all rows start on multiples of 16 bytes
+};
+struct LnBwd {
+    const void *dy, *x; const uint8_t *q, *s; const float *w, *mean, *rstd; void* dx; float* part;
+    long long lddy, ldx, lddx, rows; int C, nb; bool vec;
+};
+
+template <int G> constexpr int ln_tpb = G > 256 ? G : 256;
+
+// KEEP: 0, or KP_E4M3 / KP_E5M2: the row leaves in 8 bits too
+template <int DT, int G, int NJ, int KEEP>
+__global__ __launch_bounds__(ln_tpb<G>) void ln_fwd_k(const LnFwd P) {
+    constexpr int TPB = ln_tpb<G>, R = TPB / G;
+    __shared__ float red[G > 64 ? 2 * (G / 64) : 1];
+    const int sub = threadIdx.x & (G - 1);
+    const float inv = 1.f / (float)P.C;
+    int n[NJ];
+#pragma unroll
+    for (int j = 0; j < NJ; ++j) {
+        const int left = P.C - (j * G + sub) * 8;
+        n[j] = left < 0 ? 0 : (left < 8 ? left : 8);
+    }
+    for (long long r0 = (long long)blockIdx.x * R; r0 < P.rows; r0 += (long long)gridDim.x * R) {
+        const long long row = r0 + threadIdx.x / G;
+        const bool live = row < P.rows;
+        float v[NJ][8];
+        float sum = 0.f;
+#pragma unroll
+        for (int j = 0; j < NJ; ++j) {
+            const long long at = row * P.ldx + (j * G + sub) * 8;
+            if (P.vec && n[j] == 8 && live) el_load8<DT>(P.x, at, v[j]);
+            else el_load8_part<DT>(P.x, at, live ? n[j] : 0, v[j]);
+        }
+#pragma unroll
+        for (int j = 0; j < NJ; ++j)
+#pragma unroll
+            for (int k = 0; k < 8; ++k) sum += v[j][k];
+        const float mean = ln_sum<G>(sum, red) * inv;
+        float sq = 0.f;
+#pragma unroll
+        for (int j = 0; j < NJ; ++j)
+#pragma unroll
+            for (int k = 0; k < 8; ++k) {
+                const float d = k < n[j] ? v[j][k] - mean : 0.f;
+                sq = __builtin_fmaf(d, d, sq);
+            }
+        const float rstd = 1.f / sqrtf(ln_sum<G>(sq, red + (G > 64 ? G / 64 : 0)) * inv + P.eps);
+#pragma unroll
+        for (int j = 0; j < NJ; ++j) {
+            const int c = (j * G + sub) * 8;
+            if constexpr (KEEP != 0) {
+                const uint32_t byte = q8_scale_byte<KEEP>(ln_block_max<G>(q8_mag8(v[j])));
+                if (live && n[j] > 0) {
+                    const q8_u32x2 o = q8_cvt8<KEEP>(v[j], q8_down(byte));
+                    if (P.vec && n[j] == 8) *reinterpret_cast<q8_u32x2*>(P.q + row * P.C + c) = o;
+                    else q8_store8_part(P.q + row * P.C + c, n[j], o);
+                    if ((c & (Q8_BLOCK - 1)) == 0) P.s[row * P.nb + c / Q8_BLOCK] = (uint8_t)byte;
+                }
+            }
+            float w[8], b[8], o[8];
+            if (P.w) { if (P.vec && n[j] == 8) el_load8<KP_F32>(P.w, c, w); else el_load8_part<KP_F32>(P.w, c, n[j], w); }
+            if (P.b) { if (P.vec && n[j] == 8) el_load8<KP_F32>(P.b, c, b); else el_load8_part<KP_F32>(P.b, c, n[j], b); }
+#pragma unroll
+            for (int k = 0; k < 8; ++k) {
+                o[k] = (v[j][k] - mean) * rstd;
+                if (P.w) o[k] *= w[k];
+                if (P.b) o[k] += b[k];
+            }
+            if (live) {
+                if (P.vec && n[j] == 8) el_store8<DT>(P.y, row * P.ldy + c, o);
+                else el_store8_part<DT>(P.y, row * P.ldy + c, n[j], o);
+            }
+        }
+        if (P.mean && sub == 0 && live) {
+            P.mean[row] = mean;
+            P.rstd[row] = rstd;
+        }
+        if constexpr (G > 64) __syncthreads();   // (the sums' slots are written again)
+    }
+}
+
+template <int DT, int G, int NJ, int KEEP>
+__global__ __launch_bounds__(ln_tpb<G>) void ln_bwd_k(const LnBwd P) {
+    constexpr int TPB = ln_tpb<G>, R = TPB / G;
+    __shared__ float red[G > 64 ? 2 * (G / 64) : 1];
+    __shared__ float join[G < 256 ? 4 * (G < 64 ? G : 64) * 8 : 1];
+    const int sub = threadIdx.x & (G - 1);
+    const float inv = 1.f / (float)P.C;
+    int n[NJ];
+    float dw[NJ][8], db[NJ][8];
+#pragma unroll
+    for (int j = 0; j < NJ; ++j) {
+        const int left = P.C - (j * G + sub) * 8;
+        n[j] = left < 0 ? 0 : (left < 8 ? left : 8);
+#pragma unroll
+        for (int k = 0; k < 8; ++k) dw[j][k] = db[j][k] = 0.f;
+    }
+    for (long long r0 = (long long)blockIdx.x * R; r0 < P.rows; r0 += (long long)gridDim.x * R) {
+        const long long row = r0 + threadIdx.x / G;
+        const bool live = row < P.rows;
+        const float mean = live ? P.mean[row] : 0.f, rstd = live ? P.rstd[row] : 0.f;
+        float g[NJ][8], xh[NJ][8];
+        float a = 0.f, b = 0.f;
+#pragma unroll
+        for (int j = 0; j < NJ; ++j) {
+            const int c = (j * G + sub) * 8, m = live ? n[j] : 0;
+            if constexpr (KEEP != 0) {
+                const float up = m > 0 ? q8_up(P.s[row * P.nb + c / Q8_BLOCK]) : 1.f;
+                if (P.vec && m == 8) q8_values8<KEEP>(*reinterpret_cast<const q8_u32x2*>(P.q + row * P.C + c), up, xh[j]);
+                else q8_values8<KEEP>(q8_load8_part(P.q + row * P.C + c, m), up, xh[j]);
+            } else {
+                if (P.vec && m == 8) el_load8<DT>(P.x, row * P.ldx + c, xh[j]);
+                else el_load8_part<DT>(P.x, row * P.ldx + c, m, xh[j]);
+            }
+            if (P.vec && m == 8) el_load8<DT>(P.dy, row * P.lddy + c, g[j]);
+            else el_load8_part<DT>(P.dy, row * P.lddy + c, m, g[j]);
+        }
+#pragma unroll
+        for (int j = 0; j < NJ; ++j) {
+            const int c = (j * G + sub) * 8;
+            float w[8];
+            if (P.w) { if (P.vec && n[j] == 8) el_load8<KP_F32>(P.w, c, w); else el_load8_part<KP_F32>(P.w, c, n[j], w); }
+#pragma unroll
+            for (int k = 0; k < 8; ++k) {
+                xh[j][k] = (xh[j][k] - mean) * rstd;
+                db[j][k] += g[j][k];
+                dw[j][k] = __builtin_fmaf(g[j][k], xh[j][k], dw[j][k]);
+                if (P.w) g[j][k] *= w[k];
+                a += g[j][k];                                      // (past the row's end g is zero)
+                b = __builtin_fmaf(g[j][k], xh[j][k], b);
+            }
+        }
+        a = ln_sum<G>(a, red) * inv;
+        b = ln_sum<G>(b, red + (G > 64 ? G / 64 : 0)) * inv;
+        if (P.dx && live) {
+#pragma unroll
+            for (int j = 0; j < NJ; ++j) {
+                const int c = (j * G + sub) * 8;
+                float o[8];
+#pragma unroll
+                for (int k = 0; k < 8; ++k) o[k] = rstd * (g[j][k] - a - xh[j][k] * b);
+                if (P.vec && n[j] == 8) el_store8<DT>(P.dx, row * P.lddx + c, o);
+                else el_store8_part<DT>(P.dx, row * P.lddx + c, n[j], o);
+            }
+        }
+        if constexpr (G > 64) __syncthreads();
+    }
+    if (!P.part) return;
+    // the workgroup's partial row [2][C]: first the groups of a wave (lanes with the same columns), then the waves
+    float* prow = P.part + (long long)blockIdx.x * 2 * P.C;
+#pragma unroll
+    for (int which = 0; which < 2; ++which) {
+        float (&acc)[NJ][8] = which ? db : dw;
+#pragma unroll
+        for (int j = 0; j < NJ; ++j) {
+            const int c = (j * G + sub) * 8;
+            if constexpr (G < 256) {
+                constexpr int W = G < 64 ? G : 64;
+#pragma unroll
+                for (int k = 0; k < 8; ++k) {
+                    float s = acc[j][k];
+#pragma unroll
+                    for (int o = W; o < 64; o <<= 1) s += __shfl_xor(s, o, 64);
+                    if ((threadIdx.x & 63) < W) join[((threadIdx.x >> 6) * W + sub) * 8 + k] = s;
+                }
+                __syncthreads();
+                if (threadIdx.x < W)
+#pragma unroll
+                    for (int k = 0; k < 8; ++k)
+                        if (k < n[j]) {
+                            float s = 0.f;
+#pragma unroll
+                            for (int wv = 0; wv < 4; ++wv) s += join[(wv * W + sub) * 8 + k];
+                            prow[which * P.C + c + k] = s;
+                        }
+                __syncthreads();
+            } else {
+#pragma unroll
+                for (int k = 0; k < 8; ++k)
+                    if (k < n[j]) prow[which * P.C + c + k] = acc[j][k];
+            }
+        }
+    }
+}
+
+// Rows past 16384 elements: a workgroup walks the row, element by element and thread, and reads it again for each pass.
+template <int DT, int KEEP>
+__global__ __launch_bounds__(1024) void ln_fwd_long_k(const LnFwd P) {
+    __shared__ float red[32];
+    const float inv = 1.f / (float)P.C;
+    for (long long row = blockIdx.x; row < P.rows; row += gridDim.x) {
+        float sum = 0.f;
+        for (int c = threadIdx.x; c < P.C; c += 1024) sum += el_load<DT>(P.x, row * P.ldx + c);
+        const float mean = ln_sum<1024>(sum, red) * inv;
+        float sq = 0.f;
+        for (int c = threadIdx.x; c < P.C; c += 1024) {
+            const float d = el_load<DT>(P.x, row * P.ldx + c) - mean;
+            sq = __builtin_fmaf(d, d, sq);
+        }
+        const float rstd = 1.f / sqrtf(ln_sum<1024>(sq, red + 16) * inv + P.eps);
+        for (int c = threadIdx.x; c < P.C; c += 1024) {
+            float o = (el_load<DT>(P.x, row * P.ldx + c) - mean) * rstd;
+            if (P.w) o *= P.w[c];
+            if (P.b) o += P.b[c];
+            el_store<DT>(P.y, row * P.ldy + c, o);
+        }
+        if (P.mean && threadIdx.x == 0) {
+            P.mean[row] = mean;
+            P.rstd[row] = rstd;
+        }
+        if constexpr (KEEP != 0) {   // 16 lanes a block, as in q8_pack_k
+            const int sub = threadIdx.x & 15;
+            for (int b0 = 0; b0 < P.nb; b0 += 64) {
+                const int kb = b0 + (int)(threadIdx.x >> 4), c = kb * Q8_BLOCK + sub * 8;
+                const int n = P.C - c >= 8 ? 8 : (P.C > c ? P.C - c : 0);
+                float v[8];
+                el_load8_part<DT>(P.x, row * P.ldx + c, n, v);
+                const uint32_t byte = q8_scale_byte<KEEP>(q8_max16(q8_mag8(v)));
+                q8_store8_part(P.q + row * P.C + c, n, q8_cvt8<KEEP>(v, q8_down(byte)));
+                if (sub == 0 && kb < P.nb) P.s[row * P.nb + kb] = (uint8_t)byte;
+            }
+        }
+        __syncthreads();
+    }
+}
+template <int DT, int KEEP> __device__ __forceinline__ float ln_kept(const LnBwd& P, long long row, int c) {
+    if constexpr (KEEP == 0) return el_load<DT>(P.x, row * P.ldx + c);
+    else {
+        float v[8];
+        q8_values8<KEEP>(q8_u32x2{P.q[row * P.C + c], 0u}, q8_up(P.s[row * P.nb + c / Q8_BLOCK]), v);
+        return v[0];
+    }
+}
+template <int DT, int KEEP>
+__global__ __launch_bounds__(1024) void ln_bwd_long_k(const LnBwd P) {
+    __shared__ float red[32];
+    const float inv = 1.f / (float)P.C;
+    for (long long row = blockIdx.x; row < P.rows; row += gridDim.x) {
+        const float mean = P.mean[row], rstd = P.rstd[row];
+        float a = 0.f, b = 0.f;
+        for (int c = threadIdx.x; c < P.C; c += 1024) {
+            const float g = el_load<DT>(P.dy, row * P.lddy + c) * (P.w ? P.w[c] : 1.f);
+            a += g;
+            b = __builtin_fmaf(g, (ln_kept<DT, KEEP>(P, row, c) - mean) * rstd, b);
+        }
+        a = ln_sum<1024>(a, red) * inv;
+        b = ln_sum<1024>(b, red + 16) * inv;
+        for (int c = threadIdx.x; c < P.C; c += 1024) {
+            const float g = el_load<DT>(P.dy, row * P.lddy + c) * (P.w ? P.w[c] : 1.f);
+            el_store<DT>(P.dx, row * P.lddx + c, rstd * (g - a - (ln_kept<DT, KEEP>(P, row, c) - mean) * rstd * b));
+        }
+        __syncthreads();
+    }
+}
+template <int DT, int KEEP>
+__global__ __launch_bounds__(256) void ln_cols_long_k(const LnBwd P) {
+    const int c = blockIdx.x * 256 + threadIdx.x;
+    if (c >= P.C) return;
+    float dw = 0.f, db = 0.f;
+    for (long long row = blockIdx.y; row < P.rows; row += gridDim.y) {
+        const float g = el_load<DT>(P.dy, row * P.lddy + c);
+        db += g;
+        dw = __builtin_fmaf(g, (ln_kept<DT, KEEP>(P, row, c) - P.mean[row]) * P.rstd[row], dw);
+    }
+    float* prow = P.part + (long long)blockIdx.y * 2 * P.C;
+    prow[c] = dw;
+    prow[P.C + c] = db;
+}
+
+// the partial rows [parts][2][C] joined in a fixed order: 32 columns x 32 runs of parts a workgroup
+__global__ __launch_bounds__(1024) void ln_join_k(const float* __restrict__ part, float* __restrict__ dw, float* __restrict__ db, int parts,
+                                                  int C) {
+    __shared__ double red[32][33];
+    const int col = threadIdx.x & 31, run = threadIdx.x >> 5;
+    const long long c = (long long)blockIdx.x * 32 + col, width = 2LL * C;
+    double s = 0.0;
+    if (c < width)
+        for (int p = run; p < parts; p += 32) s += (double)part[p * width + c];
+    red[run][col] = s;
+    __syncthreads();
+    if (run == 0 && c < width) {
+        for (int k = 1; k < 32; ++k) s += red[k][col];
+        if (c < C) { if (dw) dw[c] = (float)s; }
+        else if (db) db[c - C] = (float)s;
+    }
+}
+
+// ---- which kernel -----------------------------------------------------------------------------------------------------------------
+constexpr int LONG = 16384;
+int ln_group(int C) {   // lanes of a row
+    if (C > 4096) return 1024;
+    if (C > 1024) return 256;
+    int g = 1;
+    while (g < 64 && g * 8 < C) g <<= 1;
+    return g;
+}
+// workgroups of the backward: every one leaves a partial row of 2 C floats, which the join reads back
+int ln_parts(long long rows, int C) {
+    const int g = ln_group(C), per = C > LONG ? 1 : (g > 256 ? 1 : 256 / g);
+    const long long want = (rows + per - 1) / per;
+    const long long cap = C > LONG ? 64 : (C > 1024 ? 512 : 1024);
+    return (int)(want < cap ? want : cap);
+}
+
+template <int DT, int KEEP> int fwd_launch(const LnFwd& P, hipStream_t st) {
+    if (P.C > LONG) {
+        ln_fwd_long_k<DT, KEEP><<<(unsigned)(P.rows < 1024 ? P.rows : 1024), 1024, 0, st>>>(P);
+        return kp_check_launch("layer_norm_fwd");
+    }
+    const int g = ln_group(P.C), per = g > 256 ? 1 : 256 / g;
+    const long long want = (P.rows + per - 1) / per;
+    const unsigned grid = (unsigned)(want < 4096 ? want : 4096);
+#define LN_FWD(G, NJ) ln_fwd_k<DT, G, NJ, KEEP><<<grid, ln_tpb<G>, 0, st>>>(P)
+    switch (g) {
+        case 1: LN_FWD(1, 1); break;
+        case 2: LN_FWD(2, 1); break;
+        case 4: LN_FWD(4, 1); break;
+        case 8: LN_FWD(8, 1); break;
+        case 16: LN_FWD(16, 1); break;
+        case 32: LN_FWD(32, 1); break;
+        case 64: if (P.C <= 512) LN_FWD(64, 1); else LN_FWD(64, 2); break;
+        case 256: if (P.C <= 2048) LN_FWD(256, 1); else LN_FWD(256, 2); break;
+        default: if (P.C <= 8192) LN_FWD(1024, 1); else LN_FWD(1024, 2); break;
+    }
+#undef LN_FWD
+    return kp_check_launch("layer_norm_fwd");
+}
+template <int DT, int KEEP> int bwd_launch(const LnBwd& P, int parts, hipStream_t st) {
+    if (P.C > LONG) {
+        if (P.dx) ln_bwd_long_k<DT, KEEP><<<(unsigned)(P.rows < 1024 ? P.rows : 1024), 1024, 0, st>>>(P);
+        if (P.part) ln_cols_long_k<DT, KEEP><<<dim3(cdiv(P.C, 256), parts), 256, 0, st>>>(P);
+        return kp_check_launch("layer_norm_bwd");
+    }
+#define LN_BWD(G, NJ) ln_bwd_k<DT, G, NJ, KEEP><<<parts, ln_tpb<G>, 0, st>>>(P)
+    switch (ln_group(P.C)) {
+        case 1: LN_BWD(1, 1); break;
+        case 2: LN_BWD(2, 1); break;
+        case 4: LN_BWD(4, 1); break;
+        case 8: LN_BWD(8, 1); break;
+        case 16: LN_BWD(16, 1); break;
+        case 32: LN_BWD(32, 1); break;
+        case 64: if (P.C <= 512) LN_BWD(64, 1); else LN_BWD(64, 2); break;
+        case 256: if (P.C <= 2048) LN_BWD(256, 1); else LN_BWD(256, 2); break;
+        default: if (P.C <= 8192) LN_BWD(1024, 1); else LN_BWD(1024, 2); break;
+    }
+#undef LN_BWD
+    return kp_check_launch("layer_norm_bwd");
+}
+template <int DT> int fwd_type(const LnFwd& P, int fmt, hipStream_t st) {
+    if (!P.q) return fwd_launch<DT, 0>(P, st);
+    if (fmt == KP_E4M3) return fwd_launch<DT, KP_E4M3>(P, st);
+    return fwd_launch<DT, KP_E5M2>(P, st);
+}
+template <int DT> int bwd_type(const LnBwd& P, int fmt, int parts, hipStream_t st) {
+    if (!P.q) return bwd_launch<DT, 0>(P, parts, st);
+    if (fmt == KP_E4M3) return bwd_launch<DT, KP_E4M3>(P, parts, st);
+    return bwd_launch<DT, KP_E5M2>(P, parts, st);
+}
+bool ln_aligned(const void* p, long long ld, int dtype) {
+    const int per = dtype == KP_F32 ? 4 : 8;
+    return ((size_t)p & 15) == 0 && ld % per == 0;
+}
+
+}  // namespace
+
+extern "C" {
+
+int kp_layer_norm_fwd(const void* x, long long ldx, const float* w, const float* b, float eps, void* y, long long ldy, float* mean,
+                      float* rstd, unsigned char* q, unsigned char* s, int fmt, long long rows, int C, int dtype, void* stream) {
+    KP_REQUIRE(dtype == KP_F32 || dtype == KP_BF16 || dtype == KP_F16, "kp_layer_norm_fwd: unknown dtype %d", dtype);
+    KP_REQUIRE(x && y && rows > 0 && C > 0 && (rows == 1 || (ldx >= C && ldy >= C)), "kp_layer_norm_fwd: bad args (%lld x %d, strides %lld, %lld)", rows, C, ldx, ldy);
+    KP_REQUIRE(eps >= 0.f && !mean == !rstd && !q == !s && (!q || fmt == KP_E4M3 || fmt == KP_E5M2), "kp_layer_norm_fwd: mean with rstd, q with s, a known format, eps >= 0");
+    const bool vec = ln_aligned(x, ldx, dtype) && ln_aligned(y, ldy, dtype) && ln_aligned(w, 4, KP_F32) && ln_aligned(b, 4, KP_F32) && (!q || (C % 8 == 0 && ((size_t)q & 7) == 0));
+    LnFwd P{x, w, b, y, mean, rstd, q, s, ldx, ldy, rows, C, (C + Q8_BLOCK - 1) / Q8_BLOCK, eps, vec};
+    const hipStream_t st = (hipStream_t)stream;
+    kp_count_bytes((double)rows * C * (2 * (dtype == KP_F32 ? 4 : 2) + (q ? 1 : 0)));
+    return dtype == KP_F32 ? fwd_type<KP_F32>(P, fmt, st) : dtype == KP_BF16 ? fwd_type<KP_BF16>(P, fmt, st) : fwd_type<KP_F16>(P, fmt, st);
+}
+
+long long kp_layer_norm_bwd_ws_floats(long long rows, int C) {
+    return rows > 0 && C > 0 ? (long long)ln_parts(rows, C) * 2 * C : 0;
+}
+
+int kp_layer_norm_bwd(const void* dy, long long lddy, const void* x, long long ldx, const unsigned char* q, const unsigned char* s, int fmt,
+                      const float* w, const float* mean, const float* rstd, void* dx, long long lddx, float* ws, float* dw, float* db,
+                      long long rows, int C, int dtype, void* stream) {
+    KP_REQUIRE(dtype == KP_F32 || dtype == KP_BF16 || dtype == KP_F16, "kp_layer_norm_bwd: unknown dtype %d", dtype);
+    KP_REQUIRE(dy && mean && rstd && (dx || dw || db) && rows > 0 && C > 0, "kp_layer_norm_bwd: bad args (%lld x %d)", rows, C);
+    KP_REQUIRE(rows == 1 || (lddy >= C && (!dx || lddx >= C) && (!x || ldx >= C)), "kp_layer_norm_bwd: row strides %lld, %lld, %lld for %d columns", lddy, ldx, lddx, C);
+    KP_REQUIRE((x != nullptr) != (q != nullptr) && !q == !s && (!q || fmt == KP_E4M3 || fmt == KP_E5M2), "kp_layer_norm_bwd: either x or its 8-bit form");
+    KP_REQUIRE(ws || !(dw || db), "kp_layer_norm_bwd: the weight's gradient needs a workspace (kp_layer_norm_bwd_ws_floats)");
+    const bool vec = ln_aligned(dy, lddy, dtype) && (!x || ln_aligned(x, ldx, dtype)) && (!dx || ln_aligned(dx, lddx, dtype)) && ln_aligned(w, 4, KP_F32) && (!q || (C % 8 == 0 && ((size_t)q & 7) == 0));
+    const int parts = ln_parts(rows, C);
+    LnBwd P{dy, x, q, s, w, mean, rstd, dx, (dw || db) ? ws : nullptr, lddy, ldx, lddx, rows, C, (C + Q8_BLOCK - 1) / Q8_BLOCK, vec};
+    const hipStream_t st = (hipStream_t)stream;
+    kp_count_bytes((double)rows * C * (2 * (dtype == KP_F32 ? 4 : 2) + (q ? 1 : (dtype == KP_F32 ? 4 : 2))));
+    const int rc = dtype == KP_F32 ? bwd_type<KP_F32>(P, fmt, parts, st) : dtype == KP_BF16 ? bwd_type<KP_BF16>(P, fmt, parts, st) : bwd_type<KP_F16>(P, fmt, parts, st);
+    if (rc != KP_OK || !(dw || db)) return rc;
+    ln_join_k<<<cdiv(2LL * C, 32), 1024, 0, st>>>(ws, dw, db, parts, C);
+    return kp_check_launch("layer_norm_bwd join");
+}
+
+}  // extern "C"

@@ -1,0 +1,356 @@
+// Products of two matrices in the 8-bit block format (kp_q8_dev.h): C[m][n] = sum_k A[m][k] B[n][k] (+ bias[n]), both operands in rows
+// along k, on the matrix instructions of gfx950.  Two ways to the same numbers:
+//
+//   16-bit results   the scaled 8-bit instruction.  It takes one exponent byte per operand row and 32 elements; a block of 128 hands the
+//                    same byte to its four parts, so scaling costs no arithmetic.  Its accumulator is fp32, but inside the instruction
+//                    the products of 8 neighbouring k are aligned to the largest of them and cut off below 2^-13 of it: a result is off
+//                    by less than 7 * 2^-13 of the sum of the groups' largest products (measured 1.4e-5 of the result's norm for normal
+//                    numbers, 6.6e-5 for wide-spread activations), which the rounding to 16 bits (2^-12 or 2^-9 an element) covers.
+//   fp32 results     e4m3 and e5m2 values times a power of two are exact in bfloat16 and so are their products in fp32: the elements are
+//                    converted on the way from LDS (exponent and all) and multiplied by the bfloat16 instruction, whose sums are fp32
+//                    sums (measured 6e-9 .. 4e-7 of the norm), at half its partner's rate.  Weight gradients go this way.
+//
+// Any order of the elements inside a block serves, as long as A and B agree: the fragments are read as the swizzle likes them.
+#include "kp_mfma_util.h"
+#include "kp_q8_dev.h"
+
+namespace {
+
+typedef int i32x8 __attribute__((ext_vector_type(8)));
+typedef float f32x4 __attribute__((ext_vector_type(4)));
+
+struct MmArgs {
+    const uint8_t *a, *sa, *b, *sb;
+    long long lda, ldsa, ldb, ldsb;
+    const float* bias;
+    void* c;
+    long long ldc;
+    float* part;                 // splits > 1: fp32 partial products [splits][M][N]
+    int M, N, nb;                // nb: blocks of 128 along k
+    int tiles_m, tiles_n, splits, per_split;   // per_split: blocks of a split, a multiple of 4
+    int dtype;
+};
+
+// every LDS access goes through types that may alias: the same bytes are written as fp32 or packed pairs and read as 16-byte pieces
+typedef u32x4 __attribute__((may_alias)) u32x4_a;
+typedef q8_u32x2 __attribute__((may_alias)) u32x2_a;
+typedef f32x4 __attribute__((may_alias)) f32x4_a;
+
+union Frag8 {
+    i32x8 v;
+    u32x4 h[2];
+};
+
+// fragment of 64 k-elements, half a row of 32 bytes a lane, and its conversion to bfloat16: 8 elements of piece `i`
+template <int F> __device__ __forceinline__ h16x8 q8_bf16x8(const i32x8& v, int i, float up) {
+    typedef __bf16 bf2 __attribute__((ext_vector_type(2)));
+    u32x4 r;
+#pragma unroll
+    for (int w = 0; w < 2; ++w)
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+            bf2 o;
+            if constexpr (F == 0) o = h ? __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(v[2 * i + w], up, true) : __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(v[2 * i + w], up, false);
+            else o = h ? __builtin_amdgcn_cvt_scalef32_pk_bf16_bf8(v[2 * i + w], up, true) : __builtin_amdgcn_cvt_scalef32_pk_bf16_bf8(v[2 * i + w], up, false);
+            r[2 * w + h] = __builtin_bit_cast(uint32_t, o);
+        }
+    return __builtin_bit_cast(h16x8, r);
+}
+
+// One output tile of BM x BN a workgroup, waves in a grid of WGM x WGN.  A step of 128 k-elements is staged through LDS by DMA (two buffers,
+// the next step's load in flight during this one); rows of 128 bytes, the 16-byte piece XOR-swizzled by the row pair on the DMA's source and
+// on the read, so that 16 lanes of a ds_read_b128 hit 16 different slots.  One barrier a step: fragments of a step's second half are read
+// under the first half's products, those of the next step's first half under the second's.  The operands are swapped (the instruction's
+// A = rows of B): a lane then holds 4 consecutive n of one m and the epilogue packs them.  Rows past the edge repeat the last row and are
+// not stored.  FA, FB: 0 e4m3, 1 e5m2.  F32: the bfloat16 way.
+template <int BM, int BN, int WGM, int WGN, int FA, int FB, bool F32>
+__global__ __launch_bounds__(64 * WGM * WGN, 2) void q8_mm_k(const MmArgs P) {
+    constexpr int NW = WGM * WGN, WM = BM / WGM, WN = BN / WGN, TM = WM / 32, TN = WN / 32;
+    constexpr int ABYTES = BM * 128, BBYTES = BN * 128, BUF = ABYTES + BBYTES;
+    constexpr int IA = BM / 8 / NW, IB = BN / 8 / NW;   // DMA instructions of 8 rows a wave and step
+    static_assert(NW * 32 * WN * 4 <= 2 * BUF, "epilogue staging");
+    __shared__ __attribute__((aligned(16))) uint8_t smem[2 * BUF];
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int wm = wave / WGN, wn = wave % WGN, fr = lane & 31, fh = lane >> 5;
+
+    // tile of this workgroup: an XCD (blockIdx % 8) takes a contiguous range of tiles, ordered in groups of 8 tile rows, so that the
+    // workgroups that share an L2 work on neighbouring tiles
+    const int tiles = P.tiles_m * P.tiles_n, total = tiles * P.splits;
+    const int xcd = blockIdx.x & 7, q = total >> 3, r = total & 7;
+    int id = xcd * q + (xcd < r ? xcd : r) + (blockIdx.x >> 3);
+    const int z = id / tiles;
+    id -= z * tiles;
+    const int per_group = 8 * P.tiles_n, group = id / per_group, first = group * 8;
+    const int gm = P.tiles_m - first < 8 ? P.tiles_m - first : 8;
+    const int rest = id - group * per_group;
+    const int m0 = (first + rest % gm) * BM, n0 = (rest / gm) * BN;
+    const int kb0 = z * P.per_split, kb1 = kb0 + P.per_split < P.nb ? kb0 + P.per_split : P.nb;
+
+    const auto ra = __builtin_amdgcn_make_buffer_rsrc((void*)(P.a + (long long)m0 * P.lda), 0, 0x7ffffffe, 0x00020000);
+    const auto rb = __builtin_amdgcn_make_buffer_rsrc((void*)(P.b + (long long)n0 * P.ldb), 0, 0x7ffffffe, 0x00020000);
+    const auto rsa = __builtin_amdgcn_make_buffer_rsrc((void*)(P.sa + (long long)m0 * P.ldsa), 0, 0x7ffffffe, 0x00020000);
+    const auto rsb = __builtin_amdgcn_make_buffer_rsrc((void*)(P.sb + (long long)n0 * P.ldsb), 0, 0x7ffffffe, 0x00020000);
+    const int last_m = P.M - 1 - m0, last_n = P.N - 1 - n0;
+
+    int va[IA], vb[IB];
+    const int lrow = lane >> 3, slot = lane & 7;
+#pragma unroll
+    for (int i = 0; i < IA; ++i) {
+        const int row = (i * NW + wave) * 8 + lrow;
+        va[i] = (row < last_m ? row : last_m) * (int)P.lda + ((slot ^ ((row >> 1) & 7)) << 4);
+    }
+#pragma unroll
+    for (int i = 0; i < IB; ++i) {
+        const int row = (i * NW + wave) * 8 + lrow;
+        vb[i] = (row < last_n ? row : last_n) * (int)P.ldb + ((slot ^ ((row >> 1) & 7)) << 4);
+    }
+    auto issue = [&](int buf, int kb) {
+        uint8_t* dst = smem + buf * BUF + wave * 1024;
+#pragma unroll
+        for (int i = 0; i < IA; ++i) dma16(ra, dst + i * NW * 1024, va[i], kb * 128);
+#pragma unroll
+        for (int i = 0; i < IB; ++i) dma16(rb, dst + ABYTES + i * NW * 1024, vb[i], kb * 128);
+    };
+    int vsa[TM], vsb[TN];
+#pragma unroll
+    for (int i = 0; i < TM; ++i) {
+        const int row = wm * WM + i * 32 + fr;
+        vsa[i] = (row < last_m ? row : last_m) * (int)P.ldsa;
+    }
+#pragma unroll
+    for (int i = 0; i < TN; ++i) {
+        const int row = wn * WN + i * 32 + fr;
+        vsb[i] = (row < last_n ? row : last_n) * (int)P.ldsb;
+    }
+    struct Scales { int a[TM], b[TN]; };   // exponent bytes of four consecutive blocks of this lane's rows
+    auto load_scales = [&](Scales& s, int kb) {
+#pragma unroll
+        for (int i = 0; i < TM; ++i) s.a[i] = __builtin_amdgcn_raw_buffer_load_b32(rsa, vsa[i], kb, 0);
+#pragma unroll
+        for (int i = 0; i < TN; ++i) s.b[i] = __builtin_amdgcn_raw_buffer_load_b32(rsb, vsb[i], kb, 0);
+    };
+
+    struct Frags { Frag8 a[TM], b[TN]; };
+    const int sw = (fr >> 1) & 7;
+    const int abase = (wm * WM + fr) * 128, bbase = ABYTES + (wn * WN + fr) * 128;
+    auto load_frags = [&](Frags& f, int buf, int kk) {
+        const uint8_t* base = smem + buf * BUF;
+#pragma unroll
+        for (int u = 0; u < 2; ++u) {
+            const int piece = ((kk * 4 + u * 2 + fh) ^ sw) << 4;
+#pragma unroll
+            for (int i = 0; i < TM; ++i) f.a[i].h[u] = *reinterpret_cast<const u32x4_a*>(base + abase + i * 4096 + piece);
+#pragma unroll
+            for (int i = 0; i < TN; ++i) f.b[i].h[u] = *reinterpret_cast<const u32x4_a*>(base + bbase + i * 4096 + piece);
+        }
+    };
+    f32x16 acc[TN][TM];
+#pragma unroll
+    for (int n = 0; n < TN; ++n)
+#pragma unroll
+        for (int m = 0; m < TM; ++m)
+#pragma unroll
+            for (int e = 0; e < 16; ++e) acc[n][m][e] = 0.f;
+    Scales sc, sc_next;
+    auto mma = [&](const Frags& f, auto J) {
+        constexpr int j = decltype(J)::value;
+        if constexpr (!F32) {
+#pragma unroll
+            for (int n = 0; n < TN; ++n)
+#pragma unroll
+                for (int m = 0; m < TM; ++m)
+                    acc[n][m] = __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(f.b[n].v, f.a[m].v, acc[n][m], FB, FA, j, sc.b[n], j, sc.a[m]);
+        } else {
+            typedef __bf16 bf8 __attribute__((ext_vector_type(8)));
+            float ua[TM], ub[TN];
+#pragma unroll
+            for (int m = 0; m < TM; ++m) ua[m] = q8_up(((uint32_t)sc.a[m] >> (8 * j)) & 255u);
+#pragma unroll
+            for (int n = 0; n < TN; ++n) ub[n] = q8_up(((uint32_t)sc.b[n] >> (8 * j)) & 255u);
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                bf8 xa[TM];
+#pragma unroll
+                for (int m = 0; m < TM; ++m) xa[m] = __builtin_bit_cast(bf8, q8_bf16x8<FA>(f.a[m].v, i, ua[m]));
+#pragma unroll
+                for (int n = 0; n < TN; ++n) {
+                    const bf8 xb = __builtin_bit_cast(bf8, q8_bf16x8<FB>(f.b[n].v, i, ub[n]));
+#pragma unroll
+                    for (int m = 0; m < TM; ++m) acc[n][m] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(xb, xa[m], acc[n][m], 0, 0, 0);
+                }
+            }
+        }
+    };
+
+    Frags f0, f1;
+    load_scales(sc, kb0);
+    issue(0, kb0);
+    if (kb0 + 1 < kb1) issue(1, kb0 + 1);
+    if (kb0 + 1 < kb1) wait_vm<IA + IB>();
+    else wait_vm<0>();
+    __builtin_amdgcn_s_barrier();
+    asm volatile("" ::: "memory");
+    load_frags(f0, 0, 0);
+    for (int kb = kb0; kb < kb1; kb += 4) {
+        static_for<0, 4>([&](auto J) {
+            constexpr int j = decltype(J)::value;
+            const int k = kb + j;
+            if (k < kb1) {
+                if constexpr (j == 0)
+                    if (kb + 4 < kb1) load_scales(sc_next, kb + 4);
+                load_frags(f1, j & 1, 1);
+                mma(f0, J);
+                if (k + 1 < kb1) {
+                    // this wave's reads of the buffer have returned and its part of the next step has arrived: behind the barrier that
+                    // holds for every wave, and the buffer takes the step after the next
+                    asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
+                    __builtin_amdgcn_s_barrier();
+                    asm volatile("" ::: "memory");
+                    if (k + 2 < kb1) issue(j & 1, k + 2);
+                    load_frags(f0, (j & 1) ^ 1, 0);
+                }
+                mma(f1, J);
+            }
+        });
+        sc = sc_next;
+    }
+    __syncthreads();
+
+    // epilogue: 32 rows of m at a time through a wave's own staging rows in LDS (16-byte pieces XOR-swizzled by the row), then whole rows
+    // of WN elements leave
+    uint8_t* stage = smem + wave * (32 * WN * 4);
+    const bool split = P.splits > 1;
+    const int nw = n0 + wn * WN;
+    auto store_rows = [&](auto DTC) {
+        constexpr int DT = decltype(DTC)::value, ES = el_size<DT>, ROW = WN * ES, PIECES = ROW / 16, PER = 16 / ES;
+        uint8_t* out = split ? (uint8_t*)(P.part + ((long long)z * P.M) * P.N) : (uint8_t*)P.c;
+        const long long ldc = split ? P.N : P.ldc;
+        const bool vec = ldc % PER == 0 && ((size_t)out & 15) == 0;
+#pragma unroll
+        for (int m = 0; m < TM; ++m) {
+#pragma unroll
+            for (int n = 0; n < TN; ++n)
+#pragma unroll
+                for (int g = 0; g < 4; ++g) {
+                    const int nn = n * 32 + g * 8 + fh * 4;
+                    float v[4];
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) {
+                        v[e] = acc[n][m][g * 4 + e];
+                        if (P.bias && !split && nw + nn + e < P.N) v[e] += P.bias[nw + nn + e];
+                    }
+                    const int off = nn * ES;
+                    uint8_t* p = stage + fr * ROW + (((off >> 4) ^ (fr & (PIECES - 1))) << 4) + (off & 15);
+                    if constexpr (DT == KP_F32) *reinterpret_cast<f32x4_a*>(p) = f32x4{v[0], v[1], v[2], v[3]};
+                    else *reinterpret_cast<u32x2_a*>(p) = q8_u32x2{el_pack<DT>(v[0], v[1]), el_pack<DT>(v[2], v[3])};
+                }
+#pragma unroll
+            for (int i = 0; i < 32 * PIECES / 64; ++i) {
+                const int p = i * 64 + lane, row = p / PIECES, piece = p % PIECES;
+                const u32x4 w = *reinterpret_cast<const u32x4_a*>(stage + row * ROW + ((piece ^ (row & (PIECES - 1))) << 4));
+                const int mm = m0 + wm * WM + m * 32 + row, nn = nw + piece * PER;
+                if (mm < P.M && nn < P.N) {
+                    uint8_t* dst = out + ((long long)mm * ldc + nn) * ES;
+                    if (vec && nn + PER <= P.N) *reinterpret_cast<u32x4*>(dst) = w;
+                    else {
+#pragma unroll
+                        for (int e = 0; e < PER; ++e)
+                            if (nn + e < P.N) {
+                                if constexpr (ES == 4) reinterpret_cast<uint32_t*>(dst)[e] = w[e];
+                                else reinterpret_cast<uint16_t*>(dst)[e] = (uint16_t)(w[e >> 1] >> (16 * (e & 1)));
+                            }
+                    }
+                }
+            }
+        }
+    };
+    if (split || P.dtype == KP_F32) store_rows(std::integral_constant<int, KP_F32>{});
+    else if (P.dtype == KP_BF16) store_rows(std::integral_constant<int, KP_BF16>{});
+    else store_rows(std::integral_constant<int, KP_F16>{});
+}
+
+// the splits' partial products, added in order, with the bias, rounded once
+template <int DT>
+__global__ __launch_bounds__(256) void q8_mm_join_k(const float* __restrict__ part, int splits, const float* __restrict__ bias,
+                                                    void* __restrict__ c, long long ldc, int M, int N) {
+    const long long total = (long long)M * N;
+    for (long long i = (long long)blockIdx.x * 256 + threadIdx.x; i < total; i += (long long)gridDim.x * 256) {
+        const long long m = i / N, n = i - m * N;
+        float v = part[i];
+        for (int z = 1; z < splits; ++z) v += part[z * total + i];
+        if (bias) v += bias[n];
+        el_store<DT>(c, m * ldc + n, v);
+    }
+}
+
+struct Plan { int bm, bn, splits, per_split; };
+
+// Tile and split from the sizes alone.
+Plan plan_of(int M, int N, int nb) {
+    Plan p;
+    p.bm = p.bn = (M > 128 && N > 128) ? 256 : (M > 64 && N > 64) ? 128 : 64;
+    const long long tiles = (long long)cdiv(M, p.bm) * cdiv(N, p.bn);
+    const int groups = (nb + 3) / 4;                 // splits start on multiples of four blocks (one word of exponent bytes)
+    int s = tiles >= 256 ? 1 : (int)(256 / tiles);
+    if (s > groups) s = groups;
+    if (s > 16) s = 16;
+    if (s < 1) s = 1;
+    p.per_split = (groups + s - 1) / s * 4;
+    p.splits = (nb + p.per_split - 1) / p.per_split;
+    return p;
+}
+
+template <int FA, int FB, bool F32> int mm_launch(const MmArgs& P, const Plan& p, hipStream_t st) {
+    const unsigned grid = (unsigned)(P.tiles_m * P.tiles_n * P.splits);
+    if (p.bm == 256) q8_mm_k<256, 256, 4, 2, FA, FB, F32><<<grid, 512, 0, st>>>(P);
+    else if (p.bm == 128) q8_mm_k<128, 128, 2, 2, FA, FB, F32><<<grid, 256, 0, st>>>(P);
+    else q8_mm_k<64, 64, 2, 2, FA, FB, F32><<<grid, 256, 0, st>>>(P);
+    return kp_check_launch("q8_matmul");
+}
+
+}  // namespace
+
+extern "C" {
+
+long long kp_q8_matmul_ws_floats(long long M, long long N, long long K) {
+    if (M <= 0 || N <= 0 || K <= 0 || M > 0x7fffff00LL || N > 0x7fffff00LL || K > (1LL << 23)) return 0;
+    const Plan p = plan_of((int)M, (int)N, (int)((K + Q8_BLOCK - 1) / Q8_BLOCK));
+    return p.splits > 1 ? p.splits * M * N : 0;
+}
+
+int kp_q8_matmul(const unsigned char* a, long long lda, const unsigned char* sa, long long ldsa, int fmta, const unsigned char* b,
+                 long long ldb, const unsigned char* sb, long long ldsb, int fmtb, const float* bias, void* c, long long ldc, float* ws,
+                 long long M, long long N, long long K, int dtype, void* stream) {
+    KP_REQUIRE(a && sa && b && sb && c && M > 0 && N > 0 && K > 0, "kp_q8_matmul: bad args (%lld x %lld x %lld)", M, N, K);
+    KP_REQUIRE((fmta == KP_E4M3 || fmta == KP_E5M2) && (fmtb == KP_E4M3 || fmtb == KP_E5M2), "kp_q8_matmul: unknown format %d / %d", fmta, fmtb);
+    KP_REQUIRE(dtype == KP_F32 || dtype == KP_BF16 || dtype == KP_F16, "kp_q8_matmul: unknown dtype %d", dtype);
+    const long long nb = (K + Q8_BLOCK - 1) / Q8_BLOCK, words = (nb + 3) / 4 * 4;
+    KP_REQUIRE(M <= 0x7fffff00LL && N <= 0x7fffff00LL && lda < (1LL << 23) && ldb < (1LL << 23),
+               "kp_q8_matmul: %lld x %lld x %lld is more than one call takes (2^23 along the product, 2^31 rows)", M, N, K);
+    KP_REQUIRE(lda >= nb * Q8_BLOCK && ldb >= nb * Q8_BLOCK && lda % 16 == 0 && ldb % 16 == 0 && ((size_t)a & 15) == 0 && ((size_t)b & 15) == 0,
+               "kp_q8_matmul: operand rows must be padded to whole blocks and start on multiples of 16 bytes (strides %lld, %lld)", lda, ldb);
+    KP_REQUIRE(ldsa >= words && ldsb >= words && ldsa % 4 == 0 && ldsb % 4 == 0 && ((size_t)sa & 3) == 0 && ((size_t)sb & 3) == 0,
+               "kp_q8_matmul: rows of exponent bytes must be padded to words (strides %lld, %lld)", ldsa, ldsb);
+    KP_REQUIRE(ldc >= N, "kp_q8_matmul: output row stride %lld for %lld columns", ldc, N);
+    const Plan p = plan_of((int)M, (int)N, (int)nb);
+    KP_REQUIRE(p.splits == 1 || ws, "kp_q8_matmul: this shape needs a workspace (kp_q8_matmul_ws_floats)");
+    MmArgs P;
+    P.a = a; P.sa = sa; P.b = b; P.sb = sb; P.lda = lda; P.ldsa = ldsa; P.ldb = ldb; P.ldsb = ldsb; P.bias = bias; P.c = c; P.ldc = ldc;
+    P.part = ws; P.M = (int)M; P.N = (int)N; P.nb = (int)nb; P.dtype = dtype;
+    P.tiles_m = (int)cdiv(M, p.bm); P.tiles_n = (int)cdiv(N, p.bn); P.splits = p.splits; P.per_split = p.per_split;
+    KP_REQUIRE((long long)P.tiles_m * P.tiles_n * P.splits < (1LL << 31), "kp_q8_matmul: %lld x %lld is more than one call takes", M, N);
+    kp_count_bytes((double)(M + N) * K + (double)M * N * (dtype == KP_F32 ? 4 : 2));
+    const hipStream_t st = (hipStream_t)stream;
+    int rc;
+    const int f = (fmta == KP_E5M2 ? 2 : 0) | (fmtb == KP_E5M2 ? 1 : 0);
+    if (dtype == KP_F32) rc = f == 0 ? mm_launch<0, 0, true>(P, p, st) : f == 1 ? mm_launch<0, 1, true>(P, p, st) : f == 2 ? mm_launch<1, 0, true>(P, p, st) : mm_launch<1, 1, true>(P, p, st);
+    else rc = f == 0 ? mm_launch<0, 0, false>(P, p, st) : f == 1 ? mm_launch<0, 1, false>(P, p, st) : f == 2 ? mm_launch<1, 0, false>(P, p, st) : mm_launch<1, 1, false>(P, p, st);
+    if (rc != KP_OK || p.splits == 1) return rc;
+    const unsigned grid = M * N > 256LL * 2048 ? 2048 : cdiv((size_t)(M * N), 256);
+    if (dtype == KP_F32) q8_mm_join_k<KP_F32><<<grid, 256, 0, st>>>(ws, p.splits, bias, c, ldc, (int)M, (int)N);
+    else if (dtype == KP_BF16) q8_mm_join_k<KP_BF16><<<grid, 256, 0, st>>>(ws, p.splits, bias, c, ldc, (int)M, (int)N);
+    else q8_mm_join_k<KP_F16><<<grid, 256, 0, st>>>(ws, p.splits, bias, c, ldc, (int)M, (int)N);
+    return kp_check_launch("q8_matmul join");
+}
+
+}  // extern "C"

@@ -1,0 +1,269 @@
+"""Tensors in 8 bits with a power-of-two scale for each block of 128 elements (include/kp_hip.h): activation checkpoints and matrix products.
+
+    kept = checkpoint8(x)                  # 1 byte an element (+ 1 / 128) instead of 2 or 4, between a forward and its backward
+    x = kept.unpack()
+
+    packed = pack8(weight)                 # once, for serving
+    y = linear8(x, packed, bias)
+    y = linear8(x, weight, bias)           # training: three 8-bit products a step; what it keeps of x IS the weight gradient's operand
+
+    c = matmul8(pack8(a), pack8(b))        # a @ b.T
+
+A block's scale is 2^s with the smallest s that brings the block's largest finite magnitude to at most 448 ('e4m3') or 57344 ('e5m2'); an
+element is rounded once, by at most 2^-4 ('e4m3') or 2^-3 ('e5m2') of itself (elements more than 2^14 / 2^29 below their block's largest lose
+more, down to zero).  Not-a-numbers stay what they are, so an overflowing fp16 step still reaches the loss scaler; infinities stay in
+'e5m2' and become not-a-numbers in 'e4m3'.
+"""
+from __future__ import annotations
+
+import torch
+from torch.autograd.function import once_differentiable
+
+from . import _lib
+from ._lib import call, ptr
+from .runtime import device_of, require_device, stream_ptr
+
+BLOCK = 128
+FORMATS = {'e4m3': _lib.KP_E4M3, 'e5m2': _lib.KP_E5M2}
+DTYPES = {torch.float32: _lib.KP_F32, torch.bfloat16: _lib.KP_BF16, torch.float16: _lib.KP_F16}
+
+
+def format_code(fmt: str) -> int:
+    if fmt not in FORMATS:
+        raise ValueError(f'format must be one of {sorted(FORMATS)}, not {fmt!r}')
+    return FORMATS[fmt]
+
+
+def dtype_code(dtype: torch.dtype) -> int:
+    if dtype not in DTYPES:
+        raise TypeError(f'{dtype} has no HIP kernel: float32, bfloat16 or float16')
+    return DTYPES[dtype]
+
+
+def as_rows(x: torch.Tensor):
+    """x [..., width] as (tensor, rows, row stride): x itself where its rows lie one stride apart (a column slice of a matrix does), else a
+    contiguous copy."""
+    width = x.shape[-1]
+    if x.dim() == 2 and (width <= 1 or x.stride(1) == 1) and x.stride(0) >= width:
+        return x, x.shape[0], x.stride(0)
+    x = x.contiguous()
+    return x, x.numel() // width, width
+
+
+class Packed8:
+    """A tensor in the 8-bit block format: `values` (bytes), `scales` (exponent bytes), the `shape` and `dtype` it stands for.
+
+    Operand form (pack8): values [rows][width rounded up to 128], scales [rows][blocks rounded up to 4], blocks along the last dimension.
+    Checkpoint form (checkpoint8, `flat`): the tensor's elements in memory order as one row, nothing padded; `stride` brings the order back."""
+
+    __slots__ = ('values', 'scales', 'shape', 'stride', 'dtype', 'fmt', 'flat')
+
+    def __init__(self, values, scales, shape, stride, dtype, fmt, flat):
+        self.values, self.scales, self.shape, self.stride = values, scales, shape, stride
+        self.dtype, self.fmt, self.flat = dtype, fmt, flat
+
+    @property
+    def nbytes(self) -> int:
+        return self.values.numel() + self.scales.numel()
+
+    def unpack(self, dtype: torch.dtype = None) -> torch.Tensor:
+        """The tensor again (in `dtype`, its own by default), each element rounded once to that type (to its largest number where the format
+        rounded a finite element past the type's range)."""
+        dtype = self.dtype if dtype is None else dtype
+        code = dtype_code(dtype)
+        v, s = self.values, self.scales
+        if self.flat:
+            y = torch.empty_strided(self.shape, self.stride, dtype=dtype, device=v.device)
+            rows, width, ldq, lds = 1, y.numel(), v.numel(), s.numel()
+        else:
+            y = torch.empty(self.shape, dtype=dtype, device=v.device)
+            rows, width, ldq, lds = v.shape[0], self.shape[-1], v.shape[1], s.shape[1]
+        if y.numel():
+            with device_of(v):
+                call('kp_q8_unpack', ptr(v), ldq, ptr(s), lds, ptr(y), width, rows, width, code, FORMATS[self.fmt], stream_ptr())
+        return y
+
+
+def _dense(x: torch.Tensor) -> bool:
+    """True if x's elements fill one run of memory in some order of its dimensions (channels_last, a transpose, ...)."""
+    if x.is_contiguous():
+        return True
+    run = 1
+    for stride, size in sorted((st, n) for st, n in zip(x.stride(), x.shape) if n > 1):
+        if stride != run:
+            return False
+        run *= size
+    return True
+
+
+def checkpoint8(x: torch.Tensor, fmt: str = 'e4m3') -> Packed8:
+    """x in 8 bits, to be kept between a forward and its backward: `.unpack()` gives it back with its shape, strides and type.  The blocks
+    run over the elements in memory order, across rows, whatever the shape; no gradient flows through it."""
+    code, dcode = format_code(fmt), dtype_code(x.dtype)
+    require_device(x)
+    if not _dense(x):
+        x = x.contiguous()
+    n = x.numel()
+    values = torch.empty(n, device=x.device, dtype=torch.uint8)
+    scales = torch.empty((n + BLOCK - 1) // BLOCK, device=x.device, dtype=torch.uint8)
+    if n:
+        with device_of(x):
+            call('kp_q8_pack', ptr(x), n, ptr(values), n, ptr(scales), scales.numel(), 1, n, dcode, code, stream_ptr())
+    return Packed8(values, scales, x.shape, x.stride(), x.dtype, fmt, True)
+
+
+def _form(rows, width, device):
+    """Empty operand form: values padded to whole blocks, exponent bytes to whole words."""
+    blocks = (width + BLOCK - 1) // BLOCK
+    return (torch.empty(rows, blocks * BLOCK, device=device, dtype=torch.uint8),
+            torch.empty(rows, (blocks + 3) // 4 * 4, device=device, dtype=torch.uint8))
+
+
+def pack8(x: torch.Tensor, fmt: str = 'e4m3') -> Packed8:
+    """x [..., width] as a product's operand, blocks along the last dimension.  No gradient flows through it (linear8 has its own)."""
+    code, dcode = format_code(fmt), dtype_code(x.dtype)
+    require_device(x)
+    if x.dim() < 1 or x.shape[-1] < 1:
+        raise ValueError(f'pack8: the last dimension must hold at least one element, got shape {tuple(x.shape)}')
+    m, rows, ld = as_rows(x.detach())
+    width = x.shape[-1]
+    values, scales = _form(rows, width, x.device)
+    if rows:
+        with device_of(x):
+            call('kp_q8_pack', ptr(m), ld, ptr(values), values.shape[1], ptr(scales), scales.shape[1], rows, width, dcode, code, stream_ptr())
+    return Packed8(values, scales, x.shape, None, x.dtype, fmt, False)
+
+
+def _pack_both(m, rows, ld, width, dcode, code, by_rows, by_cols, sums):
+    """kp_q8_pack_both of a matrix: (row form, column form, column sums), each (None, None) / None where not asked for."""
+    if not (by_rows or by_cols or sums):
+        return (None, None), (None, None), None
+    dev = m.device
+    q = _form(rows, width, dev) if by_rows else (None, None)
+    qt = _form(width, rows, dev) if by_cols else (None, None)
+    colsum = torch.empty(width, device=dev, dtype=torch.float32) if sums else None
+    ws = torch.empty(_lib.lib().kp_q8_pack_both_ws_floats(rows, width), device=dev, dtype=torch.float32) if sums else None
+    call('kp_q8_pack_both', ptr(m), ld, ptr(q[0]), q[0].shape[1] if by_rows else 0, ptr(q[1]), q[1].shape[1] if by_rows else 0,
+         ptr(qt[0]), qt[0].shape[1] if by_cols else 0, ptr(qt[1]), qt[1].shape[1] if by_cols else 0, ptr(ws), ptr(colsum),
+         rows, width, dcode, code, stream_ptr())
+    return q, qt, colsum
+
+
+def _product(a, fmta, b, fmtb, bias, shape, dtype):
+    """kp_q8_matmul of two operand forms (values, scales) into a new tensor of `shape` = [..., rows of b]."""
+    M, N, K = a[0].shape[0], b[0].shape[0], a[0].shape[1]
+    c = torch.empty(shape, device=a[0].device, dtype=dtype)
+    floats = _lib.lib().kp_q8_matmul_ws_floats(M, N, K)
+    ws = torch.empty(floats, device=c.device, dtype=torch.float32) if floats else None
+    call('kp_q8_matmul', ptr(a[0]), K, ptr(a[1]), a[1].shape[1], fmta, ptr(b[0]), K, ptr(b[1]), b[1].shape[1], fmtb, ptr(bias), ptr(c), N,
+         ptr(ws), M, N, K, DTYPES[dtype], stream_ptr())
+    return c
+
+
+def _check_bias(bias, width, device):
+    if bias is not None and (bias.shape != (width,) or bias.device != device or bias.dtype not in DTYPES):
+        raise ValueError(f'the bias must be a vector of {width} floats on {device}, got {tuple(bias.shape)} {bias.dtype} on {bias.device}')
+
+
+def matmul8(a: Packed8, b: Packed8, bias: torch.Tensor = None, dtype: torch.dtype = None) -> torch.Tensor:
+    """a @ b.T (+ bias) of two operand forms: a [..., k], b [n, k] -> [..., n] in `dtype` (a's by default), accumulated in fp32 and rounded
+    once.  The formats may differ."""
+    for name, p in (('a', a), ('b', b)):
+        if not isinstance(p, Packed8) or p.flat:
+            raise TypeError(f'matmul8: {name} must be a pack8 operand')
+    if len(b.shape) != 2 or a.shape[-1] != b.shape[-1]:
+        raise ValueError(f'matmul8: cannot multiply {tuple(a.shape)} with the transpose of {tuple(b.shape)}')
+    if a.values.device != b.values.device:
+        raise ValueError(f'matmul8: operands on {a.values.device} and {b.values.device}')
+    dtype = a.dtype if dtype is None else dtype
+    dtype_code(dtype)
+    _check_bias(bias, b.shape[0], a.values.device)
+    shape = (*a.shape[:-1], b.shape[0])
+    if a.values.shape[0] == 0 or b.shape[0] == 0:
+        return torch.empty(shape, device=a.values.device, dtype=dtype)
+    if bias is not None:
+        bias = bias.detach().to(torch.float32).contiguous()
+    with device_of(a.values):
+        return _product((a.values, a.scales), FORMATS[a.fmt], (b.values, b.scales), FORMATS[b.fmt], bias, shape, dtype)
+
+
+class _Linear8(torch.autograd.Function):
+    """y = P(x) P(w)^T + b;  dx = P(dy) P'(w),  dw = P'(dy)^T P'(x),  db = column sums of dy.  P: blocks along the product's inner index, P':
+    along the other one (w along its rows, x and dy along the batch), so that every product's operands have their blocks along its own
+    inner index.  P'(x) -- a byte an element -- is what waits for the backward, and P'(w)."""
+
+    @staticmethod
+    def forward(ctx, x, weight, bias, fmt, grad_fmt):
+        code, grad_code = FORMATS[fmt], FORMATS[grad_fmt]
+        m, rows, ld = as_rows(x)
+        N, K = weight.shape
+        shape = (*x.shape[:-1], N)
+        ctx.args = (x.shape, x.dtype, (N, K), weight.dtype, code, grad_code)
+        if rows == 0 or N == 0:
+            return torch.empty(shape, device=x.device, dtype=x.dtype)
+        need_x, need_w = ctx.needs_input_grad[:2]
+        with device_of(x):
+            w2, _, wld = as_rows(weight)
+            qx, qxt, _ = _pack_both(m, rows, ld, K, DTYPES[x.dtype], code, True, need_w, False)
+            qw, qwt, _ = _pack_both(w2, N, wld, K, DTYPES[weight.dtype], code, True, need_x, False)
+            ctx.save_for_backward(*qxt, *qwt)
+            return _product(qx, code, qw, code, bias, shape, x.dtype)
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, dy):
+        xshape, xdtype, wshape, wdtype, code, grad_code = ctx.args
+        need_x, need_w, need_b = ctx.needs_input_grad[:3]
+        N, dev = wshape[0], dy.device
+        if dy.numel() == 0:   # no rows, or no columns: nothing was launched
+            return (torch.zeros(xshape, device=dev, dtype=xdtype) if need_x else None,
+                    torch.zeros(wshape, device=dev, dtype=wdtype) if need_w else None,
+                    torch.zeros(N, device=dev, dtype=torch.float32) if need_b else None, None, None)
+        xv, xs, wv, ws = ctx.saved_tensors
+        m, rows, ld = as_rows(dy)
+        with device_of(dy):
+            qd, qdt, db = _pack_both(m, rows, ld, N, DTYPES[dy.dtype], grad_code, need_x, need_w, need_b)
+            dx = _product(qd, grad_code, (wv, ws), code, None, xshape, xdtype) if need_x else None
+            dw = _product(qdt, grad_code, (xv, xs), code, None, wshape, wdtype) if need_w else None
+        return dx, dw, db, None, None
+
+
+def linear8(x: torch.Tensor, weight, bias: torch.Tensor = None, fmt: str = 'e4m3', grad_fmt: str = 'e4m3') -> torch.Tensor:
+    """x [..., k] @ weight.T (+ bias) in 8-bit products: [..., n] in x's type.
+
+    weight a tensor [n, k] (fp32 master weights, or 16 bits): every call packs x and the weight in `fmt`; differentiable in x, weight and
+    bias.  The backward packs the output gradient in `grad_fmt` and takes dx and dw from two more 8-bit products; between the passes only
+    8-bit forms wait (a byte an element of x and of the weight).  Gradients come in the types of what they belong to.
+    weight a Packed8 (pack8): serving.  `fmt` is x's format; no gradient."""
+    require_device(x, bias)
+    code = format_code(fmt)
+    format_code(grad_fmt)
+    dtype_code(x.dtype)
+    packed = isinstance(weight, Packed8)
+    if packed and weight.flat:
+        raise TypeError('linear8: the weight must be a pack8 operand, not a checkpoint')
+    if not packed:
+        require_device(weight)
+        dtype_code(weight.dtype)
+    if len(weight.shape) != 2 or x.dim() < 1 or x.shape[-1] != weight.shape[1] or weight.shape[1] < 1:
+        raise ValueError(f'linear8: cannot multiply {tuple(x.shape)} with the transpose of {tuple(weight.shape)}')
+    dev = weight.values.device if packed else weight.device
+    if dev != x.device:
+        raise ValueError(f'linear8: x on {x.device}, the weight on {dev}')
+    N = weight.shape[0]
+    _check_bias(bias, N, x.device)
+    if bias is not None and (bias.dtype != torch.float32 or not bias.is_contiguous()):
+        bias = bias.to(torch.float32).contiguous()
+    if not packed:
+        return _Linear8.apply(x, weight, bias, fmt, grad_fmt)
+    if torch.is_grad_enabled() and (x.requires_grad or (bias is not None and bias.requires_grad)):
+        raise RuntimeError('linear8: a packed weight carries no gradient; pass the weight itself, or run under torch.no_grad()')
+    shape = (*x.shape[:-1], N)
+    m, rows, ld = as_rows(x)
+    if rows == 0 or N == 0:
+        return torch.empty(shape, device=x.device, dtype=x.dtype)
+    with device_of(x):
+        form = _form(rows, x.shape[-1], x.device)
+        call('kp_q8_pack', ptr(m), ld, ptr(form[0]), form[0].shape[1], ptr(form[1]), form[1].shape[1], rows, x.shape[-1],
+             DTYPES[x.dtype], code, stream_ptr())
+        return _product(form, code, (weight.values, weight.scales), FORMATS[weight.fmt], bias, shape, x.dtype)

@@ -1,0 +1,85 @@
+"""Layer norm over the last dimension (kp_layer_norm_*, include/kp_hip.h): the batch-independent normalisation beside the Units' BatchNorm --
+the same in training and inference, no running statistics, nothing to synchronise between ranks.
+
+    y = layer_norm(x, weight, bias)                  # x [..., C], fp32 / bf16 / fp16; weight, bias [C]
+    y = layer_norm(x, weight, bias, keep='e4m3')     # the backward reads x from an 8-bit copy the forward writes on its way
+"""
+from __future__ import annotations
+
+import torch
+from torch.autograd.function import once_differentiable
+
+from . import _lib
+from ._lib import call, ptr
+from .lowp import BLOCK, DTYPES, FORMATS, as_rows, dtype_code, format_code
+from .runtime import device_of, require_device, stream_ptr
+
+
+def _forward(x, weight, bias, eps, stats, fmt):
+    m, rows, ld = as_rows(x)
+    C = x.shape[-1]
+    y = torch.empty(x.shape, device=x.device, dtype=x.dtype)
+    mean = rstd = q = s = None
+    if stats:
+        mean, rstd = torch.empty(rows, device=x.device, dtype=torch.float32), torch.empty(rows, device=x.device, dtype=torch.float32)
+    if fmt:
+        q = torch.empty(rows, C, device=x.device, dtype=torch.uint8)
+        s = torch.empty(rows, (C + BLOCK - 1) // BLOCK, device=x.device, dtype=torch.uint8)
+    if rows:
+        with device_of(x):
+            call('kp_layer_norm_fwd', ptr(m), ld, ptr(weight), ptr(bias), eps, ptr(y), C, ptr(mean), ptr(rstd), ptr(q), ptr(s),
+                 FORMATS[fmt] if fmt else 0, rows, C, DTYPES[x.dtype], stream_ptr())
+    return y, m, ld, mean, rstd, q, s
+
+
+class _LayerNorm(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, x, weight, bias, eps, keep):
+        y, m, ld, mean, rstd, q, s = _forward(x, weight, bias, eps, True, keep)
+        ctx.args = (keep, ld)
+        ctx.save_for_backward(weight, mean, rstd, q if keep else m, s)
+        return y
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, dy):
+        keep, ldx = ctx.args
+        weight, mean, rstd, kept, s = ctx.saved_tensors
+        need_x, need_w, need_b = ctx.needs_input_grad[:3]
+        g, rows, ldg = as_rows(dy)
+        C, dev = dy.shape[-1], dy.device
+        f32 = dict(device=dev, dtype=torch.float32)
+        make = torch.empty if rows else torch.zeros   # (no rows: nothing is launched)
+        dx = torch.empty(dy.shape, device=dev, dtype=dy.dtype) if need_x else None
+        dw = make(C, **f32) if need_w else None
+        db = make(C, **f32) if need_b else None
+        if rows:
+            ws = torch.empty(_lib.lib().kp_layer_norm_bwd_ws_floats(rows, C), **f32) if need_w or need_b else None
+            with device_of(dy):
+                call('kp_layer_norm_bwd', ptr(g), ldg, None if keep else ptr(kept), C if keep else ldx, ptr(kept) if keep else None, ptr(s),
+                     FORMATS[keep] if keep else 0, ptr(weight), ptr(mean), ptr(rstd), ptr(dx), C, ptr(ws), ptr(dw), ptr(db),
+                     rows, C, DTYPES[dy.dtype], stream_ptr())
+        return dx, dw, db, None, None
+
+
+def layer_norm(x: torch.Tensor, weight: torch.Tensor = None, bias: torch.Tensor = None, eps: float = 1e-5, keep: str = None) -> torch.Tensor:
+    """(x - mean) / sqrt(variance + eps) * weight + bias over the last dimension, in x's type; statistics in fp32.  weight and bias are
+    vectors of x.shape[-1] floats or None.  keep: None -- the backward reads x itself -- or the 8-bit format ('e4m3', 'e5m2'; keypoints_amd.lowp)
+    in which a copy of x waits for it: half the memory of a 16-bit x, and the gradients of x and weight are those at the copy's values
+    (each off from x by at most 2^-4 / 2^-3 of itself)."""
+    require_device(x, weight, bias)
+    dtype_code(x.dtype)
+    if keep is not None:
+        format_code(keep)
+    if x.dim() < 1 or x.shape[-1] < 1:
+        raise ValueError(f'layer_norm: the last dimension must hold at least one element, got shape {tuple(x.shape)}')
+    eps = float(eps)
+    if not 0.0 <= eps < float('inf'):
+        raise ValueError(f'layer_norm: eps must be a number that is not negative, got {eps}')
+    for name, t in (('weight', weight), ('bias', bias)):
+        if t is not None and (t.shape != x.shape[-1:] or t.dtype not in DTYPES or t.device != x.device):
+            raise ValueError(f'layer_norm: {name} must be a vector of {x.shape[-1]} floats on {x.device}, got {tuple(t.shape)} {t.dtype} on {t.device}')
+    weight, bias = (t.to(torch.float32).contiguous() if t is not None else None for t in (weight, bias))
+    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (x, weight, bias)):
+        return _LayerNorm.apply(x, weight, bias, eps, keep)
+    return _forward(x, weight, bias, eps, False, None)[0]

@@ -1,6 +1,8 @@
 """Small host-side helpers shared by the op wrappers: device checks, stream handle, precision."""
 from __future__ import annotations
 
+import contextlib
+
 import torch
 
 from . import _lib
@@ -28,9 +30,17 @@ def precision_dtype(name: str):
     return _DTYPES[name]
 
 
+_HERE = contextlib.nullcontext()
+
+
 def stream_ptr() -> int:
     """hipStream_t of torch's current stream (kernels are enqueued there, never synchronised)."""
     return torch.cuda.current_stream().cuda_stream
+
+
+def device_of(t: torch.Tensor):
+    """Context in which torch's current device -- hence its current stream and the device a kernel is launched on -- is t's."""
+    return _HERE if t.device.index == torch.cuda.current_device() else torch.cuda.device(t.device)
 
 
 def require_device(*tensors) -> None:
