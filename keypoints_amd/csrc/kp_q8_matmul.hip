@@ -61,9 +61,10 @@ template <int F> __device__ __forceinline__ h16x8 q8_bf16x8(const i32x8& v, int 
 // the next step's load in flight during this one); rows of 128 bytes, the 16-byte piece XOR-swizzled by the row pair on the DMA's source and
 // on the read, so that 16 lanes of a ds_read_b128 hit 16 different slots.  One barrier a step: fragments of a step's second half are read
 // under the first half's products, those of the next step's first half under the second's.  The operands are swapped (the instruction's
-// A = rows of B): a lane then holds 4 consecutive n of one m and the epilogue packs them.  Rows past the edge repeat the last row and are
-// not stored.  FA, FB: 0 e4m3, 1 e5m2.  F32: the bfloat16 way.
-template <int BM, int BN, int WGM, int WGN, int FA, int FB, bool F32>
+// A = rows of B): a lane then holds 4 consecutive n of one m and the epilogue packs them.  Tiles at the far edges are moved back to end with
+// the matrix (the rows they share with their neighbours are computed twice, to the same values); EDGE: for matrices smaller than a tile,
+// rows past the end repeat the last one and are not stored.  FA, FB: 0 e4m3, 1 e5m2.  F32: the bfloat16 way.
+template <int BM, int BN, int WGM, int WGN, int FA, int FB, bool F32, bool EDGE>
 __global__ __launch_bounds__(64 * WGM * WGN, 2) void q8_mm_k(const MmArgs P) {
     constexpr int NW = WGM * WGN, WM = BM / WGM, WN = BN / WGN, TM = WM / 32, TN = WN / 32;
     constexpr int ABYTES = BM * 128, BBYTES = BN * 128, BUF = ABYTES + BBYTES;
@@ -83,65 +84,72 @@ __global__ __launch_bounds__(64 * WGM * WGN, 2) void q8_mm_k(const MmArgs P) {
     const int per_group = 8 * P.tiles_n, group = id / per_group, first = group * 8;
     const int gm = P.tiles_m - first < 8 ? P.tiles_m - first : 8;
     const int rest = id - group * per_group;
-    const int m0 = (first + rest % gm) * BM, n0 = (rest / gm) * BN;
+    int m0 = (first + rest % gm) * BM, n0 = (rest / gm) * BN;
+    if (!EDGE) {
+        m0 = m0 < P.M - BM ? m0 : P.M - BM;
+        n0 = n0 < P.N - BN ? n0 : P.N - BN;
+    }
     const int kb0 = z * P.per_split, kb1 = kb0 + P.per_split < P.nb ? kb0 + P.per_split : P.nb;
 
     const auto ra = __builtin_amdgcn_make_buffer_rsrc((void*)(P.a + (long long)m0 * P.lda), 0, 0x7ffffffe, 0x00020000);
     const auto rb = __builtin_amdgcn_make_buffer_rsrc((void*)(P.b + (long long)n0 * P.ldb), 0, 0x7ffffffe, 0x00020000);
     const auto rsa = __builtin_amdgcn_make_buffer_rsrc((void*)(P.sa + (long long)m0 * P.ldsa), 0, 0x7ffffffe, 0x00020000);
     const auto rsb = __builtin_amdgcn_make_buffer_rsrc((void*)(P.sb + (long long)n0 * P.ldsb), 0, 0x7ffffffe, 0x00020000);
+    const int lda = (int)P.lda, ldb = (int)P.ldb, ldsa = (int)P.ldsa, ldsb = (int)P.ldsb;
     const int last_m = P.M - 1 - m0, last_n = P.N - 1 - n0;
+    auto clamp = [](int row, int last) { return EDGE && row > last ? last : row; };
 
-    int va[IA], vb[IB];
+    // DMA instruction i of this wave fetches rows (i * NW + wave) * 8 .. + 7; its rows are i * NW * 8 below those of instruction 0, with the
+    // same swizzle, so one lane offset and a scalar one serve them all (EDGE: the clamped row is per lane)
     const int lrow = lane >> 3, slot = lane & 7;
+    constexpr int NA = EDGE ? IA : 1, NB = EDGE ? IB : 1;
+    int va[NA], vb[NB];
 #pragma unroll
-    for (int i = 0; i < IA; ++i) {
+    for (int i = 0; i < NA; ++i) {
         const int row = (i * NW + wave) * 8 + lrow;
-        va[i] = (row < last_m ? row : last_m) * (int)P.lda + ((slot ^ ((row >> 1) & 7)) << 4);
+        va[i] = clamp(row, last_m) * lda + ((slot ^ ((row >> 1) & 7)) << 4);
     }
 #pragma unroll
-    for (int i = 0; i < IB; ++i) {
+    for (int i = 0; i < NB; ++i) {
         const int row = (i * NW + wave) * 8 + lrow;
-        vb[i] = (row < last_n ? row : last_n) * (int)P.ldb + ((slot ^ ((row >> 1) & 7)) << 4);
+        vb[i] = clamp(row, last_n) * ldb + ((slot ^ ((row >> 1) & 7)) << 4);
     }
-    auto issue = [&](int buf, int kb) {
-        uint8_t* dst = smem + buf * BUF + wave * 1024;
+    auto issue = [&](int buf, int kb) {   // buf: byte offset of the buffer
+        uint8_t* dst = smem + buf + wave * 1024;
 #pragma unroll
-        for (int i = 0; i < IA; ++i) dma16(ra, dst + i * NW * 1024, va[i], kb * 128);
+        for (int i = 0; i < IA; ++i) dma16(ra, dst + i * NW * 1024, va[EDGE ? i : 0], kb * 128 + (EDGE ? 0 : i * NW * 8 * lda));
 #pragma unroll
-        for (int i = 0; i < IB; ++i) dma16(rb, dst + ABYTES + i * NW * 1024, vb[i], kb * 128);
+        for (int i = 0; i < IB; ++i) dma16(rb, dst + ABYTES + i * NW * 1024, vb[EDGE ? i : 0], kb * 128 + (EDGE ? 0 : i * NW * 8 * ldb));
     };
-    int vsa[TM], vsb[TN];
+    constexpr int NSA = EDGE ? TM : 1, NSB = EDGE ? TN : 1;
+    int vsa[NSA], vsb[NSB];
 #pragma unroll
-    for (int i = 0; i < TM; ++i) {
-        const int row = wm * WM + i * 32 + fr;
-        vsa[i] = (row < last_m ? row : last_m) * (int)P.ldsa;
-    }
+    for (int i = 0; i < NSA; ++i) vsa[i] = clamp(wm * WM + i * 32 + fr, last_m) * ldsa;
 #pragma unroll
-    for (int i = 0; i < TN; ++i) {
-        const int row = wn * WN + i * 32 + fr;
-        vsb[i] = (row < last_n ? row : last_n) * (int)P.ldsb;
-    }
-    struct Scales { int a[TM], b[TN]; };   // exponent bytes of four consecutive blocks of this lane's rows
+    for (int i = 0; i < NSB; ++i) vsb[i] = clamp(wn * WN + i * 32 + fr, last_n) * ldsb;
+    struct Scales { int a[TM], b[TN]; };   // exponent bytes of up to four consecutive blocks of this lane's rows, the current one lowest
     auto load_scales = [&](Scales& s, int kb) {
 #pragma unroll
-        for (int i = 0; i < TM; ++i) s.a[i] = __builtin_amdgcn_raw_buffer_load_b32(rsa, vsa[i], kb, 0);
+        for (int i = 0; i < TM; ++i) s.a[i] = __builtin_amdgcn_raw_buffer_load_b32(rsa, vsa[EDGE ? i : 0], kb + (EDGE ? 0 : i * 32 * ldsa), 0);
 #pragma unroll
-        for (int i = 0; i < TN; ++i) s.b[i] = __builtin_amdgcn_raw_buffer_load_b32(rsb, vsb[i], kb, 0);
+        for (int i = 0; i < TN; ++i) s.b[i] = __builtin_amdgcn_raw_buffer_load_b32(rsb, vsb[EDGE ? i : 0], kb + (EDGE ? 0 : i * 32 * ldsb), 0);
     };
 
     struct Frags { Frag8 a[TM], b[TN]; };
-    const int sw = (fr >> 1) & 7;
-    const int abase = (wm * WM + fr) * 128, bbase = ABYTES + (wn * WN + fr) * 128;
+    const int piece0 = (fh ^ ((fr >> 1) & 7)) << 4;
+    const int abase = (wm * WM + fr) * 128 + piece0, bbase = ABYTES + (wn * WN + fr) * 128 + piece0;
     auto load_frags = [&](Frags& f, int buf, int kk) {
-        const uint8_t* base = smem + buf * BUF;
 #pragma unroll
         for (int u = 0; u < 2; ++u) {
-            const int piece = ((kk * 4 + u * 2 + fh) ^ sw) << 4;
+            const int flip = (kk * 4 + u * 2) << 4;   // (16-byte piece (kk * 4 + u * 2 + fh) ^ swizzle)
+            int oa = abase + buf, ob = bbase + buf;
+            asm volatile("" : "+v"(oa), "+v"(ob));    // (formed here each time: hoisted, the eight addresses would cost registers)
+            const uint8_t* pa = smem + (oa ^ flip);
+            const uint8_t* pb = smem + (ob ^ flip);
 #pragma unroll
-            for (int i = 0; i < TM; ++i) f.a[i].h[u] = *reinterpret_cast<const u32x4_a*>(base + abase + i * 4096 + piece);
+            for (int i = 0; i < TM; ++i) f.a[i].h[u] = *reinterpret_cast<const u32x4_a*>(pa + i * 4096);
 #pragma unroll
-            for (int i = 0; i < TN; ++i) f.b[i].h[u] = *reinterpret_cast<const u32x4_a*>(base + bbase + i * 4096 + piece);
+            for (int i = 0; i < TN; ++i) f.b[i].h[u] = *reinterpret_cast<const u32x4_a*>(pb + i * 4096);
         }
     };
     f32x16 acc[TN][TM];
@@ -152,21 +160,20 @@ __global__ __launch_bounds__(64 * WGM * WGN, 2) void q8_mm_k(const MmArgs P) {
 #pragma unroll
             for (int e = 0; e < 16; ++e) acc[n][m][e] = 0.f;
     Scales sc, sc_next;
-    auto mma = [&](const Frags& f, auto J) {
-        constexpr int j = decltype(J)::value;
+    auto mma = [&](const Frags& f) {
         if constexpr (!F32) {
 #pragma unroll
             for (int n = 0; n < TN; ++n)
 #pragma unroll
                 for (int m = 0; m < TM; ++m)
-                    acc[n][m] = __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(f.b[n].v, f.a[m].v, acc[n][m], FB, FA, j, sc.b[n], j, sc.a[m]);
+                    acc[n][m] = __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(f.b[n].v, f.a[m].v, acc[n][m], FB, FA, 0, sc.b[n], 0, sc.a[m]);
         } else {
             typedef __bf16 bf8 __attribute__((ext_vector_type(8)));
             float ua[TM], ub[TN];
 #pragma unroll
-            for (int m = 0; m < TM; ++m) ua[m] = q8_up(((uint32_t)sc.a[m] >> (8 * j)) & 255u);
+            for (int m = 0; m < TM; ++m) ua[m] = q8_up((uint32_t)sc.a[m] & 255u);
 #pragma unroll
-            for (int n = 0; n < TN; ++n) ub[n] = q8_up(((uint32_t)sc.b[n] >> (8 * j)) & 255u);
+            for (int n = 0; n < TN; ++n) ub[n] = q8_up((uint32_t)sc.b[n] & 255u);
 #pragma unroll
             for (int i = 0; i < 4; ++i) {
                 bf8 xa[TM];
@@ -182,37 +189,58 @@ __global__ __launch_bounds__(64 * WGM * WGN, 2) void q8_mm_k(const MmArgs P) {
         }
     };
 
+    // keeps the products above where they are written, under the reads they cover: the compiler would sink them past the barrier and the
+    // branches behind it to the products below (an empty statement that names one register of each accumulator; nothing reads it)
+    auto pin = [&]() {
+#pragma unroll
+        for (int n = 0; n < TN; ++n)
+#pragma unroll
+            for (int m = 0; m < TM; ++m) asm volatile("" ::"v"(acc[n][m][0]));
+        __builtin_amdgcn_sched_barrier(0);
+    };
+
     Frags f0, f1;
     load_scales(sc, kb0);
+    sc_next = sc;
     issue(0, kb0);
-    if (kb0 + 1 < kb1) issue(1, kb0 + 1);
-    if (kb0 + 1 < kb1) wait_vm<IA + IB>();
-    else wait_vm<0>();
+    if (kb0 + 1 < kb1) {
+        issue(BUF, kb0 + 1);
+        wait_vm<IA + IB>();
+    } else wait_vm<0>();
     __builtin_amdgcn_s_barrier();
     asm volatile("" ::: "memory");
     load_frags(f0, 0, 0);
-    for (int kb = kb0; kb < kb1; kb += 4) {
-        static_for<0, 4>([&](auto J) {
-            constexpr int j = decltype(J)::value;
-            const int k = kb + j;
-            if (k < kb1) {
-                if constexpr (j == 0)
-                    if (kb + 4 < kb1) load_scales(sc_next, kb + 4);
-                load_frags(f1, j & 1, 1);
-                mma(f0, J);
-                if (k + 1 < kb1) {
-                    // this wave's reads of the buffer have returned and its part of the next step has arrived: behind the barrier that
-                    // holds for every wave, and the buffer takes the step after the next
-                    asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
-                    __builtin_amdgcn_s_barrier();
-                    asm volatile("" ::: "memory");
-                    if (k + 2 < kb1) issue(j & 1, k + 2);
-                    load_frags(f0, (j & 1) ^ 1, 0);
-                }
-                mma(f1, J);
-            }
-        });
-        sc = sc_next;
+    int buf = 0;
+#pragma unroll 1
+    for (int k = kb0; k < kb1; ++k) {
+        if constexpr (!F32) load_frags(f1, buf, 1);
+        __builtin_amdgcn_sched_barrier(0);
+        mma(f0);
+        pin();
+        if constexpr (F32) {   // (no registers for a second set beside the converted operands: the other wave of the SIMD covers the reads)
+            load_frags(f0, buf, 1);
+            mma(f0);
+            pin();
+        }
+        // this wave's reads of the buffer have returned and its part of the next step has arrived: behind the barrier that holds for every
+        // wave, and the buffer takes the step after the next.  (After the last step the fragments read here are never used.)
+        asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
+        __builtin_amdgcn_s_barrier();
+        asm volatile("" ::: "memory");
+        if (k + 2 < kb1) issue(buf, k + 2);
+        buf ^= BUF;
+        load_frags(f0, buf, 0);
+        __builtin_amdgcn_sched_barrier(0);
+        if constexpr (!F32) mma(f1);
+        pin();
+        if ((k & 3) == 3) sc = sc_next;     // (splits start on multiples of four blocks)
+        else {
+#pragma unroll
+            for (int i = 0; i < TM; ++i) sc.a[i] = (int)((uint32_t)sc.a[i] >> 8);
+#pragma unroll
+            for (int i = 0; i < TN; ++i) sc.b[i] = (int)((uint32_t)sc.b[i] >> 8);
+            if ((k & 3) == 0 && k + 4 < kb1) load_scales(sc_next, k + 4);
+        }
     }
     __syncthreads();
 
@@ -225,7 +253,7 @@ __global__ __launch_bounds__(64 * WGM * WGN, 2) void q8_mm_k(const MmArgs P) {
         constexpr int DT = decltype(DTC)::value, ES = el_size<DT>, ROW = WN * ES, PIECES = ROW / 16, PER = 16 / ES;
         uint8_t* out = split ? (uint8_t*)(P.part + ((long long)z * P.M) * P.N) : (uint8_t*)P.c;
         const long long ldc = split ? P.N : P.ldc;
-        const bool vec = ldc % PER == 0 && ((size_t)out & 15) == 0;
+        const bool vec = ldc % PER == 0 && nw % PER == 0 && ((size_t)out & 15) == 0;
 #pragma unroll
         for (int m = 0; m < TM; ++m) {
 #pragma unroll
@@ -288,7 +316,7 @@ struct Plan { int bm, bn, splits, per_split; };
 // Tile and split from the sizes alone.
 Plan plan_of(int M, int N, int nb) {
     Plan p;
-    p.bm = p.bn = (M > 128 && N > 128) ? 256 : (M > 64 && N > 64) ? 128 : 64;
+    p.bm = p.bn = (M >= 256 && N >= 256) ? 256 : (M >= 128 && N >= 128) ? 128 : 64;
     const long long tiles = (long long)cdiv(M, p.bm) * cdiv(N, p.bn);
     const int groups = (nb + 3) / 4;                 // splits start on multiples of four blocks (one word of exponent bytes)
     int s = tiles >= 256 ? 1 : (int)(256 / tiles);
@@ -302,9 +330,9 @@ Plan plan_of(int M, int N, int nb) {
 
 template <int FA, int FB, bool F32> int mm_launch(const MmArgs& P, const Plan& p, hipStream_t st) {
     const unsigned grid = (unsigned)(P.tiles_m * P.tiles_n * P.splits);
-    if (p.bm == 256) q8_mm_k<256, 256, 4, 2, FA, FB, F32><<<grid, 512, 0, st>>>(P);
-    else if (p.bm == 128) q8_mm_k<128, 128, 2, 2, FA, FB, F32><<<grid, 256, 0, st>>>(P);
-    else q8_mm_k<64, 64, 2, 2, FA, FB, F32><<<grid, 256, 0, st>>>(P);
+    if (p.bm == 256) q8_mm_k<256, 256, 4, 2, FA, FB, F32, false><<<grid, 512, 0, st>>>(P);
+    else if (p.bm == 128) q8_mm_k<128, 128, 2, 2, FA, FB, F32, false><<<grid, 256, 0, st>>>(P);
+    else q8_mm_k<64, 64, 2, 2, FA, FB, F32, true><<<grid, 256, 0, st>>>(P);
     return kp_check_launch("q8_matmul");
 }
 
