@@ -9,8 +9,8 @@
 //             order (fp64), so equal calls give equal bits
 //
 // Both are bound by memory.  A row is spread over G lanes, 8 consecutive elements (16 bytes of a 16-bit type) each, NJ times: the smallest
-// power of two that holds it up to a wave (rows of 64 elements: eight rows a wave), then a workgroup of 256 or 1024 threads with sums
-// through LDS, and beyond 16384 elements a workgroup that walks the row and reads it again.
+// power of two that holds it up to a wave (rows of 64 elements: eight rows a wave; a wave takes up to 1024), then 4, 8 or 16 waves with
+// sums through LDS, and beyond 16384 elements a workgroup that walks the row and reads it again.
 #include "kp_q8_dev.h"
 
 namespace {
@@ -33,204 +33,230 @@ template <int G> __device__ __forceinline__ uint32_t ln_block_max(uint32_t m) { 
     if constexpr (G >= 16) m = q8_umax(m, q8_dpp<0x128>(m));
     return m;
 }
-// `red`: one float a wave and call slot; every thread of the workgroup calls it
-template <int G> __device__ __forceinline__ float ln_sum(float v, float* red) {
-    v = ln_wave_sum<(G < 64 ? G : 64)>(v);
-    if constexpr (G > 64) {
-        if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = v;
-        __syncthreads();
-        v = 0.f;
+// sums of N values at once; `red`: N * (G / 64) * (rows a workgroup takes at once) floats that the workgroup's previous sum did not use
+// (every thread calls it; one barrier)
+template <int G, int N> __device__ __forceinline__ void ln_sums(float (&v)[N], float* red) {
 #pragma unroll
-        for (int w = 0; w < G / 64; ++w) v += red[w];
+    for (int i = 0; i < N; ++i) v[i] = ln_wave_sum<(G < 64 ? G : 64)>(v[i]);
+    if constexpr (G > 64) {
+        constexpr int W = G / 64;
+        const int wave = threadIdx.x >> 6, base = wave / W * W * N;
+        if ((threadIdx.x & 63) == 0)
+#pragma unroll
+            for (int i = 0; i < N; ++i) red[base + i * W + wave % W] = v[i];
+        __syncthreads();
+#pragma unroll
+        for (int i = 0; i < N; ++i) {
+            v[i] = 0.f;
+#pragma unroll
+            for (int w = 0; w < W; ++w) v[i] += red[base + i * W + w];
+        }
     }
-    return v;
 }
 
 struct LnFwd {
     const void* x; const float *w, *b; void* y; float *mean, *rstd; uint8_t *q, *s;
-    long long ldx, ldy, rows; int C, nb; float eps; bool vec;   // vec: all rows start on multiples of 16 bytes
+    long long ldx, ldy, rows; int C, nb; float eps;
 };
 struct LnBwd {
     const void *dy, *x; const uint8_t *q, *s; const float *w, *mean, *rstd; void* dx; float* part;
-    long long lddy, ldx, lddx, rows; int C, nb; bool vec;
+    long long lddy, ldx, lddx, rows; int C, nb;
 };
 
-template <int G> constexpr int ln_tpb = G > 256 ? G : 256;
+// A row's lanes: sub = thread % G, chunk j of 8 columns at (j * G + sub) * 8.  The next row's loads are in flight during this row's sums
+// (not in the backward of the widest rows, two chunks a lane in workgroups of 1024: the 128 registers a lane has there go to the sums).
+// A workgroup has 256 threads; past a wave 1024, so that the four rows of 256 lanes that are taken at once share one partial row of the
+// weight's gradient.
+template <int G> constexpr int ln_tpb = G > 64 ? 1024 : 256;
 
 // KEEP: 0, or KP_E4M3 / KP_E5M2: the row leaves in 8 bits too
 template <int DT, int G, int NJ, int KEEP>
 __global__ __launch_bounds__(ln_tpb<G>) void ln_fwd_k(const LnFwd P) {
     constexpr int TPB = ln_tpb<G>, R = TPB / G;
-    __shared__ float red[G > 64 ? 2 * (G / 64) : 1];
+    __shared__ float red[G > 64 ? 64 : 1];   // four sets of 16: two sums a row, alternating rows
     const int sub = threadIdx.x & (G - 1);
     const float inv = 1.f / (float)P.C;
     int n[NJ];
+    float w[NJ][8], b[NJ][8];
 #pragma unroll
     for (int j = 0; j < NJ; ++j) {
-        const int left = P.C - (j * G + sub) * 8;
+        const int c = (j * G + sub) * 8, left = P.C - c;
         n[j] = left < 0 ? 0 : (left < 8 ? left : 8);
+#pragma unroll
+        for (int k = 0; k < 8; ++k) { w[j][k] = 1.f; b[j][k] = 0.f; }
+        if (P.w) el_load8<KP_F32>(P.w, c, n[j], w[j]);
+        if (P.b) el_load8<KP_F32>(P.b, c, n[j], b[j]);
     }
-    for (long long r0 = (long long)blockIdx.x * R; r0 < P.rows; r0 += (long long)gridDim.x * R) {
-        const long long row = r0 + threadIdx.x / G;
+    const long long step = (long long)gridDim.x * R;
+    long long row = (long long)blockIdx.x * R + threadIdx.x / G;
+    El8<DT> next[NJ];
+#pragma unroll
+    for (int j = 0; j < NJ; ++j) next[j] = el_raw8_any<DT>(P.x, row * P.ldx + (j * G + sub) * 8, row < P.rows ? n[j] : 0);
+    for (long long r0 = (long long)blockIdx.x * R, odd = 0; r0 < P.rows; r0 += step, row += step, odd ^= 1) {
         const bool live = row < P.rows;
         float v[NJ][8];
-        float sum = 0.f;
+        float sum[1] = {0.f}, sq[1] = {0.f};
 #pragma unroll
         for (int j = 0; j < NJ; ++j) {
-            const long long at = row * P.ldx + (j * G + sub) * 8;
-            if (P.vec && n[j] == 8 && live) el_load8<DT>(P.x, at, v[j]);
-            else el_load8_part<DT>(P.x, at, live ? n[j] : 0, v[j]);
+            el_unpack8<DT>(next[j], v[j]);
+#pragma unroll
+            for (int k = 0; k < 8; ++k) sum[0] += v[j][k];
         }
 #pragma unroll
-        for (int j = 0; j < NJ; ++j)
-#pragma unroll
-            for (int k = 0; k < 8; ++k) sum += v[j][k];
-        const float mean = ln_sum<G>(sum, red) * inv;
-        float sq = 0.f;
+        for (int j = 0; j < NJ; ++j) next[j] = el_raw8_any<DT>(P.x, (row + step) * P.ldx + (j * G + sub) * 8, row + step < P.rows ? n[j] : 0);
+        float* slot = red + (G > 64 ? (odd ? 32 : 0) : 0);
+        ln_sums<G, 1>(sum, slot);
+        const float mean = sum[0] * inv;
 #pragma unroll
         for (int j = 0; j < NJ; ++j)
 #pragma unroll
             for (int k = 0; k < 8; ++k) {
                 const float d = k < n[j] ? v[j][k] - mean : 0.f;
-                sq = __builtin_fmaf(d, d, sq);
+                sq[0] = __builtin_fmaf(d, d, sq[0]);
             }
-        const float rstd = 1.f / sqrtf(ln_sum<G>(sq, red + (G > 64 ? G / 64 : 0)) * inv + P.eps);
+        ln_sums<G, 1>(sq, slot + (G > 64 ? 16 : 0));
+        const float rstd = 1.f / sqrtf(sq[0] * inv + P.eps);
 #pragma unroll
         for (int j = 0; j < NJ; ++j) {
             const int c = (j * G + sub) * 8;
             if constexpr (KEEP != 0) {
                 const uint32_t byte = q8_scale_byte<KEEP>(ln_block_max<G>(q8_mag8(v[j])));
                 if (live && n[j] > 0) {
-                    const q8_u32x2 o = q8_cvt8<KEEP>(v[j], q8_down(byte));
-                    if (P.vec && n[j] == 8) *reinterpret_cast<q8_u32x2*>(P.q + row * P.C + c) = o;
-                    else q8_store8_part(P.q + row * P.C + c, n[j], o);
+                    q8_store8(P.q + row * P.C + c, n[j], q8_cvt8<KEEP>(v[j], q8_down(byte)));
                     if ((c & (Q8_BLOCK - 1)) == 0) P.s[row * P.nb + c / Q8_BLOCK] = (uint8_t)byte;
                 }
             }
-            float w[8], b[8], o[8];
-            if (P.w) { if (P.vec && n[j] == 8) el_load8<KP_F32>(P.w, c, w); else el_load8_part<KP_F32>(P.w, c, n[j], w); }
-            if (P.b) { if (P.vec && n[j] == 8) el_load8<KP_F32>(P.b, c, b); else el_load8_part<KP_F32>(P.b, c, n[j], b); }
+            float o[8];
 #pragma unroll
-            for (int k = 0; k < 8; ++k) {
-                o[k] = (v[j][k] - mean) * rstd;
-                if (P.w) o[k] *= w[k];
-                if (P.b) o[k] += b[k];
-            }
-            if (live) {
-                if (P.vec && n[j] == 8) el_store8<DT>(P.y, row * P.ldy + c, o);
-                else el_store8_part<DT>(P.y, row * P.ldy + c, n[j], o);
-            }
+            for (int k = 0; k < 8; ++k) o[k] = (v[j][k] - mean) * rstd * w[j][k] + b[j][k];
+            if (live) el_store8<DT>(P.y, row * P.ldy + c, n[j], o);
         }
         if (P.mean && sub == 0 && live) {
             P.mean[row] = mean;
             P.rstd[row] = rstd;
         }
-        if constexpr (G > 64) __syncthreads();   // (the sums' slots are written again)
     }
 }
 
 template <int DT, int G, int NJ, int KEEP>
 __global__ __launch_bounds__(ln_tpb<G>) void ln_bwd_k(const LnBwd P) {
-    constexpr int TPB = ln_tpb<G>, R = TPB / G;
-    __shared__ float red[G > 64 ? 2 * (G / 64) : 1];
-    __shared__ float join[G < 256 ? 4 * (G < 64 ? G : 64) * 8 : 1];
+    constexpr int TPB = ln_tpb<G>, R = TPB / G, W = G < 64 ? G : 64;
+    __shared__ float red[G > 64 ? 64 : 1];                                     // two sets of 32: two sums at once, alternating rows
+    __shared__ float join[G == 1024 ? 1 : (G > 64 ? R * G * 8 : 4 * W * 8)];
     const int sub = threadIdx.x & (G - 1);
     const float inv = 1.f / (float)P.C;
     int n[NJ];
-    float dw[NJ][8], db[NJ][8];
+    float w[NJ][8], dw[NJ][8], db[NJ][8];
 #pragma unroll
     for (int j = 0; j < NJ; ++j) {
-        const int left = P.C - (j * G + sub) * 8;
+        const int c = (j * G + sub) * 8, left = P.C - c;
         n[j] = left < 0 ? 0 : (left < 8 ? left : 8);
 #pragma unroll
-        for (int k = 0; k < 8; ++k) dw[j][k] = db[j][k] = 0.f;
+        for (int k = 0; k < 8; ++k) { w[j][k] = 1.f; dw[j][k] = db[j][k] = 0.f; }
+        if (P.w) el_load8<KP_F32>(P.w, c, n[j], w[j]);
     }
-    for (long long r0 = (long long)blockIdx.x * R; r0 < P.rows; r0 += (long long)gridDim.x * R) {
-        const long long row = r0 + threadIdx.x / G;
+    constexpr bool PRE = !(G == 1024 && NJ == 2);
+    struct Row { El8<DT> dy[NJ], x[KEEP ? 1 : NJ]; q8_u32x2 q[KEEP ? NJ : 1]; uint32_t s[KEEP ? NJ : 1]; float mean, rstd; };
+    auto fetch = [&](Row& r, long long row) {
         const bool live = row < P.rows;
-        const float mean = live ? P.mean[row] : 0.f, rstd = live ? P.rstd[row] : 0.f;
-        float g[NJ][8], xh[NJ][8];
-        float a = 0.f, b = 0.f;
+        r.mean = live ? P.mean[row] : 0.f;
+        r.rstd = live ? P.rstd[row] : 0.f;
 #pragma unroll
         for (int j = 0; j < NJ; ++j) {
             const int c = (j * G + sub) * 8, m = live ? n[j] : 0;
             if constexpr (KEEP != 0) {
-                const float up = m > 0 ? q8_up(P.s[row * P.nb + c / Q8_BLOCK]) : 1.f;
-                if (P.vec && m == 8) q8_values8<KEEP>(*reinterpret_cast<const q8_u32x2*>(P.q + row * P.C + c), up, xh[j]);
-                else q8_values8<KEEP>(q8_load8_part(P.q + row * P.C + c, m), up, xh[j]);
-            } else {
-                if (P.vec && m == 8) el_load8<DT>(P.x, row * P.ldx + c, xh[j]);
-                else el_load8_part<DT>(P.x, row * P.ldx + c, m, xh[j]);
-            }
-            if (P.vec && m == 8) el_load8<DT>(P.dy, row * P.lddy + c, g[j]);
-            else el_load8_part<DT>(P.dy, row * P.lddy + c, m, g[j]);
+                r.s[j] = m > 0 ? P.s[row * P.nb + c / Q8_BLOCK] : 127u;
+                r.q[j] = q8_load8(P.q + row * P.C + c, m);
+            } else r.x[j] = el_raw8_any<DT>(P.x, row * P.ldx + c, m);
+            r.dy[j] = el_raw8_any<DT>(P.dy, row * P.lddy + c, m);
         }
+    };
+    const long long step = (long long)gridDim.x * R;
+    long long row = (long long)blockIdx.x * R + threadIdx.x / G;
+    Row next;
+    if constexpr (PRE) fetch(next, row);
+    for (long long r0 = (long long)blockIdx.x * R, odd = 0; r0 < P.rows; r0 += step, row += step, odd ^= 1) {
+        if constexpr (!PRE) fetch(next, row);
+        float g[NJ][8], xh[NJ][8];
+        const float mean = next.mean, rstd = next.rstd;
 #pragma unroll
         for (int j = 0; j < NJ; ++j) {
-            const int c = (j * G + sub) * 8;
-            float w[8];
-            if (P.w) { if (P.vec && n[j] == 8) el_load8<KP_F32>(P.w, c, w); else el_load8_part<KP_F32>(P.w, c, n[j], w); }
+            if constexpr (KEEP != 0) q8_values8<KEEP>(next.q[j], q8_up(next.s[j]), xh[j]);
+            else el_unpack8<DT>(next.x[j], xh[j]);
+            el_unpack8<DT>(next.dy[j], g[j]);
+        }
+        if constexpr (PRE) fetch(next, row + step);
+        float ab[2] = {0.f, 0.f};   // sums of g and of g xh; past the row's end g is zero
+#pragma unroll
+        for (int j = 0; j < NJ; ++j) {
+            if constexpr (!PRE)
+                if (P.w) el_load8<KP_F32>(P.w, (j * G + sub) * 8, n[j], w[0]);
 #pragma unroll
             for (int k = 0; k < 8; ++k) {
                 xh[j][k] = (xh[j][k] - mean) * rstd;
                 db[j][k] += g[j][k];
                 dw[j][k] = __builtin_fmaf(g[j][k], xh[j][k], dw[j][k]);
-                if (P.w) g[j][k] *= w[k];
-                a += g[j][k];                                      // (past the row's end g is zero)
-                b = __builtin_fmaf(g[j][k], xh[j][k], b);
+                g[j][k] *= w[PRE ? j : 0][k];
+                ab[0] += g[j][k];
+                ab[1] = __builtin_fmaf(g[j][k], xh[j][k], ab[1]);
             }
         }
-        a = ln_sum<G>(a, red) * inv;
-        b = ln_sum<G>(b, red + (G > 64 ? G / 64 : 0)) * inv;
-        if (P.dx && live) {
+        if (P.dx) {
+            ln_sums<G, 2>(ab, red + (G > 64 ? (odd ? 32 : 0) : 0));
+            const float a = ab[0] * inv, b = ab[1] * inv;
+            if (row < P.rows) {
 #pragma unroll
-            for (int j = 0; j < NJ; ++j) {
-                const int c = (j * G + sub) * 8;
-                float o[8];
+                for (int j = 0; j < NJ; ++j) {
+                    float o[8];
 #pragma unroll
-                for (int k = 0; k < 8; ++k) o[k] = rstd * (g[j][k] - a - xh[j][k] * b);
-                if (P.vec && n[j] == 8) el_store8<DT>(P.dx, row * P.lddx + c, o);
-                else el_store8_part<DT>(P.dx, row * P.lddx + c, n[j], o);
+                    for (int k = 0; k < 8; ++k) o[k] = rstd * (g[j][k] - a - xh[j][k] * b);
+                    el_store8<DT>(P.dx, row * P.lddx + (j * G + sub) * 8, n[j], o);
+                }
             }
         }
-        if constexpr (G > 64) __syncthreads();
     }
     if (!P.part) return;
-    // the workgroup's partial row [2][C]: first the groups of a wave (lanes with the same columns), then the waves
+    // the workgroup's partial row [2][C]: lanes of a wave with the same columns first, then the waves (or rows) that share them
     float* prow = P.part + (long long)blockIdx.x * 2 * P.C;
 #pragma unroll
     for (int which = 0; which < 2; ++which) {
         float (&acc)[NJ][8] = which ? db : dw;
 #pragma unroll
         for (int j = 0; j < NJ; ++j) {
-            const int c = (j * G + sub) * 8;
-            if constexpr (G < 256) {
-                constexpr int W = G < 64 ? G : 64;
+            float* dst = prow + which * P.C + (j * G + sub) * 8;
+            if constexpr (G == 1024) {
+#pragma unroll
+                for (int k = 0; k < 8; ++k)
+                    if (k < n[j]) dst[k] = acc[j][k];
+            } else {
+                constexpr int GL = G > 64 ? G : W, SETS = G > 64 ? R : 4;   // columns' lanes, copies of them in LDS
 #pragma unroll
                 for (int k = 0; k < 8; ++k) {
                     float s = acc[j][k];
 #pragma unroll
                     for (int o = W; o < 64; o <<= 1) s += __shfl_xor(s, o, 64);
-                    if ((threadIdx.x & 63) < W) join[((threadIdx.x >> 6) * W + sub) * 8 + k] = s;
+                    if (G > 64 || (threadIdx.x & 63) < W) join[((G > 64 ? threadIdx.x / G : threadIdx.x >> 6) * GL + sub) * 8 + k] = s;
                 }
                 __syncthreads();
-                if (threadIdx.x < W)
+                if (threadIdx.x < GL)
 #pragma unroll
                     for (int k = 0; k < 8; ++k)
                         if (k < n[j]) {
                             float s = 0.f;
 #pragma unroll
-                            for (int wv = 0; wv < 4; ++wv) s += join[(wv * W + sub) * 8 + k];
-                            prow[which * P.C + c + k] = s;
+                            for (int t = 0; t < SETS; ++t) s += join[(t * GL + sub) * 8 + k];
+                            dst[k] = s;
                         }
                 __syncthreads();
-            } else {
-#pragma unroll
-                for (int k = 0; k < 8; ++k)
-                    if (k < n[j]) prow[which * P.C + c + k] = acc[j][k];
             }
         }
     }
+}
+
+__device__ __forceinline__ float ln_total(float v, float* red) {   // over a workgroup of 1024
+    float t[1] = {v};
+    ln_sums<1024, 1>(t, red);
+    return t[0];
 }
 
 // Rows past 16384 elements: a workgroup walks the row, element by element and thread, and reads it again for each pass.
@@ -241,13 +267,13 @@ __global__ __launch_bounds__(1024) void ln_fwd_long_k(const LnFwd P) {
     for (long long row = blockIdx.x; row < P.rows; row += gridDim.x) {
         float sum = 0.f;
         for (int c = threadIdx.x; c < P.C; c += 1024) sum += el_load<DT>(P.x, row * P.ldx + c);
-        const float mean = ln_sum<1024>(sum, red) * inv;
+        const float mean = ln_total(sum, red) * inv;
         float sq = 0.f;
         for (int c = threadIdx.x; c < P.C; c += 1024) {
             const float d = el_load<DT>(P.x, row * P.ldx + c) - mean;
             sq = __builtin_fmaf(d, d, sq);
         }
-        const float rstd = 1.f / sqrtf(ln_sum<1024>(sq, red + 16) * inv + P.eps);
+        const float rstd = 1.f / sqrtf(ln_total(sq, red + 16) * inv + P.eps);
         for (int c = threadIdx.x; c < P.C; c += 1024) {
             float o = (el_load<DT>(P.x, row * P.ldx + c) - mean) * rstd;
             if (P.w) o *= P.w[c];
@@ -264,9 +290,9 @@ __global__ __launch_bounds__(1024) void ln_fwd_long_k(const LnFwd P) {
                 const int kb = b0 + (int)(threadIdx.x >> 4), c = kb * Q8_BLOCK + sub * 8;
                 const int n = P.C - c >= 8 ? 8 : (P.C > c ? P.C - c : 0);
                 float v[8];
-                el_load8_part<DT>(P.x, row * P.ldx + c, n, v);
+                el_load8<DT>(P.x, row * P.ldx + c, n, v);
                 const uint32_t byte = q8_scale_byte<KEEP>(q8_max16(q8_mag8(v)));
-                q8_store8_part(P.q + row * P.C + c, n, q8_cvt8<KEEP>(v, q8_down(byte)));
+                q8_store8(P.q + row * P.C + c, n, q8_cvt8<KEEP>(v, q8_down(byte)));
                 if (sub == 0 && kb < P.nb) P.s[row * P.nb + kb] = (uint8_t)byte;
             }
         }
@@ -293,8 +319,8 @@ __global__ __launch_bounds__(1024) void ln_bwd_long_k(const LnBwd P) {
             a += g;
             b = __builtin_fmaf(g, (ln_kept<DT, KEEP>(P, row, c) - mean) * rstd, b);
         }
-        a = ln_sum<1024>(a, red) * inv;
-        b = ln_sum<1024>(b, red + 16) * inv;
+        a = ln_total(a, red) * inv;
+        b = ln_total(b, red + 16) * inv;
         for (int c = threadIdx.x; c < P.C; c += 1024) {
             const float g = el_load<DT>(P.dy, row * P.lddy + c) * (P.w ? P.w[c] : 1.f);
             el_store<DT>(P.dx, row * P.lddx + c, rstd * (g - a - (ln_kept<DT, KEEP>(P, row, c) - mean) * rstd * b));
@@ -317,38 +343,20 @@ __global__ __launch_bounds__(256) void ln_cols_long_k(const LnBwd P) {
     prow[P.C + c] = db;
 }
 
-// the partial rows [parts][2][C] joined in a fixed order: 32 columns x 32 runs of parts a workgroup
-__global__ __launch_bounds__(1024) void ln_join_k(const float* __restrict__ part, float* __restrict__ dw, float* __restrict__ db, int parts,
-                                                  int C) {
-    __shared__ double red[32][33];
-    const int col = threadIdx.x & 31, run = threadIdx.x >> 5;
-    const long long c = (long long)blockIdx.x * 32 + col, width = 2LL * C;
-    double s = 0.0;
-    if (c < width)
-        for (int p = run; p < parts; p += 32) s += (double)part[p * width + c];
-    red[run][col] = s;
-    __syncthreads();
-    if (run == 0 && c < width) {
-        for (int k = 1; k < 32; ++k) s += red[k][col];
-        if (c < C) { if (dw) dw[c] = (float)s; }
-        else if (db) db[c - C] = (float)s;
-    }
-}
-
 // ---- which kernel -----------------------------------------------------------------------------------------------------------------
 constexpr int LONG = 16384;
 int ln_group(int C) {   // lanes of a row
-    if (C > 4096) return 1024;
-    if (C > 1024) return 256;
+    if (C > 1024) return C > 4096 ? 1024 : C > 2048 ? 512 : 256;
     int g = 1;
     while (g < 64 && g * 8 < C) g <<= 1;
     return g;
 }
-// workgroups of the backward: every one leaves a partial row of 2 C floats, which the join reads back
+int ln_rows(int C) { const int g = ln_group(C); return C > LONG ? 1 : (g > 64 ? 1024 : 256) / g; }   // rows a workgroup takes at once
+// workgroups of the backward: every one leaves a partial row of 2 C floats, which the join reads back.  Rows within a wave: 16 waves a CU,
+// short partial rows; wider ones: one workgroup of 16 waves a CU.
 int ln_parts(long long rows, int C) {
-    const int g = ln_group(C), per = C > LONG ? 1 : (g > 256 ? 1 : 256 / g);
-    const long long want = (rows + per - 1) / per;
-    const long long cap = C > LONG ? 64 : (C > 1024 ? 512 : 1024);
+    const int per = ln_rows(C);
+    const long long want = (rows + per - 1) / per, cap = C > LONG ? 64 : (ln_group(C) > 64 ? 256 : 1024);
     return (int)(want < cap ? want : cap);
 }
 
@@ -357,9 +365,9 @@ template <int DT, int KEEP> int fwd_launch(const LnFwd& P, hipStream_t st) {
         ln_fwd_long_k<DT, KEEP><<<(unsigned)(P.rows < 1024 ? P.rows : 1024), 1024, 0, st>>>(P);
         return kp_check_launch("layer_norm_fwd");
     }
-    const int g = ln_group(P.C), per = g > 256 ? 1 : 256 / g;
-    const long long want = (P.rows + per - 1) / per;
-    const unsigned grid = (unsigned)(want < 4096 ? want : 4096);
+    const int g = ln_group(P.C), per = ln_rows(P.C);
+    const long long want = (P.rows + per - 1) / per, cap = g > 64 ? 512 : 2048;
+    const unsigned grid = (unsigned)(want < cap ? want : cap);
 #define LN_FWD(G, NJ) ln_fwd_k<DT, G, NJ, KEEP><<<grid, ln_tpb<G>, 0, st>>>(P)
     switch (g) {
         case 1: LN_FWD(1, 1); break;
@@ -369,7 +377,8 @@ template <int DT, int KEEP> int fwd_launch(const LnFwd& P, hipStream_t st) {
         case 16: LN_FWD(16, 1); break;
         case 32: LN_FWD(32, 1); break;
         case 64: if (P.C <= 512) LN_FWD(64, 1); else LN_FWD(64, 2); break;
-        case 256: if (P.C <= 2048) LN_FWD(256, 1); else LN_FWD(256, 2); break;
+        case 256: LN_FWD(256, 1); break;
+        case 512: LN_FWD(512, 1); break;
         default: if (P.C <= 8192) LN_FWD(1024, 1); else LN_FWD(1024, 2); break;
     }
 #undef LN_FWD
@@ -390,7 +399,8 @@ template <int DT, int KEEP> int bwd_launch(const LnBwd& P, int parts, hipStream_
         case 16: LN_BWD(16, 1); break;
         case 32: LN_BWD(32, 1); break;
         case 64: if (P.C <= 512) LN_BWD(64, 1); else LN_BWD(64, 2); break;
-        case 256: if (P.C <= 2048) LN_BWD(256, 1); else LN_BWD(256, 2); break;
+        case 256: LN_BWD(256, 1); break;
+        case 512: LN_BWD(512, 1); break;
         default: if (P.C <= 8192) LN_BWD(1024, 1); else LN_BWD(1024, 2); break;
     }
 #undef LN_BWD
@@ -406,10 +416,6 @@ template <int DT> int bwd_type(const LnBwd& P, int fmt, int parts, hipStream_t s
     if (fmt == KP_E4M3) return bwd_launch<DT, KP_E4M3>(P, parts, st);
     return bwd_launch<DT, KP_E5M2>(P, parts, st);
 }
-bool ln_aligned(const void* p, long long ld, int dtype) {
-    const int per = dtype == KP_F32 ? 4 : 8;
-    return ((size_t)p & 15) == 0 && ld % per == 0;
-}
 
 }  // namespace
 
@@ -420,8 +426,7 @@ int kp_layer_norm_fwd(const void* x, long long ldx, const float* w, const float*
     KP_REQUIRE(dtype == KP_F32 || dtype == KP_BF16 || dtype == KP_F16, "kp_layer_norm_fwd: unknown dtype %d", dtype);
     KP_REQUIRE(x && y && rows > 0 && C > 0 && (rows == 1 || (ldx >= C && ldy >= C)), "kp_layer_norm_fwd: bad args (%lld x %d, strides %lld, %lld)", rows, C, ldx, ldy);
     KP_REQUIRE(eps >= 0.f && !mean == !rstd && !q == !s && (!q || fmt == KP_E4M3 || fmt == KP_E5M2), "kp_layer_norm_fwd: mean with rstd, q with s, a known format, eps >= 0");
-    const bool vec = ln_aligned(x, ldx, dtype) && ln_aligned(y, ldy, dtype) && ln_aligned(w, 4, KP_F32) && ln_aligned(b, 4, KP_F32) && (!q || (C % 8 == 0 && ((size_t)q & 7) == 0));
-    LnFwd P{x, w, b, y, mean, rstd, q, s, ldx, ldy, rows, C, (C + Q8_BLOCK - 1) / Q8_BLOCK, eps, vec};
+    LnFwd P{x, w, b, y, mean, rstd, q, s, ldx, ldy, rows, C, (C + Q8_BLOCK - 1) / Q8_BLOCK, eps};
     const hipStream_t st = (hipStream_t)stream;
     kp_count_bytes((double)rows * C * (2 * (dtype == KP_F32 ? 4 : 2) + (q ? 1 : 0)));
     return dtype == KP_F32 ? fwd_type<KP_F32>(P, fmt, st) : dtype == KP_BF16 ? fwd_type<KP_BF16>(P, fmt, st) : fwd_type<KP_F16>(P, fmt, st);
@@ -439,14 +444,13 @@ int kp_layer_norm_bwd(const void* dy, long long lddy, const void* x, long long l
     KP_REQUIRE(rows == 1 || (lddy >= C && (!dx || lddx >= C) && (!x || ldx >= C)), "kp_layer_norm_bwd: row strides %lld, %lld, %lld for %d columns", lddy, ldx, lddx, C);
     KP_REQUIRE((x != nullptr) != (q != nullptr) && !q == !s && (!q || fmt == KP_E4M3 || fmt == KP_E5M2), "kp_layer_norm_bwd: either x or its 8-bit form");
     KP_REQUIRE(ws || !(dw || db), "kp_layer_norm_bwd: the weight's gradient needs a workspace (kp_layer_norm_bwd_ws_floats)");
-    const bool vec = ln_aligned(dy, lddy, dtype) && (!x || ln_aligned(x, ldx, dtype)) && (!dx || ln_aligned(dx, lddx, dtype)) && ln_aligned(w, 4, KP_F32) && (!q || (C % 8 == 0 && ((size_t)q & 7) == 0));
     const int parts = ln_parts(rows, C);
-    LnBwd P{dy, x, q, s, w, mean, rstd, dx, (dw || db) ? ws : nullptr, lddy, ldx, lddx, rows, C, (C + Q8_BLOCK - 1) / Q8_BLOCK, vec};
+    LnBwd P{dy, x, q, s, w, mean, rstd, dx, (dw || db) ? ws : nullptr, lddy, ldx, lddx, rows, C, (C + Q8_BLOCK - 1) / Q8_BLOCK};
     const hipStream_t st = (hipStream_t)stream;
     kp_count_bytes((double)rows * C * (2 * (dtype == KP_F32 ? 4 : 2) + (q ? 1 : (dtype == KP_F32 ? 4 : 2))));
     const int rc = dtype == KP_F32 ? bwd_type<KP_F32>(P, fmt, parts, st) : dtype == KP_BF16 ? bwd_type<KP_BF16>(P, fmt, parts, st) : bwd_type<KP_F16>(P, fmt, parts, st);
     if (rc != KP_OK || !(dw || db)) return rc;
-    ln_join_k<<<cdiv(2LL * C, 32), 1024, 0, st>>>(ws, dw, db, parts, C);
+    q8_join_k<<<cdiv(2LL * C, 16), 1024, 0, st>>>(ws, parts, 2LL * C, dw, C, db);
     return kp_check_launch("layer_norm_bwd join");
 }
 

@@ -5,31 +5,45 @@
 namespace {
 
 constexpr int TPB = 256;
+typedef q8_u32x2 __attribute__((may_alias)) q8_u32x2_a;   // (LDS is written as pairs of words and read as 16-byte pieces)
+typedef q8_u32x4 __attribute__((may_alias)) q8_u32x4_a;
 
-// A group of 16 lanes takes a block: 8 consecutive elements a lane, the block's maximum by DPP.  VEC: the rows start on multiples of 16
-// bytes; otherwise element loads.  `padded`: the row's last block is written out to its full 128 bytes with zeros.
-template <int DT, int FMT, bool VEC>
+// A group of 16 lanes takes a block: 8 consecutive elements a lane, the block's maximum by DPP; UNROLL blocks of a thread in flight.
+// `padded`: the row's last block is written out to its full 128 bytes with zeros.
+constexpr int UNROLL = 2;
+struct BlockAt { unsigned row, kb; long long c; int n; };   // n: elements of this lane's 8 that the row has
+__device__ __forceinline__ BlockAt block_at(unsigned b, unsigned nb, unsigned total, long long cols, int sub) {
+    BlockAt r;
+    r.row = b < total ? b / nb : 0;
+    r.kb = b < total ? b - r.row * nb : 0;
+    r.c = (long long)r.kb * Q8_BLOCK + sub * 8;
+    r.n = b >= total ? 0 : (cols - r.c >= 8 ? 8 : (cols > r.c ? (int)(cols - r.c) : 0));
+    return r;
+}
+template <int DT, int FMT>
 __global__ __launch_bounds__(TPB) void q8_pack_k(const void* __restrict__ x, long long ldx, uint8_t* __restrict__ q, long long ldq,
                                                  uint8_t* __restrict__ s, long long lds, unsigned nb, unsigned total, long long cols,
                                                  int padded) {
     const int sub = threadIdx.x & 15;
-    const unsigned stride = gridDim.x * (TPB / 16);
-    for (unsigned b0 = blockIdx.x * (TPB / 16); b0 < total; b0 += stride) {
-        const unsigned b = b0 + (threadIdx.x >> 4);
-        const bool live = b < total;
-        const unsigned row = live ? b / nb : 0, kb = live ? b - row * nb : 0;
-        const long long c = (long long)kb * Q8_BLOCK + sub * 8;
-        const int n = !live ? 0 : (cols - c >= 8 ? 8 : (cols > c ? (int)(cols - c) : 0));
-        float v[8];
-        if (VEC && n == 8) el_load8<DT>(x, row * ldx + c, v);
-        else el_load8_part<DT>(x, row * ldx + c, n, v);
-        const uint32_t byte = q8_scale_byte<FMT>(q8_max16(q8_mag8(v)));
-        if (!live) continue;
-        const q8_u32x2 r = q8_cvt8<FMT>(v, q8_down(byte));
-        uint8_t* dst = q + row * ldq + c;
-        if (padded || (VEC && n == 8)) *reinterpret_cast<q8_u32x2*>(dst) = r;
-        else q8_store8_part(dst, n, r);
-        if (sub == 0) s[row * lds + kb] = (uint8_t)byte;
+    const unsigned per = TPB / 16, stride = gridDim.x * per * UNROLL;
+    for (unsigned b0 = blockIdx.x * per * UNROLL; b0 < total; b0 += stride) {
+        BlockAt at[UNROLL];
+        El8<DT> raw[UNROLL];
+#pragma unroll
+        for (int u = 0; u < UNROLL; ++u) {
+            at[u] = block_at(b0 + u * per + (threadIdx.x >> 4), nb, total, cols, sub);
+            raw[u] = el_raw8_any<DT>(x, at[u].row * ldx + at[u].c, at[u].n);
+        }
+#pragma unroll
+        for (int u = 0; u < UNROLL; ++u) {
+            float v[8];
+            el_unpack8<DT>(raw[u], v);
+            const uint32_t byte = q8_scale_byte<FMT>(q8_max16(q8_mag8(v)));
+            if (b0 + u * per + (threadIdx.x >> 4) < total) {
+                q8_store8(q + at[u].row * ldq + at[u].c, padded ? 8 : at[u].n, q8_cvt8<FMT>(v, q8_down(byte)));
+                if (sub == 0) s[at[u].row * lds + at[u].kb] = (uint8_t)byte;
+            }
+        }
     }
 }
 
@@ -48,41 +62,42 @@ template <int DT, int FMT> __device__ __forceinline__ void q8_unpack8(q8_u32x2 q
         v[k] = fabsf(v[k]) >= __uint_as_float((uint32_t)(127 + RANGE - 4) << 23) && fabsf(v[k]) < __builtin_inff() ? copysignf(largest, v[k]) : v[k] * 16.f;
 }
 
-template <int DT, int FMT, bool VEC>
+template <int DT, int FMT>
 __global__ __launch_bounds__(TPB) void q8_unpack_k(const uint8_t* __restrict__ q, long long ldq, const uint8_t* __restrict__ s,
                                                    long long lds, void* __restrict__ y, long long ldy, unsigned nb, unsigned total,
                                                    long long cols) {
     const int sub = threadIdx.x & 15;
-    const unsigned stride = gridDim.x * (TPB / 16);
-    for (unsigned b = blockIdx.x * (TPB / 16) + (threadIdx.x >> 4); b < total; b += stride) {
-        const unsigned row = b / nb, kb = b - row * nb;
-        const long long c = (long long)kb * Q8_BLOCK + sub * 8;
-        const int n = cols - c >= 8 ? 8 : (cols > c ? (int)(cols - c) : 0);
-        if (n == 0) continue;
-        const uint32_t byte = s[row * lds + kb];
-        float v[8];
-        if (VEC && n == 8) {
-            q8_unpack8<DT, FMT>(*reinterpret_cast<const q8_u32x2*>(q + row * ldq + c), byte, v);
-            el_store8<DT>(y, row * ldy + c, v);
-        } else {
-            q8_unpack8<DT, FMT>(q8_load8_part(q + row * ldq + c, n), byte, v);
-            el_store8_part<DT>(y, row * ldy + c, n, v);
+    const unsigned per = TPB / 16, stride = gridDim.x * per * UNROLL;
+    for (unsigned b0 = blockIdx.x * per * UNROLL; b0 < total; b0 += stride) {
+        BlockAt at[UNROLL];
+        q8_u32x2 raw[UNROLL];
+        uint32_t byte[UNROLL];
+#pragma unroll
+        for (int u = 0; u < UNROLL; ++u) {
+            at[u] = block_at(b0 + u * per + (threadIdx.x >> 4), nb, total, cols, sub);
+            raw[u] = q8_load8(q + at[u].row * ldq + at[u].c, at[u].n);
+            byte[u] = s[at[u].row * lds + at[u].kb];
+        }
+#pragma unroll
+        for (int u = 0; u < UNROLL; ++u) {
+            float v[8];
+            q8_unpack8<DT, FMT>(raw[u], byte[u], v);
+            el_store8<DT>(y, at[u].row * ldy + at[u].c, at[u].n, v);
         }
     }
 }
 
 // Rows and columns at once, a 128 x 128 tile of x a workgroup: a thread holds 8 rows x 8 columns (rows 8 g .. 8 g + 7 with g = thread / 16,
 // columns 8 (thread % 16) ..), so that a row's block is a DPP row of lanes and a column's block the 16 values of g: four in the wave, four
-// waves through LDS.  The column form leaves through LDS as 16-byte pieces along the rows.  Tiles at the matrix's edge read zeros beyond
-// it, and both forms are written to full 128-byte blocks.  With colsum: the tile's column sums, one fp32 row a tile row (summed in a
-// fixed order by q8_colsum_k).
-template <int DT, int FMT, bool VEC>
+// waves through LDS.  The column form leaves through LDS as 16-byte pieces along the rows (rows of 128 bytes, the piece XOR-swizzled by the
+// column's octet: the eight columns that differ in it hit different banks).  Tiles at the matrix's edge read zeros beyond it, and both
+// forms are written to full 128-byte blocks.  With colsum: the tile's column sums, one fp32 row a tile row (joined by q8_join_k).
+template <int DT, int FMT>
 __global__ __launch_bounds__(TPB) void q8_pack_both_k(const void* __restrict__ x, long long ldx, uint8_t* __restrict__ q, long long ldq,
                                                       uint8_t* __restrict__ s, long long lds, uint8_t* __restrict__ qt, long long ldqt,
                                                       uint8_t* __restrict__ st, long long ldst, float* __restrict__ colsum,
                                                       long long rows, long long cols) {
-    constexpr int PITCH = 144;                      // bytes of an LDS row of the column form (16 more than a block: spread over the banks)
-    __shared__ __attribute__((aligned(16))) uint8_t tile[128 * PITCH];
+    __shared__ __attribute__((aligned(16))) uint8_t tile[128 * 128];
     __shared__ uint32_t wmax[4][128];
     __shared__ float wsum[4][128];
     const int t = threadIdx.x, cv = t & 15, g = t >> 4, wave = t >> 6;
@@ -90,11 +105,7 @@ __global__ __launch_bounds__(TPB) void q8_pack_both_k(const void* __restrict__ x
     const int n = cols - c0 >= 8 ? 8 : (cols > c0 ? (int)(cols - c0) : 0);
     float v[8][8];
 #pragma unroll
-    for (int j = 0; j < 8; ++j) {
-        const bool in = r0 + j < rows;
-        if (VEC && n == 8 && in) el_load8<DT>(x, (r0 + j) * ldx + c0, v[j]);
-        else el_load8_part<DT>(x, (r0 + j) * ldx + c0, in ? n : 0, v[j]);
-    }
+    for (int j = 0; j < 8; ++j) el_load8<DT>(x, (r0 + j) * ldx + c0, r0 + j < rows ? n : 0, v[j]);
     if (q) {
 #pragma unroll
         for (int j = 0; j < 8; ++j) {
@@ -107,26 +118,27 @@ __global__ __launch_bounds__(TPB) void q8_pack_both_k(const void* __restrict__ x
     }
     if (!qt && !colsum) return;
     uint32_t m[8];
-    float sum[8];
 #pragma unroll
     for (int k = 0; k < 8; ++k) {
         m[k] = 0;
-        sum[k] = 0.f;
 #pragma unroll
-        for (int j = 0; j < 8; ++j) {
-            m[k] = q8_umax(m[k], q8_mag(v[j][k]));
-            sum[k] += v[j][k];
-        }
+        for (int j = 0; j < 8; ++j) m[k] = q8_umax(m[k], q8_mag(v[j][k]));
         m[k] = q8_umax(m[k], (uint32_t)__shfl_xor((int)m[k], 16, 64));
         m[k] = q8_umax(m[k], (uint32_t)__shfl_xor((int)m[k], 32, 64));
-        sum[k] += __shfl_xor(sum[k], 16, 64);
-        sum[k] += __shfl_xor(sum[k], 32, 64);
     }
     if ((t & 63) < 16) {
 #pragma unroll
+        for (int k = 0; k < 8; ++k) wmax[wave][cv * 8 + k] = m[k];
+    }
+    if (colsum) {
+#pragma unroll
         for (int k = 0; k < 8; ++k) {
-            wmax[wave][cv * 8 + k] = m[k];
-            wsum[wave][cv * 8 + k] = sum[k];
+            float sum = 0.f;
+#pragma unroll
+            for (int j = 0; j < 8; ++j) sum += v[j][k];
+            sum += __shfl_xor(sum, 16, 64);
+            sum += __shfl_xor(sum, 32, 64);
+            if ((t & 63) < 16) wsum[wave][cv * 8 + k] = sum;
         }
     }
     __syncthreads();
@@ -140,64 +152,44 @@ __global__ __launch_bounds__(TPB) void q8_pack_both_k(const void* __restrict__ x
         float col[8];
 #pragma unroll
         for (int j = 0; j < 8; ++j) col[j] = v[j][k];
-        *reinterpret_cast<q8_u32x2*>(tile + c * PITCH + g * 8) = q8_cvt8<FMT>(col, q8_down(byte));
+        *reinterpret_cast<q8_u32x2_a*>(tile + c * 128 + (((g >> 1) ^ (cv & 7)) << 4) + (g & 1) * 8) = q8_cvt8<FMT>(col, q8_down(byte));
         if (g == 0 && c0 + k < cols) st[(c0 + k) * ldst + blockIdx.y] = (uint8_t)byte;
     }
     __syncthreads();
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
-        const int id = i * TPB + t, c = id >> 3, piece = (id & 7) * 16;
+        const int id = i * TPB + t, c = id >> 3, piece = id & 7;
         const long long col = (long long)blockIdx.x * 128 + c;
         if (col < cols)
-            *reinterpret_cast<q8_u32x4*>(qt + col * ldqt + (long long)blockIdx.y * 128 + piece) =
-                *reinterpret_cast<const q8_u32x4*>(tile + c * PITCH + piece);
+            *reinterpret_cast<q8_u32x4*>(qt + col * ldqt + (long long)blockIdx.y * 128 + piece * 16) =
+                *reinterpret_cast<const q8_u32x4_a*>(tile + c * 128 + ((piece ^ ((c >> 3) & 7)) << 4));
     }
-}
-
-// column sums of the tile rows' partial sums, in a fixed order, accumulated in fp64 and rounded once
-__global__ __launch_bounds__(TPB) void q8_colsum_k(const float* __restrict__ part, float* __restrict__ out, long long parts, long long cols) {
-    __shared__ double red[4][64];
-    const int lane = threadIdx.x & 63, w = threadIdx.x >> 6;
-    const long long c = (long long)blockIdx.x * 64 + lane;
-    double a = 0.0;
-    if (c < cols)
-        for (long long p = w; p < parts; p += 4) a += (double)part[p * cols + c];
-    red[w][lane] = a;
-    __syncthreads();
-    if (w == 0 && c < cols) out[c] = (float)((red[0][lane] + red[1][lane]) + (red[2][lane] + red[3][lane]));
 }
 
 bool q8_aligned(const void* p, unsigned n) { return ((size_t)p % n) == 0; }
 unsigned q8_grid(unsigned total) {
-    const unsigned g = cdiv(total, TPB / 16);
+    const unsigned g = cdiv(total, TPB / 16 * UNROLL);
     return g < 8192 ? g : 8192;
 }
 
 template <int DT, int FMT>
 int pack_launch(const void* x, long long ldx, uint8_t* q, long long ldq, uint8_t* s, long long lds, unsigned nb, unsigned total,
                 long long cols, int padded, hipStream_t st) {
-    const bool vec = q8_aligned(x, 16) && ldx % (16 / el_size<DT>) == 0 && ldq % 8 == 0 && q8_aligned(q, 8);
-    if (vec) q8_pack_k<DT, FMT, true><<<q8_grid(total), TPB, 0, st>>>(x, ldx, q, ldq, s, lds, nb, total, cols, padded);
-    else q8_pack_k<DT, FMT, false><<<q8_grid(total), TPB, 0, st>>>(x, ldx, q, ldq, s, lds, nb, total, cols, padded);
+    q8_pack_k<DT, FMT><<<q8_grid(total), TPB, 0, st>>>(x, ldx, q, ldq, s, lds, nb, total, cols, padded);
     return kp_check_launch("q8_pack");
 }
 template <int DT, int FMT>
 int unpack_launch(const uint8_t* q, long long ldq, const uint8_t* s, long long lds, void* y, long long ldy, unsigned nb, unsigned total,
                   long long cols, hipStream_t st) {
-    const bool vec = q8_aligned(y, 16) && ldy % (16 / el_size<DT>) == 0 && ldq % 8 == 0 && q8_aligned(q, 8);
-    if (vec) q8_unpack_k<DT, FMT, true><<<q8_grid(total), TPB, 0, st>>>(q, ldq, s, lds, y, ldy, nb, total, cols);
-    else q8_unpack_k<DT, FMT, false><<<q8_grid(total), TPB, 0, st>>>(q, ldq, s, lds, y, ldy, nb, total, cols);
+    q8_unpack_k<DT, FMT><<<q8_grid(total), TPB, 0, st>>>(q, ldq, s, lds, y, ldy, nb, total, cols);
     return kp_check_launch("q8_unpack");
 }
 template <int DT, int FMT>
 int both_launch(const void* x, long long ldx, uint8_t* q, long long ldq, uint8_t* s, long long lds, uint8_t* qt, long long ldqt,
                 uint8_t* stq, long long ldst, float* ws, float* colsum, long long rows, long long cols, hipStream_t st) {
-    const bool vec = q8_aligned(x, 16) && ldx % (16 / el_size<DT>) == 0;
     const dim3 grid(cdiv(cols, 128), cdiv(rows, 128));
-    float* part = colsum ? ws : nullptr;
-    if (vec) q8_pack_both_k<DT, FMT, true><<<grid, TPB, 0, st>>>(x, ldx, q, ldq, s, lds, qt, ldqt, stq, ldst, part, rows, cols);
-    else q8_pack_both_k<DT, FMT, false><<<grid, TPB, 0, st>>>(x, ldx, q, ldq, s, lds, qt, ldqt, stq, ldst, part, rows, cols);
-    if (colsum) q8_colsum_k<<<cdiv(cols, 64), TPB, 0, st>>>(part, colsum, cdiv(rows, 128), cols);
+    q8_pack_both_k<DT, FMT><<<grid, TPB, 0, st>>>(x, ldx, q, ldq, s, lds, qt, ldqt, stq, ldst, colsum ? ws : nullptr, rows, cols);
+    if (colsum) q8_join_k<<<cdiv(cols, 16), 1024, 0, st>>>(ws, cdiv(rows, 128), cols, colsum, cols, nullptr);
     return kp_check_launch("q8_pack_both");
 }
 
@@ -222,7 +214,6 @@ int kp_q8_pack(const void* x, long long ldx, unsigned char* q, long long ldq, un
     KP_REQUIRE((rows == 1 || (ldx >= cols && lds >= nb)) && (ldq >= nb * Q8_BLOCK || ldq == cols), "kp_q8_pack: row strides %lld, %lld, %lld do not fit %lld columns", ldx, ldq, lds, cols);
     KP_REQUIRE(rows * nb < (1LL << 31), "kp_q8_pack: %lld blocks are more than one call takes", rows * nb);
     const int padded = ldq >= nb * Q8_BLOCK;
-    KP_REQUIRE(!padded || (q8_aligned(q, 8) && ldq % 8 == 0), "kp_q8_pack: padded rows must start on multiples of 8 bytes");
     kp_count_bytes((double)rows * cols * ((dtype == KP_F32 ? 4 : 2) + 1));
     return Q8_DISPATCH(pack_launch, x, ldx, q, ldq, s, lds, (unsigned)nb, (unsigned)(rows * nb), cols, padded, (hipStream_t)stream);
 }

@@ -48,35 +48,60 @@ template <int DT> __device__ __forceinline__ uint32_t el_pack(float lo, float hi
     if constexpr (DT == KP_BF16) return __builtin_bit_cast(uint32_t, __builtin_convertvector(v, q8_bf16x2));
     else return __builtin_bit_cast(uint32_t, __builtin_convertvector(v, q8_f16x2));
 }
-// 8 consecutive elements i .. i + 7; the address is a multiple of 16 bytes
-template <int DT> __device__ __forceinline__ void el_load8(const void* p, long long i, float (&v)[8]) {
+// 8 consecutive elements i .. i + 7.  Rows may start anywhere: gfx950 takes wide accesses on any element's address (a row of 1001 elements
+// costs what one of 1000 does), so the vector types only promise the element's alignment.
+typedef unsigned int q8_u32x4_e2 __attribute__((ext_vector_type(4), aligned(2)));
+typedef unsigned int q8_u32x4_e4 __attribute__((ext_vector_type(4), aligned(4)));
+typedef unsigned int q8_u32x2_e1 __attribute__((ext_vector_type(2), aligned(1)));
+template <int DT> struct El8 { q8_u32x4 w[DT == KP_F32 ? 2 : 1]; };   // as loaded
+template <int DT> __device__ __forceinline__ El8<DT> el_raw8(const void* p, long long i) {
+    El8<DT> r;
     if constexpr (DT == KP_F32) {
-        const float4 a = *reinterpret_cast<const float4*>((const float*)p + i), b = *reinterpret_cast<const float4*>((const float*)p + i + 4);
-        v[0] = a.x; v[1] = a.y; v[2] = a.z; v[3] = a.w; v[4] = b.x; v[5] = b.y; v[6] = b.z; v[7] = b.w;
-    } else {
-        const q8_u32x4 w = *reinterpret_cast<const q8_u32x4*>((const uint16_t*)p + i);
+        r.w[0] = *reinterpret_cast<const q8_u32x4_e4*>((const float*)p + i);
+        r.w[1] = *reinterpret_cast<const q8_u32x4_e4*>((const float*)p + i + 4);
+    } else r.w[0] = *reinterpret_cast<const q8_u32x4_e2*>((const uint16_t*)p + i);
+    return r;
+}
+// the first n of them (n <= 0: none), the others zero
+template <int DT> __device__ __forceinline__ El8<DT> el_raw8_part(const void* p, long long i, int n) {
+    El8<DT> r;
+    if constexpr (DT == KP_F32) {
 #pragma unroll
-        for (int k = 0; k < 4; ++k) el_unpack<DT>(w[k], v[2 * k], v[2 * k + 1]);
+        for (int k = 0; k < 8; ++k) r.w[k >> 2][k & 3] = k < n ? ((const uint32_t*)p)[i + k] : 0u;
+    } else {
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+            const uint32_t lo = 2 * k < n ? ((const uint16_t*)p)[i + 2 * k] : 0u, hi = 2 * k + 1 < n ? ((const uint16_t*)p)[i + 2 * k + 1] : 0u;
+            r.w[0][k] = lo | hi << 16;
+        }
+    }
+    return r;
+}
+template <int DT> __device__ __forceinline__ El8<DT> el_raw8_any(const void* p, long long i, int n) {
+    return n >= 8 ? el_raw8<DT>(p, i) : el_raw8_part<DT>(p, i, n);
+}
+template <int DT> __device__ __forceinline__ void el_unpack8(const El8<DT>& r, float (&v)[8]) {
+    if constexpr (DT == KP_F32) {
+#pragma unroll
+        for (int k = 0; k < 8; ++k) v[k] = __uint_as_float(r.w[k >> 2][k & 3]);
+    } else {
+#pragma unroll
+        for (int k = 0; k < 4; ++k) el_unpack<DT>(r.w[0][k], v[2 * k], v[2 * k + 1]);
     }
 }
-template <int DT> __device__ __forceinline__ void el_store8(void* p, long long i, const float (&v)[8]) {
-    if constexpr (DT == KP_F32) {
-        *reinterpret_cast<float4*>((float*)p + i) = make_float4(v[0], v[1], v[2], v[3]);
-        *reinterpret_cast<float4*>((float*)p + i + 4) = make_float4(v[4], v[5], v[6], v[7]);
+template <int DT> __device__ __forceinline__ void el_load8(const void* p, long long i, int n, float (&v)[8]) { el_unpack8<DT>(el_raw8_any<DT>(p, i, n), v); }
+template <int DT> __device__ __forceinline__ void el_store8(void* p, long long i, int n, const float (&v)[8]) {
+    if (n >= 8) {
+        if constexpr (DT == KP_F32) {
+            *reinterpret_cast<q8_u32x4_e4*>((float*)p + i) = q8_u32x4{__float_as_uint(v[0]), __float_as_uint(v[1]), __float_as_uint(v[2]), __float_as_uint(v[3])};
+            *reinterpret_cast<q8_u32x4_e4*>((float*)p + i + 4) = q8_u32x4{__float_as_uint(v[4]), __float_as_uint(v[5]), __float_as_uint(v[6]), __float_as_uint(v[7])};
+        } else
+            *reinterpret_cast<q8_u32x4_e2*>((uint16_t*)p + i) = q8_u32x4{el_pack<DT>(v[0], v[1]), el_pack<DT>(v[2], v[3]), el_pack<DT>(v[4], v[5]), el_pack<DT>(v[6], v[7])};
     } else {
-        const q8_u32x4 w = {el_pack<DT>(v[0], v[1]), el_pack<DT>(v[2], v[3]), el_pack<DT>(v[4], v[5]), el_pack<DT>(v[6], v[7])};
-        *reinterpret_cast<q8_u32x4*>((uint16_t*)p + i) = w;
+#pragma unroll
+        for (int k = 0; k < 8; ++k)
+            if (k < n) el_store<DT>(p, i + k, v[k]);
     }
-}
-// the same with any alignment and only the first `n` elements there (n <= 0: none); the others are zero / not written
-template <int DT> __device__ __forceinline__ void el_load8_part(const void* p, long long i, int n, float (&v)[8]) {
-#pragma unroll
-    for (int k = 0; k < 8; ++k) v[k] = k < n ? el_load<DT>(p, i + k) : 0.f;
-}
-template <int DT> __device__ __forceinline__ void el_store8_part(void* p, long long i, int n, const float (&v)[8]) {
-#pragma unroll
-    for (int k = 0; k < 8; ++k)
-        if (k < n) el_store<DT>(p, i + k, v[k]);
 }
 
 // ---- the format -------------------------------------------------------------------------------------------------------------------
@@ -129,18 +154,22 @@ template <int FMT> __device__ __forceinline__ void q8_values8(q8_u32x2 q, float 
         v[4 * k] = lo[0] * up; v[4 * k + 1] = lo[1] * up; v[4 * k + 2] = hi[0] * up; v[4 * k + 3] = hi[1] * up;
     }
 }
-// 8 bytes with any alignment, the first `n` of them
-__device__ __forceinline__ q8_u32x2 q8_load8_part(const uint8_t* p, int n) {
+// 8 bytes anywhere, the first n of them
+__device__ __forceinline__ q8_u32x2 q8_load8(const uint8_t* p, int n) {
+    if (n >= 8) return *reinterpret_cast<const q8_u32x2_e1*>(p);
     q8_u32x2 r = {0u, 0u};
 #pragma unroll
     for (int k = 0; k < 8; ++k)
         if (k < n) r[k >> 2] |= (uint32_t)p[k] << (8 * (k & 3));
     return r;
 }
-__device__ __forceinline__ void q8_store8_part(uint8_t* p, int n, q8_u32x2 q) {
+__device__ __forceinline__ void q8_store8(uint8_t* p, int n, q8_u32x2 q) {
+    if (n >= 8) *reinterpret_cast<q8_u32x2_e1*>(p) = q;
+    else {
 #pragma unroll
-    for (int k = 0; k < 8; ++k)
-        if (k < n) p[k] = (uint8_t)(q[k >> 2] >> (8 * (k & 3)));
+        for (int k = 0; k < 8; ++k)
+            if (k < n) p[k] = (uint8_t)(q[k >> 2] >> (8 * (k & 3)));
+    }
 }
 
 // ---- reductions over aligned groups of 16 lanes (one DPP row): lane ^ 1, ^ 2, ^ 7, + 8.  All lanes of the wave are active -------------
@@ -153,6 +182,44 @@ __device__ __forceinline__ uint32_t q8_max16(uint32_t m) {
     m = q8_umax(m, q8_dpp<0x4E>(m));
     m = q8_umax(m, q8_dpp<0x141>(m));
     return q8_umax(m, q8_dpp<0x128>(m));
+}
+
+// Sums of `parts` partial rows of `width` floats, in a fixed order, in fp64, rounded once: 16 columns x 64 runs of parts a workgroup of 1024;
+// column c goes to out0[c], from `cut` on to out1[c - cut] (either may be NULL).
+__global__ __launch_bounds__(1024) void q8_join_k(const float* __restrict__ part, long long parts, long long width, float* __restrict__ out0,
+                                                  long long cut, float* __restrict__ out1) {
+    __shared__ double red[64][17];
+    const int col = threadIdx.x & 15, run = threadIdx.x >> 4;
+    const long long c = (long long)blockIdx.x * 16 + col;
+    double s = 0.0;
+    if (c < width) {
+        long long p = run;
+        for (; p + 7 * 64 < parts; p += 8 * 64) {
+            float v[8];
+#pragma unroll
+            for (int u = 0; u < 8; ++u) v[u] = part[(p + u * 64) * width + c];
+#pragma unroll
+            for (int u = 0; u < 8; ++u) s += (double)v[u];
+        }
+        float v[8];
+#pragma unroll
+        for (int u = 0; u < 8; ++u) v[u] = p + u * 64 < parts ? part[(p + u * 64) * width + c] : 0.f;
+#pragma unroll
+        for (int u = 0; u < 8; ++u) s += (double)v[u];
+    }
+    red[run][col] = s;
+    __syncthreads();
+    if (run < 4) {   // four groups of 16 runs, then the groups: lanes run * 16 + col of the first wave
+        s = 0.0;
+        for (int k = 0; k < 16; ++k) s += red[run * 16 + k][col];
+        red[run * 16][col] = s;   // (read by this thread only, above)
+    }
+    __syncthreads();
+    if (run == 0 && c < width) {
+        s = (red[0][col] + red[16][col]) + (red[32][col] + red[48][col]);
+        if (c < cut) { if (out0) out0[c] = (float)s; }
+        else if (out1) out1[c - cut] = (float)s;
+    }
 }
 
 }  // namespace

@@ -50,6 +50,13 @@ def as_rows(x: torch.Tensor):
     return x, x.numel() // width, width
 
 
+def as_vector(t):
+    """A weight or bias vector as the kernels read it: fp32, dense (differentiable; itself where it already is; None stays None)."""
+    if t is None or (t.dtype == torch.float32 and t.is_contiguous()):
+        return t
+    return t.to(torch.float32).contiguous()
+
+
 class Packed8:
     """A tensor in the 8-bit block format: `values` (bytes), `scales` (exponent bytes), the `shape` and `dtype` it stands for.
 
@@ -181,8 +188,7 @@ def matmul8(a: Packed8, b: Packed8, bias: torch.Tensor = None, dtype: torch.dtyp
     shape = (*a.shape[:-1], b.shape[0])
     if a.values.shape[0] == 0 or b.shape[0] == 0:
         return torch.empty(shape, device=a.values.device, dtype=dtype)
-    if bias is not None:
-        bias = bias.detach().to(torch.float32).contiguous()
+    bias = as_vector(bias)
     with device_of(a.values):
         return _product((a.values, a.scales), FORMATS[a.fmt], (b.values, b.scales), FORMATS[b.fmt], bias, shape, dtype)
 
@@ -252,8 +258,7 @@ def linear8(x: torch.Tensor, weight, bias: torch.Tensor = None, fmt: str = 'e4m3
         raise ValueError(f'linear8: x on {x.device}, the weight on {dev}')
     N = weight.shape[0]
     _check_bias(bias, N, x.device)
-    if bias is not None and (bias.dtype != torch.float32 or not bias.is_contiguous()):
-        bias = bias.to(torch.float32).contiguous()
+    bias = as_vector(bias)
     if not packed:
         return _Linear8.apply(x, weight, bias, fmt, grad_fmt)
     if torch.is_grad_enabled() and (x.requires_grad or (bias is not None and bias.requires_grad)):

@@ -11,17 +11,17 @@ from torch.autograd.function import once_differentiable
 
 from . import _lib
 from ._lib import call, ptr
-from .lowp import BLOCK, DTYPES, FORMATS, as_rows, dtype_code, format_code
+from .lowp import BLOCK, DTYPES, FORMATS, as_rows, as_vector, dtype_code, format_code
 from .runtime import device_of, require_device, stream_ptr
 
 
 def _forward(x, weight, bias, eps, stats, fmt):
     m, rows, ld = as_rows(x)
     C = x.shape[-1]
-    y = torch.empty(x.shape, device=x.device, dtype=x.dtype)
+    y = x.new_empty(x.shape)
     mean = rstd = q = s = None
     if stats:
-        mean, rstd = torch.empty(rows, device=x.device, dtype=torch.float32), torch.empty(rows, device=x.device, dtype=torch.float32)
+        mean, rstd = x.new_empty(rows, dtype=torch.float32), x.new_empty(rows, dtype=torch.float32)
     if fmt:
         q = torch.empty(rows, C, device=x.device, dtype=torch.uint8)
         s = torch.empty(rows, (C + BLOCK - 1) // BLOCK, device=x.device, dtype=torch.uint8)
@@ -50,7 +50,7 @@ class _LayerNorm(torch.autograd.Function):
         C, dev = dy.shape[-1], dy.device
         f32 = dict(device=dev, dtype=torch.float32)
         make = torch.empty if rows else torch.zeros   # (no rows: nothing is launched)
-        dx = torch.empty(dy.shape, device=dev, dtype=dy.dtype) if need_x else None
+        dx = dy.new_empty(dy.shape) if need_x else None
         dw = make(C, **f32) if need_w else None
         db = make(C, **f32) if need_b else None
         if rows:
@@ -79,7 +79,7 @@ def layer_norm(x: torch.Tensor, weight: torch.Tensor = None, bias: torch.Tensor 
     for name, t in (('weight', weight), ('bias', bias)):
         if t is not None and (t.shape != x.shape[-1:] or t.dtype not in DTYPES or t.device != x.device):
             raise ValueError(f'layer_norm: {name} must be a vector of {x.shape[-1]} floats on {x.device}, got {tuple(t.shape)} {t.dtype} on {t.device}')
-    weight, bias = (t.to(torch.float32).contiguous() if t is not None else None for t in (weight, bias))
+    weight, bias = as_vector(weight), as_vector(bias)
     if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (x, weight, bias)):
         return _LayerNorm.apply(x, weight, bias, eps, keep)
     return _forward(x, weight, bias, eps, False, None)[0]

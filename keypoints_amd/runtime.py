@@ -34,8 +34,9 @@ _HERE = contextlib.nullcontext()
 
 
 def stream_ptr() -> int:
-    """hipStream_t of torch's current stream (kernels are enqueued there, never synchronised)."""
-    return torch.cuda.current_stream().cuda_stream
+    """hipStream_t of torch's current stream (kernels are enqueued there, never synchronised).  The raw getter: 0.3 us of host time a
+    launch instead of the 2.8 us of building a torch.cuda.Stream."""
+    return torch._C._cuda_getCurrentRawStream(torch.cuda.current_device())
 
 
 def device_of(t: torch.Tensor):
