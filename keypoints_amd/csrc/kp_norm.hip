@@ -26,13 +26,6 @@ template <int G> __device__ __forceinline__ float ln_wave_sum(float v) {
     if constexpr (G >= 64) v += __shfl_xor(v, 32, 64);
     return v;
 }
-template <int G> __device__ __forceinline__ uint32_t ln_block_max(uint32_t m) {   // over the lanes of one 128-block: min(G, 16)
-    if constexpr (G >= 2) m = q8_umax(m, q8_dpp<0xB1>(m));
-    if constexpr (G >= 4) m = q8_umax(m, q8_dpp<0x4E>(m));
-    if constexpr (G >= 8) m = q8_umax(m, q8_dpp<0x141>(m));
-    if constexpr (G >= 16) m = q8_umax(m, q8_dpp<0x128>(m));
-    return m;
-}
 // sums of N values at once; `red`: N * (G / 64) * (rows a workgroup takes at once) floats that the workgroup's previous sum did not use
 // (every thread calls it; one barrier)
 template <int G, int N> __device__ __forceinline__ void ln_sums(float (&v)[N], float* red) {
@@ -65,14 +58,15 @@ struct LnBwd {
 
 // A row's lanes: sub = thread % G, chunk j of 8 columns at (j * G + sub) * 8.  The next row's loads are in flight during this row's sums
 // (not in the backward of the widest rows, two chunks a lane in workgroups of 1024: the 128 registers a lane has there go to the sums).
-// A workgroup has 256 threads; past a wave 1024, so that the four rows of 256 lanes that are taken at once share one partial row of the
+// A workgroup has 256 threads; past a wave, G in the forward and 1024 in the backward, so that the four rows of 256 lanes that are taken at once share one partial row of the
 // weight's gradient.
 template <int G> constexpr int ln_tpb = G > 64 ? 1024 : 256;
+template <int G> constexpr int ln_fwd_tpb = G > 64 ? G : 256;
 
 // KEEP: 0, or KP_E4M3 / KP_E5M2: the row leaves in 8 bits too
 template <int DT, int G, int NJ, int KEEP>
-__global__ __launch_bounds__(ln_tpb<G>) void ln_fwd_k(const LnFwd P) {
-    constexpr int TPB = ln_tpb<G>, R = TPB / G;
+__global__ __launch_bounds__(ln_fwd_tpb<G>) void ln_fwd_k(const LnFwd P) {
+    constexpr int TPB = ln_fwd_tpb<G>, R = TPB / G;
     __shared__ float red[G > 64 ? 64 : 1];   // four sets of 16: two sums a row, alternating rows
     const int sub = threadIdx.x & (G - 1);
     const float inv = 1.f / (float)P.C;
@@ -96,8 +90,10 @@ __global__ __launch_bounds__(ln_tpb<G>) void ln_fwd_k(const LnFwd P) {
         const bool live = row < P.rows;
         float v[NJ][8];
         float sum[1] = {0.f}, sq[1] = {0.f};
+        El8<DT> raw[KEEP ? NJ : 1];
 #pragma unroll
         for (int j = 0; j < NJ; ++j) {
+            if constexpr (KEEP != 0) raw[j] = next[j];
             el_unpack8<DT>(next[j], v[j]);
 #pragma unroll
             for (int k = 0; k < 8; ++k) sum[0] += v[j][k];
@@ -111,8 +107,8 @@ __global__ __launch_bounds__(ln_tpb<G>) void ln_fwd_k(const LnFwd P) {
         for (int j = 0; j < NJ; ++j)
 #pragma unroll
             for (int k = 0; k < 8; ++k) {
-                const float d = k < n[j] ? v[j][k] - mean : 0.f;
-                sq[0] = __builtin_fmaf(d, d, sq[0]);
+                v[j][k] = k < n[j] ? v[j][k] - mean : 0.f;
+                sq[0] = __builtin_fmaf(v[j][k], v[j][k], sq[0]);
             }
         ln_sums<G, 1>(sq, slot + (G > 64 ? 16 : 0));
         const float rstd = 1.f / sqrtf(sq[0] * inv + P.eps);
@@ -120,15 +116,16 @@ __global__ __launch_bounds__(ln_tpb<G>) void ln_fwd_k(const LnFwd P) {
         for (int j = 0; j < NJ; ++j) {
             const int c = (j * G + sub) * 8;
             if constexpr (KEEP != 0) {
-                const uint32_t byte = q8_scale_byte<KEEP>(ln_block_max<G>(q8_mag8(v[j])));
+                q8_u32x2 out;
+                const uint32_t byte = q8_pack_block<DT, KEEP, (G < 16 ? G : 16)>(raw[j], out);
                 if (live && n[j] > 0) {
-                    q8_store8(P.q + row * P.C + c, n[j], q8_cvt8<KEEP>(v[j], q8_down(byte)));
+                    q8_store8(P.q + row * P.C + c, n[j], out);
                     if ((c & (Q8_BLOCK - 1)) == 0) P.s[row * P.nb + c / Q8_BLOCK] = (uint8_t)byte;
                 }
             }
             float o[8];
 #pragma unroll
-            for (int k = 0; k < 8; ++k) o[k] = (v[j][k] - mean) * rstd * w[j][k] + b[j][k];
+            for (int k = 0; k < 8; ++k) o[k] = __builtin_fmaf(v[j][k] * rstd, w[j][k], b[j][k]);
             if (live) el_store8<DT>(P.y, row * P.ldy + c, n[j], o);
         }
         if (P.mean && sub == 0 && live) {
@@ -289,10 +286,9 @@ __global__ __launch_bounds__(1024) void ln_fwd_long_k(const LnFwd P) {
             for (int b0 = 0; b0 < P.nb; b0 += 64) {
                 const int kb = b0 + (int)(threadIdx.x >> 4), c = kb * Q8_BLOCK + sub * 8;
                 const int n = P.C - c >= 8 ? 8 : (P.C > c ? P.C - c : 0);
-                float v[8];
-                el_load8<DT>(P.x, row * P.ldx + c, n, v);
-                const uint32_t byte = q8_scale_byte<KEEP>(q8_max16(q8_mag8(v)));
-                q8_store8(P.q + row * P.C + c, n, q8_cvt8<KEEP>(v, q8_down(byte)));
+                q8_u32x2 out;
+                const uint32_t byte = q8_pack_block<DT, KEEP, 16>(el_raw8_any<DT>(P.x, row * P.ldx + c, n), out);
+                q8_store8(P.q + row * P.C + c, n, out);
                 if (sub == 0 && kb < P.nb) P.s[row * P.nb + kb] = (uint8_t)byte;
             }
         }
@@ -365,10 +361,10 @@ template <int DT, int KEEP> int fwd_launch(const LnFwd& P, hipStream_t st) {
         ln_fwd_long_k<DT, KEEP><<<(unsigned)(P.rows < 1024 ? P.rows : 1024), 1024, 0, st>>>(P);
         return kp_check_launch("layer_norm_fwd");
     }
-    const int g = ln_group(P.C), per = ln_rows(P.C);
-    const long long want = (P.rows + per - 1) / per, cap = g > 64 ? 512 : 2048;
+    const int g = ln_group(P.C), per = g > 64 ? 1 : 256 / g;
+    const long long want = (P.rows + per - 1) / per, cap = g > 64 ? 1024 * 512 / g : 2048;
     const unsigned grid = (unsigned)(want < cap ? want : cap);
-#define LN_FWD(G, NJ) ln_fwd_k<DT, G, NJ, KEEP><<<grid, ln_tpb<G>, 0, st>>>(P)
+#define LN_FWD(G, NJ) ln_fwd_k<DT, G, NJ, KEEP><<<grid, ln_fwd_tpb<G>, 0, st>>>(P)
     switch (g) {
         case 1: LN_FWD(1, 1); break;
         case 2: LN_FWD(2, 1); break;

@@ -12,9 +12,20 @@ typedef q8_u32x4 __attribute__((may_alias)) q8_u32x4_a;
 // `padded`: the row's last block is written out to its full 128 bytes with zeros.
 constexpr int UNROLL = 2;
 struct BlockAt { unsigned row, kb; long long c; int n; };   // n: elements of this lane's 8 that the row has
-__device__ __forceinline__ BlockAt block_at(unsigned b, unsigned nb, unsigned total, long long cols, int sub) {
+// division of block numbers below 2^31 by the blocks of a row: (b * mul) >> (32 + shift), mul = ceil(2^(32 + shift) / nb) with the shift
+// that brings it to 32 bits (exact: the error b * (mul nb - 2^(32 + shift)) / (nb 2^(32 + shift)) stays below 1 / nb); mul = 0: one row
+struct RowDiv { unsigned mul, shift; };
+RowDiv row_div(unsigned nb, unsigned total) {
+    if (nb == total) return RowDiv{0, 0};
+    if (nb == 1) return RowDiv{1, 0};
+    unsigned l = 1;
+    while (l < 31 && (1u << l) < nb) ++l;   // 2^(l-1) < nb <= 2^l
+    return RowDiv{(unsigned)(((1ull << (31 + l)) + nb - 1) / nb), l - 1};
+}
+__device__ __forceinline__ BlockAt block_at(unsigned b, unsigned nb, RowDiv div, unsigned total, long long cols, int sub) {
     BlockAt r;
-    r.row = b < total ? b / nb : 0;
+    r.row = nb == 1 ? b : __umulhi(b, div.mul) >> div.shift;
+    if (b >= total) r.row = 0;
     r.kb = b < total ? b - r.row * nb : 0;
     r.c = (long long)r.kb * Q8_BLOCK + sub * 8;
     r.n = b >= total ? 0 : (cols - r.c >= 8 ? 8 : (cols > r.c ? (int)(cols - r.c) : 0));
@@ -22,8 +33,8 @@ __device__ __forceinline__ BlockAt block_at(unsigned b, unsigned nb, unsigned to
 }
 template <int DT, int FMT>
 __global__ __launch_bounds__(TPB) void q8_pack_k(const void* __restrict__ x, long long ldx, uint8_t* __restrict__ q, long long ldq,
-                                                 uint8_t* __restrict__ s, long long lds, unsigned nb, unsigned total, long long cols,
-                                                 int padded) {
+                                                 uint8_t* __restrict__ s, long long lds, unsigned nb, RowDiv div, unsigned total,
+                                                 long long cols, int padded) {
     const int sub = threadIdx.x & 15;
     const unsigned per = TPB / 16, stride = gridDim.x * per * UNROLL;
     for (unsigned b0 = blockIdx.x * per * UNROLL; b0 < total; b0 += stride) {
@@ -31,16 +42,15 @@ __global__ __launch_bounds__(TPB) void q8_pack_k(const void* __restrict__ x, lon
         El8<DT> raw[UNROLL];
 #pragma unroll
         for (int u = 0; u < UNROLL; ++u) {
-            at[u] = block_at(b0 + u * per + (threadIdx.x >> 4), nb, total, cols, sub);
+            at[u] = block_at(b0 + u * per + (threadIdx.x >> 4), nb, div, total, cols, sub);
             raw[u] = el_raw8_any<DT>(x, at[u].row * ldx + at[u].c, at[u].n);
         }
 #pragma unroll
         for (int u = 0; u < UNROLL; ++u) {
-            float v[8];
-            el_unpack8<DT>(raw[u], v);
-            const uint32_t byte = q8_scale_byte<FMT>(q8_max16(q8_mag8(v)));
+            q8_u32x2 out;
+            const uint32_t byte = q8_pack_block<DT, FMT, 16>(raw[u], out);
             if (b0 + u * per + (threadIdx.x >> 4) < total) {
-                q8_store8(q + at[u].row * ldq + at[u].c, padded ? 8 : at[u].n, q8_cvt8<FMT>(v, q8_down(byte)));
+                q8_store8(q + at[u].row * ldq + at[u].c, padded ? 8 : at[u].n, out);
                 if (sub == 0) s[at[u].row * lds + at[u].kb] = (uint8_t)byte;
             }
         }
@@ -64,8 +74,8 @@ template <int DT, int FMT> __device__ __forceinline__ void q8_unpack8(q8_u32x2 q
 
 template <int DT, int FMT>
 __global__ __launch_bounds__(TPB) void q8_unpack_k(const uint8_t* __restrict__ q, long long ldq, const uint8_t* __restrict__ s,
-                                                   long long lds, void* __restrict__ y, long long ldy, unsigned nb, unsigned total,
-                                                   long long cols) {
+                                                   long long lds, void* __restrict__ y, long long ldy, unsigned nb, RowDiv div,
+                                                   unsigned total, long long cols) {
     const int sub = threadIdx.x & 15;
     const unsigned per = TPB / 16, stride = gridDim.x * per * UNROLL;
     for (unsigned b0 = blockIdx.x * per * UNROLL; b0 < total; b0 += stride) {
@@ -74,7 +84,7 @@ __global__ __launch_bounds__(TPB) void q8_unpack_k(const uint8_t* __restrict__ q
         uint32_t byte[UNROLL];
 #pragma unroll
         for (int u = 0; u < UNROLL; ++u) {
-            at[u] = block_at(b0 + u * per + (threadIdx.x >> 4), nb, total, cols, sub);
+            at[u] = block_at(b0 + u * per + (threadIdx.x >> 4), nb, div, total, cols, sub);
             raw[u] = q8_load8(q + at[u].row * ldq + at[u].c, at[u].n);
             byte[u] = s[at[u].row * lds + at[u].kb];
         }
@@ -103,57 +113,104 @@ __global__ __launch_bounds__(TPB) void q8_pack_both_k(const void* __restrict__ x
     const int t = threadIdx.x, cv = t & 15, g = t >> 4, wave = t >> 6;
     const long long c0 = (long long)blockIdx.x * 128 + cv * 8, r0 = (long long)blockIdx.y * 128 + g * 8;
     const int n = cols - c0 >= 8 ? 8 : (cols > c0 ? (int)(cols - c0) : 0);
-    float v[8][8];
+    constexpr int W = DT == KP_F32 ? 8 : 4, PER = 8 / W;   // words of a thread's 8 columns, columns a word
+    El8<DT> v[8];
 #pragma unroll
-    for (int j = 0; j < 8; ++j) el_load8<DT>(x, (r0 + j) * ldx + c0, r0 + j < rows ? n : 0, v[j]);
+    for (int j = 0; j < 8; ++j) v[j] = el_raw8_any<DT>(x, (r0 + j) * ldx + c0, r0 + j < rows ? n : 0);
     if (q) {
 #pragma unroll
         for (int j = 0; j < 8; ++j) {
-            const uint32_t byte = q8_scale_byte<FMT>(q8_max16(q8_mag8(v[j])));
+            q8_u32x2 out;
+            const uint32_t byte = q8_pack_block<DT, FMT, 16>(v[j], out);
             if (r0 + j < rows) {
-                *reinterpret_cast<q8_u32x2*>(q + (r0 + j) * ldq + c0) = q8_cvt8<FMT>(v[j], q8_down(byte));
+                *reinterpret_cast<q8_u32x2*>(q + (r0 + j) * ldq + c0) = out;
                 if (cv == 0) s[(r0 + j) * lds + blockIdx.x] = (uint8_t)byte;
             }
         }
     }
     if (!qt && !colsum) return;
-    uint32_t m[8];
-#pragma unroll
-    for (int k = 0; k < 8; ++k) {
-        m[k] = 0;
-#pragma unroll
-        for (int j = 0; j < 8; ++j) m[k] = q8_umax(m[k], q8_mag(v[j][k]));
-        m[k] = q8_umax(m[k], (uint32_t)__shfl_xor((int)m[k], 16, 64));
-        m[k] = q8_umax(m[k], (uint32_t)__shfl_xor((int)m[k], 32, 64));
-    }
-    if ((t & 63) < 16) {
-#pragma unroll
-        for (int k = 0; k < 8; ++k) wmax[wave][cv * 8 + k] = m[k];
-    }
     if (colsum) {
+        float sum[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+            float f[8];
+            el_unpack8<DT>(v[j], f);
+#pragma unroll
+            for (int k = 0; k < 8; ++k) sum[k] += f[k];
+        }
 #pragma unroll
         for (int k = 0; k < 8; ++k) {
-            float sum = 0.f;
-#pragma unroll
-            for (int j = 0; j < 8; ++j) sum += v[j][k];
-            sum += __shfl_xor(sum, 16, 64);
-            sum += __shfl_xor(sum, 32, 64);
-            if ((t & 63) < 16) wsum[wave][cv * 8 + k] = sum;
+            sum[k] += __shfl_xor(sum[k], 16, 64);
+            sum[k] += __shfl_xor(sum[k], 32, 64);
+            if ((t & 63) < 16) wsum[wave][cv * 8 + k] = sum[k];
         }
+    }
+    // the columns' maxima in the type's own bits, two columns a word in 16 bits
+#pragma unroll
+    for (int k = 0; k < W; ++k) {
+        uint32_t m = q8_raw_mag<DT>(v[0].w[k >> 2][k & 3]);
+#pragma unroll
+        for (int j = 1; j < 8; ++j) m = q8_raw_max<DT>(m, q8_raw_mag<DT>(v[j].w[k >> 2][k & 3]));
+        m = q8_raw_max<DT>(m, (uint32_t)__shfl_xor((int)m, 16, 64));
+        m = q8_raw_max<DT>(m, (uint32_t)__shfl_xor((int)m, 32, 64));
+        if ((t & 63) < 16) wmax[wave][cv * W + k] = m;
     }
     __syncthreads();
     if (colsum && t < 128 && (long long)blockIdx.x * 128 + t < cols)
         colsum[(long long)blockIdx.y * cols + (long long)blockIdx.x * 128 + t] = (wsum[0][t] + wsum[1][t]) + (wsum[2][t] + wsum[3][t]);
     if (!qt) return;
+    uint32_t bits[8];
+    bool plain = false;
 #pragma unroll
     for (int k = 0; k < 8; ++k) {
+        const int w = cv * W + k / PER;
+        const uint32_t m = q8_raw_max<DT>(q8_raw_max<DT>(wmax[0][w], wmax[1][w]), q8_raw_max<DT>(wmax[2][w], wmax[3][w]));
+        bits[k] = q8_raw_bits<DT>(DT == KP_F32 ? m : (k & 1 ? m >> 16 : m & 0xffffu));
+        plain |= q8_plain<FMT>(bits[k]);
+    }
+    auto leave = [&](int k, uint32_t byte, q8_u32x2 out) {
         const int c = cv * 8 + k;
-        const uint32_t byte = q8_scale_byte<FMT>(q8_umax(q8_umax(wmax[0][c], wmax[1][c]), q8_umax(wmax[2][c], wmax[3][c])));
-        float col[8];
-#pragma unroll
-        for (int j = 0; j < 8; ++j) col[j] = v[j][k];
-        *reinterpret_cast<q8_u32x2_a*>(tile + c * 128 + (((g >> 1) ^ (cv & 7)) << 4) + (g & 1) * 8) = q8_cvt8<FMT>(col, q8_down(byte));
+        *reinterpret_cast<q8_u32x2_a*>(tile + c * 128 + (((g >> 1) ^ (cv & 7)) << 4) + (g & 1) * 8) = out;
         if (g == 0 && c0 + k < cols) st[(c0 + k) * ldst + blockIdx.y] = (uint8_t)byte;
+    };
+    if (__any(plain)) {   // every wave holds all 128 columns: one answer for the workgroup
+        float f[8][8];
+#pragma unroll
+        for (int j = 0; j < 8; ++j) el_unpack8<DT>(v[j], f[j]);
+        __syncthreads();
+#pragma unroll
+        for (int k = 0; k < 8; ++k) {
+            uint32_t m = 0;
+#pragma unroll
+            for (int j = 0; j < 8; ++j) m = q8_umax(m, q8_mag(f[j][k]));
+            m = q8_umax(m, (uint32_t)__shfl_xor((int)m, 16, 64));
+            m = q8_umax(m, (uint32_t)__shfl_xor((int)m, 32, 64));
+            if ((t & 63) < 16) wmax[wave][cv * 8 + k] = m;
+        }
+        __syncthreads();
+#pragma unroll
+        for (int k = 0; k < 8; ++k) {
+            const int c = cv * 8 + k;
+            const uint32_t byte = q8_scale_byte<FMT>(q8_umax(q8_umax(wmax[0][c], wmax[1][c]), q8_umax(wmax[2][c], wmax[3][c])));
+            float col[8];
+#pragma unroll
+            for (int j = 0; j < 8; ++j) col[j] = f[j][k];
+            leave(k, byte, q8_cvt8<FMT>(col, q8_down(byte)));
+        }
+    } else {
+#pragma unroll
+        for (int k = 0; k < 8; ++k) {
+            const uint32_t byte = q8_scale_byte<FMT>(bits[k]);
+            const float up = q8_up(byte);
+            uint32_t e[8];   // the column's elements: fp32 words, or pairs of rows in the first four
+#pragma unroll
+            for (int j = 0; j < 8; ++j) {
+                if constexpr (DT == KP_F32) e[j] = v[j].w[k >> 2][k & 3];
+                else if (j < 4) e[j] = __builtin_amdgcn_perm(v[2 * j + 1].w[0][k >> 1], v[2 * j].w[0][k >> 1], k & 1 ? 0x07060302u : 0x05040100u);
+            }
+            if constexpr (DT == KP_F32) leave(k, byte, q8_u32x2{q8_scaled4<DT, FMT>(e[0], e[1], e[2], e[3], up), q8_scaled4<DT, FMT>(e[4], e[5], e[6], e[7], up)});
+            else leave(k, byte, q8_u32x2{q8_scaled4<DT, FMT>(e[0], e[1], 0u, 0u, up), q8_scaled4<DT, FMT>(e[2], e[3], 0u, 0u, up)});
+        }
     }
     __syncthreads();
 #pragma unroll
@@ -175,13 +232,13 @@ unsigned q8_grid(unsigned total) {
 template <int DT, int FMT>
 int pack_launch(const void* x, long long ldx, uint8_t* q, long long ldq, uint8_t* s, long long lds, unsigned nb, unsigned total,
                 long long cols, int padded, hipStream_t st) {
-    q8_pack_k<DT, FMT><<<q8_grid(total), TPB, 0, st>>>(x, ldx, q, ldq, s, lds, nb, total, cols, padded);
+    q8_pack_k<DT, FMT><<<q8_grid(total), TPB, 0, st>>>(x, ldx, q, ldq, s, lds, nb, row_div(nb, total), total, cols, padded);
     return kp_check_launch("q8_pack");
 }
 template <int DT, int FMT>
 int unpack_launch(const uint8_t* q, long long ldq, const uint8_t* s, long long lds, void* y, long long ldy, unsigned nb, unsigned total,
                   long long cols, hipStream_t st) {
-    q8_unpack_k<DT, FMT><<<q8_grid(total), TPB, 0, st>>>(q, ldq, s, lds, y, ldy, nb, total, cols);
+    q8_unpack_k<DT, FMT><<<q8_grid(total), TPB, 0, st>>>(q, ldq, s, lds, y, ldy, nb, row_div(nb, total), total, cols);
     return kp_check_launch("q8_unpack");
 }
 template <int DT, int FMT>

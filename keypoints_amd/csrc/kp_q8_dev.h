@@ -172,16 +172,94 @@ __device__ __forceinline__ void q8_store8(uint8_t* p, int n, q8_u32x2 q) {
     }
 }
 
-// ---- reductions over aligned groups of 16 lanes (one DPP row): lane ^ 1, ^ 2, ^ 7, + 8.  All lanes of the wave are active -------------
+// ---- maxima over aligned groups of G <= 16 lanes: lane ^ 1, ^ 2, ^ 7, + 8 of a DPP row.  All lanes of the wave are active ------------------
 template <int CTRL> __device__ __forceinline__ uint32_t q8_dpp(uint32_t v) {
     return (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, CTRL, 0xf, 0xf, true);
 }
 __device__ __forceinline__ uint32_t q8_umax(uint32_t a, uint32_t b) { return a > b ? a : b; }
-__device__ __forceinline__ uint32_t q8_max16(uint32_t m) {
-    m = q8_umax(m, q8_dpp<0xB1>(m));
-    m = q8_umax(m, q8_dpp<0x4E>(m));
-    m = q8_umax(m, q8_dpp<0x141>(m));
-    return q8_umax(m, q8_dpp<0x128>(m));
+typedef unsigned short q8_u16x2 __attribute__((ext_vector_type(2)));
+__device__ __forceinline__ uint32_t q8_umax16(uint32_t a, uint32_t b) {   // two 16-bit maxima
+    return __builtin_bit_cast(uint32_t, __builtin_elementwise_max(__builtin_bit_cast(q8_u16x2, a), __builtin_bit_cast(q8_u16x2, b)));
+}
+template <int G, bool PAIRS> __device__ __forceinline__ uint32_t q8_group_max(uint32_t m) {
+    auto mx = [](uint32_t a, uint32_t b) { return PAIRS ? q8_umax16(a, b) : q8_umax(a, b); };
+    if constexpr (G >= 2) m = mx(m, q8_dpp<0xB1>(m));
+    if constexpr (G >= 4) m = mx(m, q8_dpp<0x4E>(m));
+    if constexpr (G >= 8) m = mx(m, q8_dpp<0x141>(m));
+    if constexpr (G >= 16) m = mx(m, q8_dpp<0x128>(m));
+    return m;
+}
+
+// ---- a block from its elements as loaded.  The largest magnitude is taken over the type's own bits as integers (two at a time in 16 bits)
+// and the elements are converted by the scaling conversions of gfx950, 2 operations an element in all instead of 7.  Blocks that hold an infinity or a not-a-number, or whose
+// scale is the smallest one, take the plain sequence: the maximum over finite elements, a multiplication and a conversion.
+template <int DT> __device__ __forceinline__ uint32_t q8_raw_mag(uint32_t w) { return w & (DT == KP_F32 ? 0x7fffffffu : 0x7fff7fffu); }
+template <int DT> __device__ __forceinline__ uint32_t q8_raw_max(uint32_t a, uint32_t b) { return DT == KP_F32 ? q8_umax(a, b) : q8_umax16(a, b); }
+template <int DT> __device__ __forceinline__ uint32_t q8_raw_peak(const El8<DT>& r) {
+    uint32_t m = q8_raw_mag<DT>(r.w[0][0]);
+#pragma unroll
+    for (int k = 1; k < (DT == KP_F32 ? 8 : 4); ++k) m = q8_raw_max<DT>(m, q8_raw_mag<DT>(r.w[k >> 2][k & 3]));
+    return m;
+}
+// fp32 bits of a magnitude given in the type's own bits
+template <int DT> __device__ __forceinline__ uint32_t q8_raw_bits(uint32_t m) {
+    if constexpr (DT == KP_F32) return m;
+    else if constexpr (DT == KP_BF16) return m << 16;
+    else return __float_as_uint((float)__builtin_bit_cast(_Float16, (uint16_t)m));
+}
+template <int FMT> __device__ __forceinline__ bool q8_plain(uint32_t bits) {   // not for the scaling conversions
+    return bits >= 0x7f800000u || bits - 1u < ((uint32_t)(q8_top<FMT> + 1) << 23);
+}
+// four bytes of four elements, two words of 16-bit pairs or four fp32 words, divided by `up` = 2^s
+template <int DT, int FMT> __device__ __forceinline__ uint32_t q8_scaled4(uint32_t a, uint32_t b, uint32_t c, uint32_t d, float up) {
+    typedef short s16x2 __attribute__((ext_vector_type(2)));
+    s16x2 r = {0, 0};
+    if constexpr (DT == KP_F32) {
+        if constexpr (FMT == KP_E4M3) {
+            r = __builtin_amdgcn_cvt_scalef32_pk_fp8_f32(r, __uint_as_float(a), __uint_as_float(b), up, false);
+            r = __builtin_amdgcn_cvt_scalef32_pk_fp8_f32(r, __uint_as_float(c), __uint_as_float(d), up, true);
+        } else {
+            r = __builtin_amdgcn_cvt_scalef32_pk_bf8_f32(r, __uint_as_float(a), __uint_as_float(b), up, false);
+            r = __builtin_amdgcn_cvt_scalef32_pk_bf8_f32(r, __uint_as_float(c), __uint_as_float(d), up, true);
+        }
+    } else if constexpr (DT == KP_BF16) {
+        const q8_bf16x2 x = __builtin_bit_cast(q8_bf16x2, a), y = __builtin_bit_cast(q8_bf16x2, b);
+        if constexpr (FMT == KP_E4M3) {
+            r = __builtin_amdgcn_cvt_scalef32_pk_fp8_bf16(r, x, up, false);
+            r = __builtin_amdgcn_cvt_scalef32_pk_fp8_bf16(r, y, up, true);
+        } else {
+            r = __builtin_amdgcn_cvt_scalef32_pk_bf8_bf16(r, x, up, false);
+            r = __builtin_amdgcn_cvt_scalef32_pk_bf8_bf16(r, y, up, true);
+        }
+    } else {
+        const q8_f16x2 x = __builtin_bit_cast(q8_f16x2, a), y = __builtin_bit_cast(q8_f16x2, b);
+        if constexpr (FMT == KP_E4M3) {
+            r = __builtin_amdgcn_cvt_scalef32_pk_fp8_f16(r, x, up, false);
+            r = __builtin_amdgcn_cvt_scalef32_pk_fp8_f16(r, y, up, true);
+        } else {
+            r = __builtin_amdgcn_cvt_scalef32_pk_bf8_f16(r, x, up, false);
+            r = __builtin_amdgcn_cvt_scalef32_pk_bf8_f16(r, y, up, true);
+        }
+    }
+    return __builtin_bit_cast(uint32_t, r);
+}
+// This lane's 8 elements of a block that G lanes hold (G <= 16, a power of two): their bytes, and the block's exponent byte.
+template <int DT, int FMT, int G> __device__ __forceinline__ uint32_t q8_pack_block(const El8<DT>& r, q8_u32x2& out) {
+    uint32_t m = q8_group_max<G, DT != KP_F32>(q8_raw_peak<DT>(r));
+    if constexpr (DT != KP_F32) m = q8_umax(m & 0xffffu, m >> 16);
+    uint32_t bits = q8_raw_bits<DT>(m), byte;
+    if (__any(q8_plain<FMT>(bits))) {
+        float v[8];
+        el_unpack8<DT>(r, v);
+        byte = q8_scale_byte<FMT>(q8_group_max<G, false>(q8_mag8(v)));
+        out = q8_cvt8<FMT>(v, q8_down(byte));
+        return byte;
+    }
+    byte = q8_scale_byte<FMT>(bits);
+    const float up = q8_up(byte);
+    if constexpr (DT == KP_F32) out = q8_u32x2{q8_scaled4<DT, FMT>(r.w[0][0], r.w[0][1], r.w[0][2], r.w[0][3], up), q8_scaled4<DT, FMT>(r.w[1][0], r.w[1][1], r.w[1][2], r.w[1][3], up)};
+    else out = q8_u32x2{q8_scaled4<DT, FMT>(r.w[0][0], r.w[0][1], 0u, 0u, up), q8_scaled4<DT, FMT>(r.w[0][2], r.w[0][3], 0u, 0u, up)};
+    return byte;
 }
 
 // Sums of `parts` partial rows of `width` floats, in a fixed order, in fp64, rounded once: 16 columns x 64 runs of parts a workgroup of 1024;
