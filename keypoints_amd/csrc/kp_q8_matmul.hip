@@ -152,13 +152,26 @@ __global__ __launch_bounds__(64 * WGM * WGN, 2) void q8_mm_k(const MmArgs P) {
             for (int i = 0; i < TN; ++i) f.b[i].h[u] = *reinterpret_cast<const u32x4_a*>(pb + i * 4096);
         }
     };
+    // accumulators start at the bias of the lane's columns (the join adds it to split sums)
+    const bool split = P.splits > 1;
+    const int nw = n0 + wn * WN;
     f32x16 acc[TN][TM];
 #pragma unroll
     for (int n = 0; n < TN; ++n)
 #pragma unroll
-        for (int m = 0; m < TM; ++m)
+        for (int g = 0; g < 4; ++g) {
+            float v[4] = {0.f, 0.f, 0.f, 0.f};
+            if (P.bias && !split) {
+                const int at = nw + n * 32 + g * 8 + fh * 4;
 #pragma unroll
-            for (int e = 0; e < 16; ++e) acc[n][m][e] = 0.f;
+                for (int e = 0; e < 4; ++e)
+                    if (!EDGE || at + e < P.N) v[e] = P.bias[at + e];
+            }
+#pragma unroll
+            for (int m = 0; m < TM; ++m)
+#pragma unroll
+                for (int e = 0; e < 4; ++e) acc[n][m][g * 4 + e] = v[e];
+        }
     Scales sc, sc_next;
     auto mma = [&](const Frags& f) {
         if constexpr (!F32) {
@@ -247,47 +260,44 @@ __global__ __launch_bounds__(64 * WGM * WGN, 2) void q8_mm_k(const MmArgs P) {
     // epilogue: 32 rows of m at a time through a wave's own staging rows in LDS (16-byte pieces XOR-swizzled by the row), then whole rows
     // of WN elements leave
     uint8_t* stage = smem + wave * (32 * WN * 4);
-    const bool split = P.splits > 1;
-    const int nw = n0 + wn * WN;
     auto store_rows = [&](auto DTC) {
-        constexpr int DT = decltype(DTC)::value, ES = el_size<DT>, ROW = WN * ES, PIECES = ROW / 16, PER = 16 / ES;
+        constexpr int DT = decltype(DTC)::value, ES = el_size<DT>, ROW = WN * ES, PIECES = ROW / 16, PER = 16 / ES, RPI = 64 / PIECES;
         uint8_t* out = split ? (uint8_t*)(P.part + ((long long)z * P.M) * P.N) : (uint8_t*)P.c;
         const long long ldc = split ? P.N : P.ldc;
-        const bool vec = ldc % PER == 0 && nw % PER == 0 && ((size_t)out & 15) == 0;
+        const int prow = lane / PIECES, piece = lane % PIECES;   // this lane's piece of rows prow, prow + RPI, ...
+        uint8_t* dst = out + ((m0 + wm * WM + prow) * ldc + nw + piece * PER) * ES;
+        const bool whole = !EDGE || (m0 + BM <= P.M && n0 + BN <= P.N);
 #pragma unroll
         for (int m = 0; m < TM; ++m) {
 #pragma unroll
             for (int n = 0; n < TN; ++n)
 #pragma unroll
                 for (int g = 0; g < 4; ++g) {
-                    const int nn = n * 32 + g * 8 + fh * 4;
-                    float v[4];
-#pragma unroll
-                    for (int e = 0; e < 4; ++e) {
-                        v[e] = acc[n][m][g * 4 + e];
-                        if (P.bias && !split && nw + nn + e < P.N) v[e] += P.bias[nw + nn + e];
-                    }
-                    const int off = nn * ES;
+                    const int off = (n * 32 + g * 8 + fh * 4) * ES;
                     uint8_t* p = stage + fr * ROW + (((off >> 4) ^ (fr & (PIECES - 1))) << 4) + (off & 15);
-                    if constexpr (DT == KP_F32) *reinterpret_cast<f32x4_a*>(p) = f32x4{v[0], v[1], v[2], v[3]};
-                    else *reinterpret_cast<u32x2_a*>(p) = q8_u32x2{el_pack<DT>(v[0], v[1]), el_pack<DT>(v[2], v[3])};
+                    const f32x16& v = acc[n][m];
+                    if constexpr (DT == KP_F32) *reinterpret_cast<f32x4_a*>(p) = f32x4{v[g * 4], v[g * 4 + 1], v[g * 4 + 2], v[g * 4 + 3]};
+                    else *reinterpret_cast<u32x2_a*>(p) = q8_u32x2{el_pack<DT>(v[g * 4], v[g * 4 + 1]), el_pack<DT>(v[g * 4 + 2], v[g * 4 + 3])};
                 }
+            auto piece_at = [&](int i) {
+                const int row = i * RPI + prow;
+                return *reinterpret_cast<const u32x4_a*>(stage + row * ROW + ((piece ^ (row & (PIECES - 1))) << 4));
+            };
+            if (whole) {
 #pragma unroll
-            for (int i = 0; i < 32 * PIECES / 64; ++i) {
-                const int p = i * 64 + lane, row = p / PIECES, piece = p % PIECES;
-                const u32x4 w = *reinterpret_cast<const u32x4_a*>(stage + row * ROW + ((piece ^ (row & (PIECES - 1))) << 4));
-                const int mm = m0 + wm * WM + m * 32 + row, nn = nw + piece * PER;
-                if (mm < P.M && nn < P.N) {
-                    uint8_t* dst = out + ((long long)mm * ldc + nn) * ES;
-                    if (vec && nn + PER <= P.N) *reinterpret_cast<u32x4*>(dst) = w;
-                    else {
+                for (int i = 0; i < 32 / RPI; ++i) *reinterpret_cast<q8_u32x4_e2*>(dst + (long long)(m * 32 + i * RPI) * ldc * ES) = piece_at(i);   // (rows may start anywhere)
+            } else {
+#pragma unroll 1
+                for (int i = 0; i < 32 / RPI; ++i) {
+                    const u32x4 w = piece_at(i);
+                    uint8_t* d = dst + (long long)(m * 32 + i * RPI) * ldc * ES;
+                    const int left = m0 + wm * WM + m * 32 + i * RPI + prow < P.M ? P.N - nw - piece * PER : 0;
 #pragma unroll
-                        for (int e = 0; e < PER; ++e)
-                            if (nn + e < P.N) {
-                                if constexpr (ES == 4) reinterpret_cast<uint32_t*>(dst)[e] = w[e];
-                                else reinterpret_cast<uint16_t*>(dst)[e] = (uint16_t)(w[e >> 1] >> (16 * (e & 1)));
-                            }
-                    }
+                    for (int e = 0; e < PER; ++e)
+                        if (e < left) {
+                            if constexpr (ES == 4) reinterpret_cast<uint32_t*>(d)[e] = w[e];
+                            else reinterpret_cast<uint16_t*>(d)[e] = (uint16_t)(w[e >> 1] >> (16 * (e & 1)));
+                        }
                 }
             }
         }
