@@ -78,7 +78,12 @@ template <int DT> __device__ __forceinline__ El8<DT> el_raw8_part(const void* p,
     return r;
 }
 template <int DT> __device__ __forceinline__ El8<DT> el_raw8_any(const void* p, long long i, int n) {
-    return n >= 8 ? el_raw8<DT>(p, i) : el_raw8_part<DT>(p, i, n);
+    if (n >= 8) return el_raw8<DT>(p, i);
+    if (n > 0) return el_raw8_part<DT>(p, i, n);
+    El8<DT> none;
+#pragma unroll
+    for (int k = 0; k < (DT == KP_F32 ? 2 : 1); ++k) none.w[k] = q8_u32x4{0u, 0u, 0u, 0u};
+    return none;
 }
 template <int DT> __device__ __forceinline__ void el_unpack8(const El8<DT>& r, float (&v)[8]) {
     if constexpr (DT == KP_F32) {
@@ -97,7 +102,7 @@ template <int DT> __device__ __forceinline__ void el_store8(void* p, long long i
             *reinterpret_cast<q8_u32x4_e4*>((float*)p + i + 4) = q8_u32x4{__float_as_uint(v[4]), __float_as_uint(v[5]), __float_as_uint(v[6]), __float_as_uint(v[7])};
         } else
             *reinterpret_cast<q8_u32x4_e2*>((uint16_t*)p + i) = q8_u32x4{el_pack<DT>(v[0], v[1]), el_pack<DT>(v[2], v[3]), el_pack<DT>(v[4], v[5]), el_pack<DT>(v[6], v[7])};
-    } else {
+    } else if (n > 0) {
 #pragma unroll
         for (int k = 0; k < 8; ++k)
             if (k < n) el_store<DT>(p, i + k, v[k]);
@@ -158,6 +163,7 @@ template <int FMT> __device__ __forceinline__ void q8_values8(q8_u32x2 q, float 
 __device__ __forceinline__ q8_u32x2 q8_load8(const uint8_t* p, int n) {
     if (n >= 8) return *reinterpret_cast<const q8_u32x2_e1*>(p);
     q8_u32x2 r = {0u, 0u};
+    if (n > 0)
 #pragma unroll
     for (int k = 0; k < 8; ++k)
         if (k < n) r[k >> 2] |= (uint32_t)p[k] << (8 * (k & 3));
@@ -165,7 +171,7 @@ __device__ __forceinline__ q8_u32x2 q8_load8(const uint8_t* p, int n) {
 }
 __device__ __forceinline__ void q8_store8(uint8_t* p, int n, q8_u32x2 q) {
     if (n >= 8) *reinterpret_cast<q8_u32x2_e1*>(p) = q;
-    else {
+    else if (n > 0) {
 #pragma unroll
         for (int k = 0; k < 8; ++k)
             if (k < n) p[k] = (uint8_t)(q[k >> 2] >> (8 * (k & 3)));
@@ -243,6 +249,11 @@ template <int DT, int FMT> __device__ __forceinline__ uint32_t q8_scaled4(uint32
     }
     return __builtin_bit_cast(uint32_t, r);
 }
+template <int DT, int FMT> __device__ __forceinline__ q8_u32x2 q8_scaled8(const El8<DT>& r, float up) {
+    if constexpr (DT == KP_F32)
+        return q8_u32x2{q8_scaled4<DT, FMT>(r.w[0][0], r.w[0][1], r.w[0][2], r.w[0][3], up), q8_scaled4<DT, FMT>(r.w[1][0], r.w[1][1], r.w[1][2], r.w[1][3], up)};
+    else return q8_u32x2{q8_scaled4<DT, FMT>(r.w[0][0], r.w[0][1], 0u, 0u, up), q8_scaled4<DT, FMT>(r.w[0][2], r.w[0][3], 0u, 0u, up)};
+}
 // This lane's 8 elements of a block that G lanes hold (G <= 16, a power of two): their bytes, and the block's exponent byte.
 template <int DT, int FMT, int G> __device__ __forceinline__ uint32_t q8_pack_block(const El8<DT>& r, q8_u32x2& out) {
     uint32_t m = q8_group_max<G, DT != KP_F32>(q8_raw_peak<DT>(r));
@@ -256,9 +267,7 @@ template <int DT, int FMT, int G> __device__ __forceinline__ uint32_t q8_pack_bl
         return byte;
     }
     byte = q8_scale_byte<FMT>(bits);
-    const float up = q8_up(byte);
-    if constexpr (DT == KP_F32) out = q8_u32x2{q8_scaled4<DT, FMT>(r.w[0][0], r.w[0][1], r.w[0][2], r.w[0][3], up), q8_scaled4<DT, FMT>(r.w[1][0], r.w[1][1], r.w[1][2], r.w[1][3], up)};
-    else out = q8_u32x2{q8_scaled4<DT, FMT>(r.w[0][0], r.w[0][1], 0u, 0u, up), q8_scaled4<DT, FMT>(r.w[0][2], r.w[0][3], 0u, 0u, up)};
+    out = q8_scaled8<DT, FMT>(r, q8_up(byte));
     return byte;
 }
 

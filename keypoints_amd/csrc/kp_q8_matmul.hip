@@ -307,6 +307,126 @@ __global__ __launch_bounds__(64 * WGM * WGN, 2) void q8_mm_k(const MmArgs P) {
     else store_rows(std::integral_constant<int, KP_F16>{});
 }
 
+// Few rows of x in their own type against a packed matrix: y[m][n] = P(x)[m] . W[n] (+ bias).  One launch: a wave packs its own blocks of up
+// to 16 rows of x in registers (the exponent goes straight into the instruction) and streams 16 rows of W past them, 16 x 16 x 128 a
+// block; the 8 waves of a workgroup take every 8th block and join through LDS in wave order.  Bound by the bytes of W and, for a few
+// million of them, by the way to memory and back: every wave has U blocks of loads in flight before its first product.  NT: groups of 16
+// rows of W a wave; two once that still gives every CU a workgroup, which halves the packing of x.
+struct RowArgs {
+    const void* x;
+    long long ldx;
+    const uint8_t *w, *sw;
+    long long ldw, ldsw;
+    const float* bias;
+    void* y;
+    long long ldy;
+    int M, N, K, nb;
+};
+template <int DT, int FX, int FW, int NT>
+__global__ __launch_bounds__(512) void q8_rows_k(const RowArgs P) {
+    constexpr int NW = 8, U = DT == KP_F32 ? 2 : 4;
+    __shared__ float red[NW][16][16 * NT + 1];
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, r16 = lane & 15, quarter = lane >> 4;
+    const int n0 = blockIdx.x * 16 * NT, m0 = blockIdx.y * 16;
+    const bool mine = m0 + r16 < P.M;
+    const uint8_t *w[NT], *sw[NT];
+    f32x4 acc[NT];
+#pragma unroll
+    for (int t = 0; t < NT; ++t) {
+        const int at = n0 + t * 16 + r16, n = at < P.N ? at : P.N - 1;   // (rows of W past the end repeat the last one and are not stored)
+        w[t] = P.w + (long long)n * P.ldw + quarter * 16;
+        sw[t] = P.sw + (long long)n * P.ldsw;
+        acc[t] = f32x4{0.f, 0.f, 0.f, 0.f};
+    }
+    const long long xrow = (long long)(m0 + r16) * P.ldx;
+    for (int kb0 = wave; kb0 < P.nb; kb0 += NW * U) {
+        Frag8 fw[U][NT];
+        int es[U][NT];
+        El8<DT> raw[U][4];   // elements quarter * 16 .. + 15 and 64 further, as the fragment of W has them
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+            const int kb = kb0 + u * NW < P.nb ? kb0 + u * NW : P.nb - 1;
+            const bool live = mine && kb0 + u * NW < P.nb;
+#pragma unroll
+            for (int t = 0; t < NT; ++t) {
+                fw[u][t].h[0] = *reinterpret_cast<const u32x4*>(w[t] + (long long)kb * 128);
+                fw[u][t].h[1] = *reinterpret_cast<const u32x4*>(w[t] + (long long)kb * 128 + 64);
+                es[u][t] = sw[t][kb];
+            }
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                const int k = kb * 128 + (i >> 1) * 64 + quarter * 16 + (i & 1) * 8;
+                raw[u][i] = el_raw8_any<DT>(P.x, xrow + k, live ? P.K - k : 0);
+            }
+        }
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+            if (kb0 + u * NW >= P.nb) break;
+            uint32_t m = 0;
+#pragma unroll
+            for (int i = 0; i < 4; ++i) m = q8_raw_max<DT>(m, q8_raw_peak<DT>(raw[u][i]));
+            m = q8_raw_max<DT>(m, (uint32_t)__shfl_xor((int)m, 16, 64));   // the row's four lanes
+            m = q8_raw_max<DT>(m, (uint32_t)__shfl_xor((int)m, 32, 64));
+            if constexpr (DT != KP_F32) m = q8_umax(m & 0xffffu, m >> 16);
+            const uint32_t bits = q8_raw_bits<DT>(m);
+            Frag8 fx;
+            uint32_t byte;
+            if (__any(q8_plain<FX + 1>(bits))) {
+                float v[4][8];
+                uint32_t t = 0;
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    el_unpack8<DT>(raw[u][i], v[i]);
+                    t = q8_umax(t, q8_mag8(v[i]));
+                }
+                t = q8_umax(t, (uint32_t)__shfl_xor((int)t, 16, 64));
+                t = q8_umax(t, (uint32_t)__shfl_xor((int)t, 32, 64));
+                byte = q8_scale_byte<FX + 1>(t);
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    const q8_u32x2 o = q8_cvt8<FX + 1>(v[i], q8_down(byte));
+                    fx.v[2 * i] = (int)o[0];
+                    fx.v[2 * i + 1] = (int)o[1];
+                }
+            } else {
+                byte = q8_scale_byte<FX + 1>(bits);
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    const q8_u32x2 o = q8_scaled8<DT, FX + 1>(raw[u][i], q8_up(byte));
+                    fx.v[2 * i] = (int)o[0];
+                    fx.v[2 * i + 1] = (int)o[1];
+                }
+            }
+#pragma unroll
+            for (int t = 0; t < NT; ++t) {
+                if constexpr (DT != KP_F32) acc[t] = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(fw[u][t].v, fx.v, acc[t], FW, FX, 0, es[u][t], 0, (int)byte);
+                else {
+                    typedef __bf16 bf8 __attribute__((ext_vector_type(8)));
+                    const float uw = q8_up((uint32_t)es[u][t]), ux = q8_up(byte);
+#pragma unroll
+                    for (int i = 0; i < 4; ++i)
+                        acc[t] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf8, q8_bf16x8<FW>(fw[u][t].v, i, uw)),
+                                                                         __builtin_bit_cast(bf8, q8_bf16x8<FX>(fx.v, i, ux)), acc[t], 0, 0, 0);
+                }
+            }
+        }
+    }
+#pragma unroll
+    for (int t = 0; t < NT; ++t)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) red[wave][r16][t * 16 + quarter * 4 + e] = acc[t][e];   // (a lane: column m = r16, rows n = 4 quarter + e)
+    __syncthreads();
+    if (threadIdx.x < 256 * NT) {
+        const int m = threadIdx.x / (16 * NT), c = threadIdx.x % (16 * NT);
+        if (m0 + m < P.M && n0 + c < P.N) {
+            float v = P.bias ? P.bias[n0 + c] : 0.f;
+#pragma unroll
+            for (int k = 0; k < NW; ++k) v += red[k][m][c];
+            el_store<DT>(P.y, (long long)(m0 + m) * P.ldy + n0 + c, v);
+        }
+    }
+}
+
 // the splits' partial products, added in order, with the bias, rounded once
 template <int DT>
 __global__ __launch_bounds__(256) void q8_mm_join_k(const float* __restrict__ part, int splits, const float* __restrict__ bias,
@@ -344,6 +464,19 @@ template <int FA, int FB, bool F32> int mm_launch(const MmArgs& P, const Plan& p
     else if (p.bm == 128) q8_mm_k<128, 128, 2, 2, FA, FB, F32, false><<<grid, 256, 0, st>>>(P);
     else q8_mm_k<64, 64, 2, 2, FA, FB, F32, true><<<grid, 256, 0, st>>>(P);
     return kp_check_launch("q8_matmul");
+}
+
+template <int DT, int FX> int rows_launch(const RowArgs& P, int fmtw, hipStream_t st) {
+    const bool two = P.N >= 32 * 256;
+    const dim3 grid(cdiv(P.N, two ? 32 : 16), cdiv(P.M, 16));
+    if (two) {
+        if (fmtw == KP_E4M3) q8_rows_k<DT, FX, 0, 2><<<grid, 512, 0, st>>>(P);
+        else q8_rows_k<DT, FX, 1, 2><<<grid, 512, 0, st>>>(P);
+    } else {
+        if (fmtw == KP_E4M3) q8_rows_k<DT, FX, 0, 1><<<grid, 512, 0, st>>>(P);
+        else q8_rows_k<DT, FX, 1, 1><<<grid, 512, 0, st>>>(P);
+    }
+    return kp_check_launch("q8_linear_rows");
 }
 
 }  // namespace
@@ -389,6 +522,33 @@ int kp_q8_matmul(const unsigned char* a, long long lda, const unsigned char* sa,
     else if (dtype == KP_BF16) q8_mm_join_k<KP_BF16><<<grid, 256, 0, st>>>(ws, p.splits, bias, c, ldc, (int)M, (int)N);
     else q8_mm_join_k<KP_F16><<<grid, 256, 0, st>>>(ws, p.splits, bias, c, ldc, (int)M, (int)N);
     return kp_check_launch("q8_matmul join");
+}
+
+// Against packing x and the tiles (bf16, us): 4096 x 4096: 1 row 6.7 / 11.8, 16 rows 9.2 / 12.6, 32 rows 16.6 / 13.4; 8192 x 8192: 1 row
+// 17.3 / 23.7, 16 rows 20.9 / 24.1; 1024 x 1024, 64 rows 4.4 / 8.1; 4096 x 1000, 32 rows 6.7 / 8.8, 64 rows 12.0 / 9.1; 512 x 8192 (32
+// workgroups that walk 64 blocks each), 4 rows 10.6 / 11.3, 16 rows 14.8 / 12.2.  So: up to 16 rows, unless few workgroups walk far; more
+// where the walk is short and two rounds of workgroups are enough.
+int kp_q8_linear_rows_suits(long long M, long long N, long long K) {
+    if (M <= 4) return 1;
+    if (M <= 16) return K <= 4096 || N >= 4096;
+    return K <= 1024 && ((N + 15) / 16) * ((M + 15) / 16) <= 512;
+}
+
+int kp_q8_linear_rows(const void* x, long long ldx, int fmtx, const unsigned char* w, long long ldw, const unsigned char* sw, long long ldsw,
+                      int fmtw, const float* bias, void* y, long long ldy, long long M, long long N, long long K, int dtype, void* stream) {
+    KP_REQUIRE(x && w && sw && y && M > 0 && N > 0 && K > 0, "kp_q8_linear_rows: bad args (%lld x %lld x %lld)", M, N, K);
+    KP_REQUIRE((fmtx == KP_E4M3 || fmtx == KP_E5M2) && (fmtw == KP_E4M3 || fmtw == KP_E5M2), "kp_q8_linear_rows: unknown format %d / %d", fmtx, fmtw);
+    KP_REQUIRE(dtype == KP_F32 || dtype == KP_BF16 || dtype == KP_F16, "kp_q8_linear_rows: unknown dtype %d", dtype);
+    const long long nb = (K + Q8_BLOCK - 1) / Q8_BLOCK;
+    KP_REQUIRE(M < (1LL << 20) && N <= 0x7fffff00LL && K < (1LL << 30), "kp_q8_linear_rows: %lld x %lld x %lld is more than one call takes", M, N, K);
+    KP_REQUIRE(ldw >= nb * Q8_BLOCK && ldw % 16 == 0 && ((size_t)w & 15) == 0 && ldsw >= nb, "kp_q8_linear_rows: the weight's rows must be padded to whole blocks and start on multiples of 16 bytes (strides %lld, %lld)", ldw, ldsw);
+    KP_REQUIRE((M == 1 || ldx >= K) && ldy >= N, "kp_q8_linear_rows: row strides %lld, %lld for %lld and %lld columns", ldx, ldy, K, N);
+    RowArgs P{x, ldx, w, sw, ldw, ldsw, bias, y, ldy, (int)M, (int)N, (int)K, (int)nb};
+    const hipStream_t st = (hipStream_t)stream;
+    kp_count_bytes((double)N * K + (double)(M * K + M * N) * (dtype == KP_F32 ? 4 : 2));
+    if (dtype == KP_F32) return fmtx == KP_E4M3 ? rows_launch<KP_F32, 0>(P, fmtw, st) : rows_launch<KP_F32, 1>(P, fmtw, st);
+    if (dtype == KP_BF16) return fmtx == KP_E4M3 ? rows_launch<KP_BF16, 0>(P, fmtw, st) : rows_launch<KP_BF16, 1>(P, fmtw, st);
+    return fmtx == KP_E4M3 ? rows_launch<KP_F16, 0>(P, fmtw, st) : rows_launch<KP_F16, 1>(P, fmtw, st);
 }
 
 }  // extern "C"

@@ -122,8 +122,8 @@ def checkpoint8(x: torch.Tensor, fmt: str = 'e4m3') -> Packed8:
 def _form(rows, width, device):
     """Empty operand form: values padded to whole blocks, exponent bytes to whole words."""
     blocks = (width + BLOCK - 1) // BLOCK
-    return (torch.empty(rows, blocks * BLOCK, device=device, dtype=torch.uint8),
-            torch.empty(rows, (blocks + 3) // 4 * 4, device=device, dtype=torch.uint8))
+    return (torch.empty((rows, blocks * BLOCK), device=device, dtype=torch.uint8),
+            torch.empty((rows, (blocks + 3) // 4 * 4), device=device, dtype=torch.uint8))
 
 
 def pack8(x: torch.Tensor, fmt: str = 'e4m3') -> Packed8:
@@ -267,8 +267,15 @@ def linear8(x: torch.Tensor, weight, bias: torch.Tensor = None, fmt: str = 'e4m3
     m, rows, ld = as_rows(x)
     if rows == 0 or N == 0:
         return torch.empty(shape, device=x.device, dtype=x.dtype)
+    K = x.shape[-1]
     with device_of(x):
-        form = _form(rows, x.shape[-1], x.device)
-        call('kp_q8_pack', ptr(m), ld, ptr(form[0]), form[0].shape[1], ptr(form[1]), form[1].shape[1], rows, x.shape[-1],
-             DTYPES[x.dtype], code, stream_ptr())
+        if _lib.lib().kp_q8_linear_rows_suits(rows, N, K):
+            y = x.new_empty(shape)
+            v, s = weight.values, weight.scales
+            call('kp_q8_linear_rows', ptr(m), ld, code, ptr(v), v.shape[1], ptr(s), s.shape[1], FORMATS[weight.fmt], ptr(bias), ptr(y), N,
+                 rows, N, K, DTYPES[x.dtype], stream_ptr())
+            return y
+        form = _form(rows, K, x.device)
+        call('kp_q8_pack', ptr(m), ld, ptr(form[0]), form[0].shape[1], ptr(form[1]), form[1].shape[1], rows, K, DTYPES[x.dtype], code,
+             stream_ptr())
         return _product(form, code, (weight.values, weight.scales), FORMATS[weight.fmt], bias, shape, x.dtype)
