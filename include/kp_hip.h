@@ -567,7 +567,7 @@ long long kp_q8_pack_both_ws_floats(long long rows, long long cols);
 int kp_q8_matmul(const unsigned char* a, long long lda, const unsigned char* sa, long long ldsa, int fmta, const unsigned char* b,
                  long long ldb, const unsigned char* sb, long long ldsb, int fmtb, const float* bias, void* c, long long ldc, float* ws,
                  long long M, long long N, long long K, int dtype, void* stream);
-long long kp_q8_matmul_ws_floats(long long M, long long N, long long K);
+long long kp_q8_matmul_ws_floats(long long M, long long N, long long K, int dtype);
 /* y T [M][N] = sum_k P(x)[m][k] w[n][k] (+ bias[n]) for a few rows of x T [M][K], P(x) = x's row form in fmtx, formed on the way: what
  * kp_q8_pack + kp_q8_matmul give (up to the order of the fp32 additions), as one launch that streams w once for every 16 rows. */
 int kp_q8_linear_rows(const void* x, long long ldx, int fmtx, const unsigned char* w, long long ldw, const unsigned char* sw, long long ldsw,

@@ -11,6 +11,7 @@
 //                    sums (measured 6e-9 .. 4e-7 of the norm), at half its partner's rate.  Weight gradients go this way.
 //
 // Any order of the elements inside a block serves, as long as A and B agree: the fragments are read as the swizzle likes them.
+#include <math.h>
 #include "kp_mfma_util.h"
 #include "kp_q8_dev.h"
 
@@ -155,18 +156,15 @@ __global__ __launch_bounds__(64 * WGM * WGN, 2) void q8_mm_k(const MmArgs P) {
     // accumulators start at the bias of the lane's columns (the join adds it to split sums)
     const bool split = P.splits > 1;
     const int nw = n0 + wn * WN;
+    const auto rbias = __builtin_amdgcn_make_buffer_rsrc((void*)P.bias, 0, P.bias && !split ? P.N * 4 : 0, 0x00020000);
     f32x16 acc[TN][TM];
 #pragma unroll
     for (int n = 0; n < TN; ++n)
 #pragma unroll
         for (int g = 0; g < 4; ++g) {
-            float v[4] = {0.f, 0.f, 0.f, 0.f};
-            if (P.bias && !split) {
-                const int at = nw + n * 32 + g * 8 + fh * 4;
+            float v[4];   // (out of the resource's range -- no bias, or columns past the end -- loads give zero)
 #pragma unroll
-                for (int e = 0; e < 4; ++e)
-                    if (!EDGE || at + e < P.N) v[e] = P.bias[at + e];
-            }
+            for (int e = 0; e < 4; ++e) v[e] = __uint_as_float(__builtin_amdgcn_raw_buffer_load_b32(rbias, (nw + n * 32 + g * 8 + fh * 4 + e) * 4, 0, 0));
 #pragma unroll
             for (int m = 0; m < TM; ++m)
 #pragma unroll
@@ -240,6 +238,11 @@ __global__ __launch_bounds__(64 * WGM * WGN, 2) void q8_mm_k(const MmArgs P) {
         asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
         __builtin_amdgcn_s_barrier();
         asm volatile("" ::: "memory");
+        // (nothing is in flight here: named at this point, the exponent words cost no wait of their own where they are taken over)
+#pragma unroll
+        for (int i = 0; i < TM; ++i) asm volatile("" : "+v"(sc_next.a[i]));
+#pragma unroll
+        for (int i = 0; i < TN; ++i) asm volatile("" : "+v"(sc_next.b[i]));
         if (k + 2 < kb1) issue(buf, k + 2);
         buf ^= BUF;
         load_frags(f0, buf, 0);
@@ -441,27 +444,44 @@ __global__ __launch_bounds__(256) void q8_mm_join_k(const float* __restrict__ pa
     }
 }
 
-struct Plan { int bm, bn, splits, per_split; };
+struct Plan { int tile, splits, per_split; };
 
-// Tile and split from the sizes alone.
-Plan plan_of(int M, int N, int nb) {
-    Plan p;
-    p.bm = p.bn = (M >= 256 && N >= 256) ? 256 : (M >= 128 && N >= 128) ? 128 : 64;
-    const long long tiles = (long long)cdiv(M, p.bm) * cdiv(N, p.bn);
-    const int groups = (nb + 3) / 4;                 // splits start on multiples of four blocks (one word of exponent bytes)
-    int s = tiles >= 256 ? 1 : (int)(256 / tiles);
-    if (s > groups) s = groups;
-    if (s > 16) s = 16;
-    if (s < 1) s = 1;
-    p.per_split = (groups + s - 1) / s * 4;
-    p.splits = (nb + p.per_split - 1) / p.per_split;
-    return p;
+// Tile and split by a model of the time, from the sizes alone.  A step of 128 k-elements of w workgroups on a CU takes (us, fitted to
+// measurements of 22 shapes; right: fp32 results):
+//     64 x 64    0.15 + 0.18 w   0.23 + 0.29 w   (w <= 4)
+//     128 x 128  0.29 + 0.44 w   0.80 + 0.60 w   (w <= 2)
+//     256 x 256  1.95            3.2             (w = 1)
+// and a split's partial products are written and read once more, at 4 TB/s, by a launch of 3 us.  Against the largest tile that fits, split
+// until every CU has one (the first rule here): 777 x 1234 x 1000 18.3 -> 6.4 us, 1024^3 16.6 -> 5.2, 2048^3 36.6 -> 14.6, 512 x 4096 x 4096
+// 35.6 -> 19.7, 300 x 300 x 8192 20.3 -> 10.6.
+Plan plan_of(long long M, long long N, int nb, bool f32) {
+    static const struct { int tile, most; double base[2], each[2]; } T[3] = {
+        {64, 4, {0.15, 0.23}, {0.18, 0.29}}, {128, 2, {0.29, 0.80}, {0.44, 0.60}}, {256, 1, {0.0, 0.0}, {1.95, 3.2}}};
+    const int groups = (nb + 3) / 4;   // splits start on multiples of four blocks (one word of exponent bytes)
+    Plan best = {64, 1, groups * 4};
+    double least = 1e30;
+    for (const auto& t : T) {
+        if (t.tile > 64 && (M < t.tile || N < t.tile)) break;
+        const double tiles = (double)((M + t.tile - 1) / t.tile) * (double)((N + t.tile - 1) / t.tile);
+        for (int s = 1; s <= 32 && s <= groups; s *= 2) {
+            const int per = (groups + s - 1) / s * 4, splits = (nb + per - 1) / per;
+            const double work = tiles * splits, slots = 256.0 * t.most, full = floor(work / slots), rest = work - full * slots;
+            const double steps = per < nb ? per : nb, w = ceil(rest / 256.0);
+            double us = steps * (full * (t.base[f32] + t.each[f32] * t.most) + (w > 0 ? t.base[f32] + t.each[f32] * w : 0.0));
+            if (splits > 1) us += 3.0 + (double)M * (double)N * 8.0 * splits / 4e6;
+            if (us < least) {
+                least = us;
+                best = Plan{t.tile, splits, per};
+            }
+        }
+    }
+    return best;
 }
 
 template <int FA, int FB, bool F32> int mm_launch(const MmArgs& P, const Plan& p, hipStream_t st) {
     const unsigned grid = (unsigned)(P.tiles_m * P.tiles_n * P.splits);
-    if (p.bm == 256) q8_mm_k<256, 256, 4, 2, FA, FB, F32, false><<<grid, 512, 0, st>>>(P);
-    else if (p.bm == 128) q8_mm_k<128, 128, 2, 2, FA, FB, F32, false><<<grid, 256, 0, st>>>(P);
+    if (p.tile == 256) q8_mm_k<256, 256, 4, 2, FA, FB, F32, false><<<grid, 512, 0, st>>>(P);
+    else if (p.tile == 128) q8_mm_k<128, 128, 2, 2, FA, FB, F32, false><<<grid, 256, 0, st>>>(P);
     else q8_mm_k<64, 64, 2, 2, FA, FB, F32, true><<<grid, 256, 0, st>>>(P);
     return kp_check_launch("q8_matmul");
 }
@@ -483,9 +503,13 @@ template <int DT, int FX> int rows_launch(const RowArgs& P, int fmtw, hipStream_
 
 extern "C" {
 
-long long kp_q8_matmul_ws_floats(long long M, long long N, long long K) {
-    if (M <= 0 || N <= 0 || K <= 0 || M > 0x7fffff00LL || N > 0x7fffff00LL || K > (1LL << 23)) return 0;
-    const Plan p = plan_of((int)M, (int)N, (int)((K + Q8_BLOCK - 1) / Q8_BLOCK));
+static bool mm_sizes_ok(long long M, long long N, long long K) {
+    return M > 0 && N > 0 && K > 0 && M <= 0x7fffff00LL && N <= 0x1fffff00LL && K <= (1LL << 23);
+}
+
+long long kp_q8_matmul_ws_floats(long long M, long long N, long long K, int dtype) {
+    if (!mm_sizes_ok(M, N, K)) return 0;
+    const Plan p = plan_of(M, N, (int)((K + Q8_BLOCK - 1) / Q8_BLOCK), dtype == KP_F32);
     return p.splits > 1 ? p.splits * M * N : 0;
 }
 
@@ -496,19 +520,19 @@ int kp_q8_matmul(const unsigned char* a, long long lda, const unsigned char* sa,
     KP_REQUIRE((fmta == KP_E4M3 || fmta == KP_E5M2) && (fmtb == KP_E4M3 || fmtb == KP_E5M2), "kp_q8_matmul: unknown format %d / %d", fmta, fmtb);
     KP_REQUIRE(dtype == KP_F32 || dtype == KP_BF16 || dtype == KP_F16, "kp_q8_matmul: unknown dtype %d", dtype);
     const long long nb = (K + Q8_BLOCK - 1) / Q8_BLOCK, words = (nb + 3) / 4 * 4;
-    KP_REQUIRE(M <= 0x7fffff00LL && N <= 0x7fffff00LL && lda < (1LL << 23) && ldb < (1LL << 23),
-               "kp_q8_matmul: %lld x %lld x %lld is more than one call takes (2^23 along the product, 2^31 rows)", M, N, K);
+    KP_REQUIRE(mm_sizes_ok(M, N, K) && lda < (1LL << 23) && ldb < (1LL << 23),
+               "kp_q8_matmul: %lld x %lld x %lld is more than one call takes (2^23 along the product, 2^31 and 2^29 rows)", M, N, K);
     KP_REQUIRE(lda >= nb * Q8_BLOCK && ldb >= nb * Q8_BLOCK && lda % 16 == 0 && ldb % 16 == 0 && ((size_t)a & 15) == 0 && ((size_t)b & 15) == 0,
                "kp_q8_matmul: operand rows must be padded to whole blocks and start on multiples of 16 bytes (strides %lld, %lld)", lda, ldb);
     KP_REQUIRE(ldsa >= words && ldsb >= words && ldsa % 4 == 0 && ldsb % 4 == 0 && ((size_t)sa & 3) == 0 && ((size_t)sb & 3) == 0,
                "kp_q8_matmul: rows of exponent bytes must be padded to words (strides %lld, %lld)", ldsa, ldsb);
     KP_REQUIRE(ldc >= N, "kp_q8_matmul: output row stride %lld for %lld columns", ldc, N);
-    const Plan p = plan_of((int)M, (int)N, (int)nb);
+    const Plan p = plan_of(M, N, (int)nb, dtype == KP_F32);
     KP_REQUIRE(p.splits == 1 || ws, "kp_q8_matmul: this shape needs a workspace (kp_q8_matmul_ws_floats)");
     MmArgs P;
     P.a = a; P.sa = sa; P.b = b; P.sb = sb; P.lda = lda; P.ldsa = ldsa; P.ldb = ldb; P.ldsb = ldsb; P.bias = bias; P.c = c; P.ldc = ldc;
     P.part = ws; P.M = (int)M; P.N = (int)N; P.nb = (int)nb; P.dtype = dtype;
-    P.tiles_m = (int)cdiv(M, p.bm); P.tiles_n = (int)cdiv(N, p.bn); P.splits = p.splits; P.per_split = p.per_split;
+    P.tiles_m = (int)cdiv(M, p.tile); P.tiles_n = (int)cdiv(N, p.tile); P.splits = p.splits; P.per_split = p.per_split;
     KP_REQUIRE((long long)P.tiles_m * P.tiles_n * P.splits < (1LL << 31), "kp_q8_matmul: %lld x %lld is more than one call takes", M, N);
     kp_count_bytes((double)(M + N) * K + (double)M * N * (dtype == KP_F32 ? 4 : 2));
     const hipStream_t st = (hipStream_t)stream;

@@ -160,7 +160,7 @@ def _product(a, fmta, b, fmtb, bias, shape, dtype):
     """kp_q8_matmul of two operand forms (values, scales) into a new tensor of `shape` = [..., rows of b]."""
     M, N, K = a[0].shape[0], b[0].shape[0], a[0].shape[1]
     c = torch.empty(shape, device=a[0].device, dtype=dtype)
-    floats = _lib.lib().kp_q8_matmul_ws_floats(M, N, K)
+    floats = _lib.lib().kp_q8_matmul_ws_floats(M, N, K, DTYPES[dtype])
     ws = torch.empty(floats, device=c.device, dtype=torch.float32) if floats else None
     call('kp_q8_matmul', ptr(a[0]), K, ptr(a[1]), a[1].shape[1], fmta, ptr(b[0]), K, ptr(b[1]), b[1].shape[1], fmtb, ptr(bias), ptr(c), N,
          ptr(ws), M, N, K, DTYPES[dtype], stream_ptr())
