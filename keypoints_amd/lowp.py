@@ -111,19 +111,17 @@ def checkpoint8(x: torch.Tensor, fmt: str = 'e4m3') -> Packed8:
     if not _dense(x):
         x = x.contiguous()
     n = x.numel()
-    values = torch.empty(n, device=x.device, dtype=torch.uint8)
-    scales = torch.empty((n + BLOCK - 1) // BLOCK, device=x.device, dtype=torch.uint8)
+    values, scales = x.new_empty(n, dtype=torch.uint8), x.new_empty((n + BLOCK - 1) // BLOCK, dtype=torch.uint8)
     if n:
         with device_of(x):
             call('kp_q8_pack', ptr(x), n, ptr(values), n, ptr(scales), scales.numel(), 1, n, dcode, code, stream_ptr())
     return Packed8(values, scales, x.shape, x.stride(), x.dtype, fmt, True)
 
 
-def _form(rows, width, device):
-    """Empty operand form: values padded to whole blocks, exponent bytes to whole words."""
+def _form(rows, width, like):
+    """Empty operand form on `like`'s device: values padded to whole blocks, exponent bytes to whole words."""
     blocks = (width + BLOCK - 1) // BLOCK
-    return (torch.empty((rows, blocks * BLOCK), device=device, dtype=torch.uint8),
-            torch.empty((rows, (blocks + 3) // 4 * 4), device=device, dtype=torch.uint8))
+    return (like.new_empty((rows, blocks * BLOCK), dtype=torch.uint8), like.new_empty((rows, (blocks + 3) // 4 * 4), dtype=torch.uint8))
 
 
 def pack8(x: torch.Tensor, fmt: str = 'e4m3') -> Packed8:
@@ -134,7 +132,7 @@ def pack8(x: torch.Tensor, fmt: str = 'e4m3') -> Packed8:
         raise ValueError(f'pack8: the last dimension must hold at least one element, got shape {tuple(x.shape)}')
     m, rows, ld = as_rows(x.detach())
     width = x.shape[-1]
-    values, scales = _form(rows, width, x.device)
+    values, scales = _form(rows, width, x)
     if rows:
         with device_of(x):
             call('kp_q8_pack', ptr(m), ld, ptr(values), values.shape[1], ptr(scales), scales.shape[1], rows, width, dcode, code, stream_ptr())
@@ -145,11 +143,10 @@ def _pack_both(m, rows, ld, width, dcode, code, by_rows, by_cols, sums):
     """kp_q8_pack_both of a matrix: (row form, column form, column sums), each (None, None) / None where not asked for."""
     if not (by_rows or by_cols or sums):
         return (None, None), (None, None), None
-    dev = m.device
-    q = _form(rows, width, dev) if by_rows else (None, None)
-    qt = _form(width, rows, dev) if by_cols else (None, None)
-    colsum = torch.empty(width, device=dev, dtype=torch.float32) if sums else None
-    ws = torch.empty(_lib.lib().kp_q8_pack_both_ws_floats(rows, width), device=dev, dtype=torch.float32) if sums else None
+    q = _form(rows, width, m) if by_rows else (None, None)
+    qt = _form(width, rows, m) if by_cols else (None, None)
+    colsum = m.new_empty(width, dtype=torch.float32) if sums else None
+    ws = m.new_empty(_lib.lib().kp_q8_pack_both_ws_floats(rows, width), dtype=torch.float32) if sums else None
     call('kp_q8_pack_both', ptr(m), ld, ptr(q[0]), q[0].shape[1] if by_rows else 0, ptr(q[1]), q[1].shape[1] if by_rows else 0,
          ptr(qt[0]), qt[0].shape[1] if by_cols else 0, ptr(qt[1]), qt[1].shape[1] if by_cols else 0, ptr(ws), ptr(colsum),
          rows, width, dcode, code, stream_ptr())
@@ -159,9 +156,9 @@ def _pack_both(m, rows, ld, width, dcode, code, by_rows, by_cols, sums):
 def _product(a, fmta, b, fmtb, bias, shape, dtype):
     """kp_q8_matmul of two operand forms (values, scales) into a new tensor of `shape` = [..., rows of b]."""
     M, N, K = a[0].shape[0], b[0].shape[0], a[0].shape[1]
-    c = torch.empty(shape, device=a[0].device, dtype=dtype)
+    c = a[0].new_empty(shape, dtype=dtype)
     floats = _lib.lib().kp_q8_matmul_ws_floats(M, N, K, DTYPES[dtype])
-    ws = torch.empty(floats, device=c.device, dtype=torch.float32) if floats else None
+    ws = c.new_empty(floats, dtype=torch.float32) if floats else None
     call('kp_q8_matmul', ptr(a[0]), K, ptr(a[1]), a[1].shape[1], fmta, ptr(b[0]), K, ptr(b[1]), b[1].shape[1], fmtb, ptr(bias), ptr(c), N,
          ptr(ws), M, N, K, DTYPES[dtype], stream_ptr())
     return c
@@ -275,7 +272,7 @@ def linear8(x: torch.Tensor, weight, bias: torch.Tensor = None, fmt: str = 'e4m3
             call('kp_q8_linear_rows', ptr(m), ld, code, ptr(v), v.shape[1], ptr(s), s.shape[1], FORMATS[weight.fmt], ptr(bias), ptr(y), N,
                  rows, N, K, DTYPES[x.dtype], stream_ptr())
             return y
-        form = _form(rows, K, x.device)
+        form = _form(rows, K, x)
         call('kp_q8_pack', ptr(m), ld, ptr(form[0]), form[0].shape[1], ptr(form[1]), form[1].shape[1], rows, K, DTYPES[x.dtype], code,
              stream_ptr())
         return _product(form, code, (weight.values, weight.scales), FORMATS[weight.fmt], bias, shape, x.dtype)

@@ -16,49 +16,51 @@ from .runtime import device_of, require_device, stream_ptr
 
 
 def _forward(x, weight, bias, eps, stats, fmt):
+    """-> y, x as rows, its row stride, [means | deviations' reciprocals], 8-bit copy, its exponents (each None where not asked for)."""
     m, rows, ld = as_rows(x)
     C = x.shape[-1]
     y = x.new_empty(x.shape)
-    mean = rstd = q = s = None
+    st = q = s = None
     if stats:
-        mean, rstd = x.new_empty(rows, dtype=torch.float32), x.new_empty(rows, dtype=torch.float32)
+        st = x.new_empty((2, rows), dtype=torch.float32)
     if fmt:
-        q = torch.empty(rows, C, device=x.device, dtype=torch.uint8)
-        s = torch.empty(rows, (C + BLOCK - 1) // BLOCK, device=x.device, dtype=torch.uint8)
+        q = x.new_empty((rows, C), dtype=torch.uint8)
+        s = x.new_empty((rows, (C + BLOCK - 1) // BLOCK), dtype=torch.uint8)
     if rows:
+        at = ptr(st)
         with device_of(x):
-            call('kp_layer_norm_fwd', ptr(m), ld, ptr(weight), ptr(bias), eps, ptr(y), C, ptr(mean), ptr(rstd), ptr(q), ptr(s),
+            call('kp_layer_norm_fwd', ptr(m), ld, ptr(weight), ptr(bias), eps, ptr(y), C, at, at + 4 * rows if stats else None, ptr(q), ptr(s),
                  FORMATS[fmt] if fmt else 0, rows, C, DTYPES[x.dtype], stream_ptr())
-    return y, m, ld, mean, rstd, q, s
+    return y, m, ld, st, q, s
 
 
 class _LayerNorm(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, weight, bias, eps, keep):
-        y, m, ld, mean, rstd, q, s = _forward(x, weight, bias, eps, True, keep)
+        y, m, ld, st, q, s = _forward(x, weight, bias, eps, True, keep)
         ctx.args = (keep, ld)
-        ctx.save_for_backward(weight, mean, rstd, q if keep else m, s)
+        ctx.save_for_backward(weight, st, q if keep else m, s)
         return y
 
     @staticmethod
     @once_differentiable
     def backward(ctx, dy):
         keep, ldx = ctx.args
-        weight, mean, rstd, kept, s = ctx.saved_tensors
+        weight, st, kept, s = ctx.saved_tensors
         need_x, need_w, need_b = ctx.needs_input_grad[:3]
         g, rows, ldg = as_rows(dy)
-        C, dev = dy.shape[-1], dy.device
-        f32 = dict(device=dev, dtype=torch.float32)
-        make = torch.empty if rows else torch.zeros   # (no rows: nothing is launched)
+        C = dy.shape[-1]
+        make = st.new_empty if rows else st.new_zeros   # (no rows: nothing is launched)
         dx = dy.new_empty(dy.shape) if need_x else None
-        dw = make(C, **f32) if need_w else None
-        db = make(C, **f32) if need_b else None
+        dw = make(C) if need_w else None
+        db = make(C) if need_b else None
         if rows:
-            ws = torch.empty(_lib.lib().kp_layer_norm_bwd_ws_floats(rows, C), **f32) if need_w or need_b else None
+            ws = st.new_empty(_lib.lib().kp_layer_norm_bwd_ws_floats(rows, C)) if need_w or need_b else None
+            at = ptr(st)
             with device_of(dy):
                 call('kp_layer_norm_bwd', ptr(g), ldg, None if keep else ptr(kept), C if keep else ldx, ptr(kept) if keep else None, ptr(s),
-                     FORMATS[keep] if keep else 0, ptr(weight), ptr(mean), ptr(rstd), ptr(dx), C, ptr(ws), ptr(dw), ptr(db),
-                     rows, C, DTYPES[dy.dtype], stream_ptr())
+                     FORMATS[keep] if keep else 0, ptr(weight), at, at + 4 * rows, ptr(dx), C, ptr(ws), ptr(dw), ptr(db), rows, C,
+                     DTYPES[dy.dtype], stream_ptr())
         return dx, dw, db, None, None
 
 
