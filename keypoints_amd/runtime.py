@@ -380,3 +380,20 @@ def set_keep_saved_activations(on: bool) -> None:
     _KEEP_SAVED = bool(on)
 
 
+_SAVED_FORMAT = None
+
+
+def saved_activations():
+    """None, or the 8-bit format ('e4m3', 'e5m2'; keypoints_amd.lowp) in which a Unit keeps what its backward reads -- every layer's input and
+    conv output -- between the two passes: half the memory of 16-bit storage, a quarter of fp32's, for one packing pass per tensor and one
+    back.  The backward then runs on the kept values (each off by at most 2^-4 / 2^-3 of itself): outputs and running statistics do not
+    change, gradients are approximate.  In this mode weight gradients run on the backward's own stream (a side stream would keep every
+    unpacked tensor of the Unit alive) and the source / target pair of a Transporter as two calls.  OFF (None) by default."""
+    return _SAVED_FORMAT
+
+
+def set_saved_activations(fmt) -> None:
+    global _SAVED_FORMAT
+    if fmt not in (None, 'e4m3', 'e5m2'):
+        raise ValueError(f"saved activations: None, 'e4m3' or 'e5m2', not {fmt!r}")
+    _SAVED_FORMAT = fmt

@@ -26,6 +26,7 @@ import torch.nn as nn
 from . import _lib
 from ._lib import call, ptr, try_call
 from . import runtime
+from .lowp import checkpoint8
 from .runtime import f32c, precision_dtype, require_device, stream_ptr
 
 TAILS = {None: _lib.TAIL_NONE, 'M': _lib.TAIL_MAXPOOL2, 'U': _lib.TAIL_UPSAMPLE2}
@@ -260,7 +261,7 @@ def pair_ok(unit, N, Cin, H, W, out_t=False):
     """True if `UnitFunction._forward_pair` can run source + target frame of N images each through this Unit as one batch: 16-bit
     storage, train-mode BatchNorm with a momentum in every 3x3 layer, no pool / upsample, every layer and the head on a kernel that
     has the pair form AND the fused BatchNorm-input forms the backward of the target half uses (the Pong-class nets of vgg.py:53,66)."""
-    if not (runtime.pair_calls() and runtime.fuse_bn_input() and unit.precision in ('bf16', 'fp16') and unit.sync_bn is None):
+    if not (runtime.pair_calls() and runtime.fuse_bn_input() and runtime.saved_activations() is None and unit.precision in ('bf16', 'fp16') and unit.sync_bn is None):
         return False
     try:
         plan = unit.plan()
@@ -296,6 +297,31 @@ def _materialise(fin, N, H, W, C, pad, tdt, code, st):
     a = torch.empty(N, H + 2 * pad, W + 2 * pad, C, device=fin['y'].device, dtype=tdt)
     call('kp_bn_act_fwd', ptr(fin['y']), *fin['bn'], fin['slope'], TAILS[None], ptr(a), pad, None, N, H, W, C, code, st)
     return a
+
+
+class _Kept:
+    """A saved activation in 8 bits (runtime.saved_activations): unpacked when the backward first asks, until it lets go."""
+    __slots__ = ('packed', 'tensor')
+
+    def __init__(self, t, fmt):
+        self.packed, self.tensor = checkpoint8(t, fmt), None
+
+    def get(self):
+        if self.tensor is None:
+            self.tensor = self.packed.unpack()
+        return self.tensor
+
+    def drop(self):
+        self.tensor = None
+
+
+def _opened(v):
+    """A saved activation as a tensor: itself, unpacked (_Kept), or a pending BatchNorm input (`fin`) with its conv output opened."""
+    if isinstance(v, _Kept):
+        return v.get()
+    if isinstance(v, dict):
+        return dict(v, y=_opened(v['y']))
+    return v
 
 
 def _wgrad_layer(sv, dy, gw, parts, N, H, W, C, K, dp, tdt, code, dev):
@@ -396,6 +422,9 @@ class UnitFunction(torch.autograd.Function):
         H0, W0 = H, W
         saved = []
         fin = None   # pending BatchNorm-apply of the previous layer, fused into the next convolution (None: `a` is materialised)
+        fmt8 = runtime.saved_activations() if record else None
+        kept = (lambda t: _Kept(t, fmt8)) if fmt8 else (lambda t: t)
+        y_kept = None   # the previous layer's conv output as it is saved
         packs = _pack_unit(plan, Cin, Cp0, record, dev, tdt, code, st)
         C = Cin
         for idx, stp in enumerate(plan[:-1]):
@@ -506,8 +535,10 @@ class UnitFunction(torch.autograd.Function):
                 call('kp_bn_act_fwd', ptr(y), ptr(mean), ptr(invstd), ptr(gamma), ptr(beta), stp['slope'], TAILS[tail],
                      ptr(a_next), out_pad, ptr(argmax), N, H, W, K, code, st)
             if record:
-                saved.append(dict(a=a, fin=fin, y=y, mean=mean, invstd=invstd, argmax=argmax, wd=wd, H=H, W=W, C=C, Cl=Cl, K=K,
-                                  eval_bn=bn is not None and not training))
+                fin_kept = dict(fin, y=y_kept) if fin is not None else None
+                y_kept = kept(y)
+                saved.append(dict(a=kept(a) if a is not None else None, fin=fin_kept, y=y_kept, mean=mean, invstd=invstd, argmax=argmax,
+                                  wd=wd, H=H, W=W, C=C, Cl=Cl, K=K, eval_bn=bn is not None and not training))
             a, fin, C, H, W = a_next, fin_next, K, Ho, Wo
         head = plan[-1]
         hconv = head['conv']
@@ -528,7 +559,8 @@ class UnitFunction(torch.autograd.Function):
             else:
                 call('kp_head_fwd', ptr(a), ptr(hconv.weight), ptr(hconv.bias), head['slope'], ptr(out), N, H, W, C, Kout, code, st)
         if record:
-            ctx.unit, ctx.saved, ctx.head_in = unit, saved, (a if fin is None else fin)
+            ctx.unit, ctx.saved, ctx.head_in = unit, saved, (kept(a) if fin is None else dict(fin, y=y_kept))
+            ctx.fmt8 = fmt8
             ctx.save_for_backward(out)   # an OUTPUT kept as a plain ctx attribute would be a reference cycle
             ctx.dims = (N, Cin, H0, W0, H, W, C, Kout, pad0)
             ctx.cp0 = Cp0
@@ -615,7 +647,8 @@ class UnitFunction(torch.autograd.Function):
             raise RuntimeError('keypoints_amd Unit: backward was already run for this forward; the saved activations are '
                                'released after the first backward (for retain_graph=True call '
                                'keypoints_amd.runtime.set_keep_saved_activations(True) before the forward)')
-        unit, saved, a_last = ctx.unit, ctx.saved, ctx.head_in
+        unit, saved, a_last = ctx.unit, ctx.saved, _opened(ctx.head_in)
+        fmt8 = getattr(ctx, 'fmt8', None)
         (out,) = ctx.saved_tensors
         N, Cin, H0, W0, Hh, Wh, Ch, Kout, pad0 = ctx.dims
         plan = unit.plan()
@@ -629,7 +662,7 @@ class UnitFunction(torch.autograd.Function):
         # the weight-gradient side stream is taken when the first layer asks for it: a Unit whose weight gradients all run inline
         # (Pong-class layers, below) then neither touches nor joins it (two events per Unit backward: 0.4 % of a config-2 step)
         side = None
-        side_ok = runtime.multi_stream('wgrad') and not runtime.nested_fork_under_capture()   # (a side stream OF a side stream inside a stream capture crashes hipStreamEndCapture, ROCm 7.0)
+        side_ok = fmt8 is None and runtime.multi_stream('wgrad') and not runtime.nested_fork_under_capture()   # (a side stream OF a side stream inside a stream capture crashes hipStreamEndCapture, ROCm 7.0)
         keep = []
         gv = arena.views
         c1 = ctx.c1
@@ -676,10 +709,15 @@ class UnitFunction(torch.autograd.Function):
                 hgrads = hgrads[:3] + (ptr(hws),)
             call('kp_head_bwd', ptr(gout), ptr(out), ptr(a_last), ptr(hconv.weight), head['slope'], *hgrads,
                  N, Hh, Wh, Ch, Kout, code, st)
+        a_last = None
+        if isinstance(ctx.head_in, _Kept):
+            ctx.head_in.drop()
         gp = 0   # border width of g (0 = plain, 1 = padded-domain gradient that still needs folding)
         pending_red = None   # (partial rows, count) of the NEXT layer's BatchNorm-backward sums, left by a fused data gradient
         for idx in range(len(saved) - 1, -1, -1):
             stp, sv = plan[idx], saved[idx]
+            if fmt8 is not None:
+                sv = dict(sv, a=_opened(sv['a']), fin=_opened(sv['fin']), y=_opened(sv['y']))
             conv, bn = stp['conv'], stp['bn']
             H, W, C, K = sv['H'], sv['W'], sv['C'], sv['K']
             tail = stp['tail']
@@ -758,7 +796,7 @@ class UnitFunction(torch.autograd.Function):
                     svb, bnb = saved[idx - 1], below['bn']
                     rows_b = _lib.lib().kp_conv_dgrad_bnred_rows(N, H, W, K, C, code)
                     part_b = torch.empty(rows_b, 2, C, device=dev, dtype=torch.float32)
-                    call('kp_conv_dgrad_bnred', ptr(dy), ptr(sv['wd']), ptr(gx), ptr(svb['y']), ptr(svb['mean']), ptr(svb['invstd']),
+                    call('kp_conv_dgrad_bnred', ptr(dy), ptr(sv['wd']), ptr(gx), ptr(_opened(svb['y'])), ptr(svb['mean']), ptr(svb['invstd']),
                          ptr(bnb.weight if bnb is not None else None), ptr(bnb.bias if bnb is not None else None), below['slope'],
                          ptr(part_b), N, H, W, K, C, code, st)
                     pending_red = (part_b, rows_b)
@@ -790,6 +828,11 @@ class UnitFunction(torch.autograd.Function):
                 keep.append((dy, sv['a'], sv['fin']))
                 if unit.layer_done is not None:   # a gradient reducer reads the arena from this stream
                     cur.wait_stream(side)
+            if fmt8 is not None:   # (the layer below still reads its own conv output, unpacked above where this layer's input was it)
+                for v in (saved[idx]['a'], saved[idx]['y']):
+                    if isinstance(v, _Kept):
+                        v.drop()
+                sv = None
             unit._layer_done(idx)   # the arena slots of plan steps >= idx (and of the head) are final from here on
         dx = dx2 = None
         if need_x and in_t:
