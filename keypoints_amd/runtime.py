@@ -2,6 +2,7 @@
 from __future__ import annotations
 
 import contextlib
+import contextvars
 
 import torch
 
@@ -65,7 +66,10 @@ def f32c(t: torch.Tensor) -> torch.Tensor:
 # encoder runs on a side stream of the feature encoder's.  Results do not depend on it (every kernel is deterministic).
 _multi_stream = True
 _side_streams = {}     # (device index, parent stream id, role) -> torch.cuda.Stream
-_parents = {}          # side stream -> the stream it was forked from
+# the stream a side block (`with side:`) was forked from, inside it; None outside.  A property of the running block, not of the stream it
+# runs on: torch hands streams out of a pool of 32 in turn, so a stream an application (or a graph capture) gets may be one that was once
+# taken as a side stream here
+_FORKED = contextvars.ContextVar('keypoints_amd_forked_from', default=None)
 _used = set()          # side streams with work their parent has not waited for yet
 
 
@@ -91,16 +95,24 @@ def side_stream(role: str) -> torch.cuda.Stream:
     key = (cur.device.index, cur.stream_id, role)
     s = _side_streams.get(key)
     if s is None:
-        s = _side_streams[key] = torch.cuda.Stream(device=cur.device)
-        _parents[s] = cur
+        for _ in range(33):   # (the pool may come round to the current stream itself)
+            s = torch.cuda.Stream(device=cur.device)
+            if s != cur:
+                break
+        _side_streams[key] = s
     _used.add(s)
     return s
 
 
-def nested_fork_under_capture() -> bool:
-    """True when torch's current stream is itself a side stream and a stream capture is in progress on it."""
-    cur = torch.cuda.current_stream()
-    return cur in _parents and torch.cuda.is_current_stream_capturing()
+def forked_from():
+    """The stream this code's side block was forked from (None outside a side block).  A forward notes it for its backward, which the autograd
+    engine runs on the same stream in no block."""
+    return _FORKED.get()
+
+
+def nested_fork_under_capture(forked) -> bool:
+    """True when torch's current stream was forked from another (`forked`, see forked_from) and a stream capture is in progress on it."""
+    return forked is not None and torch.cuda.is_current_stream_capturing()
 
 
 def join_side_streams() -> None:
@@ -116,17 +128,16 @@ def join_side_streams() -> None:
             _used.discard(s)
 
 
-def join_after_backward() -> None:
+def join_after_backward(forked) -> None:
     """Called at the end of a Unit's backward, on the stream the autograd engine runs it on (= the stream of its forward).
-    If that is a side stream, the stream it was forked from waits for it here: by the time `backward()` returns, that
+    If the forward ran in a side block, the stream it was forked from (`forked`) waits here: by the time `backward()` returns, that
     wait is enqueued, so whatever the caller enqueues next on the forward's stream (`p.grad`, the optimiser, the gradient
     reducer) sees finished arenas.  (An engine callback -- `queue_callback` -- would be the general hook, but it runs on
     the engine's worker thread, whose thread-local current stream is the legacy default stream: waiting THERE on a
     capturing stream aborts the capture of keypoints_amd.graph.)"""
-    cur = torch.cuda.current_stream()
-    parent = _parents.get(cur)
-    if parent is not None:
-        parent.wait_stream(cur)
+    if forked is not None:
+        cur = torch.cuda.current_stream()
+        forked.wait_stream(cur)
         _used.discard(cur)
 
 
@@ -171,10 +182,12 @@ class _SideBlock:
         if self._o._stream is not None:
             self._ctx = torch.cuda.stream(self._o._stream)
             self._ctx.__enter__()
+            self._token = _FORKED.set(self._o._cur)
         return self
 
     def __exit__(self, *exc):
         if self._o._stream is not None:
+            _FORKED.reset(self._token)
             self._ctx.__exit__(*exc)
         return False
 

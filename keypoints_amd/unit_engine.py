@@ -566,6 +566,7 @@ class UnitFunction(torch.autograd.Function):
             ctx.cp0 = Cp0
             ctx.c1 = C1
             ctx.fmt = (bool(in_t), bool(out_t))
+            ctx.forked = runtime.forked_from()
         return out
 
     @staticmethod
@@ -636,6 +637,7 @@ class UnitFunction(torch.autograd.Function):
             ctx.cp0 = Cin
             ctx.c1 = 0
             ctx.fmt = (False, bool(out_t))
+            ctx.forked = runtime.forked_from()
         return out_s, out
 
     @staticmethod
@@ -662,7 +664,7 @@ class UnitFunction(torch.autograd.Function):
         # the weight-gradient side stream is taken when the first layer asks for it: a Unit whose weight gradients all run inline
         # (Pong-class layers, below) then neither touches nor joins it (two events per Unit backward: 0.4 % of a config-2 step)
         side = None
-        side_ok = fmt8 is None and runtime.multi_stream('wgrad') and not runtime.nested_fork_under_capture()   # (a side stream OF a side stream inside a stream capture crashes hipStreamEndCapture, ROCm 7.0)
+        side_ok = fmt8 is None and runtime.multi_stream('wgrad') and not runtime.nested_fork_under_capture(ctx.forked)   # (a side stream OF a side stream inside a stream capture crashes hipStreamEndCapture, ROCm 7.0)
         keep = []
         gv = arena.views
         c1 = ctx.c1
@@ -851,6 +853,6 @@ class UnitFunction(torch.autograd.Function):
             cur.wait_stream(side)
             runtime._used.discard(side)
             keep.clear()
-        runtime.join_after_backward()   # a backward that runs on a side stream itself is joined when the pass ends
+        runtime.join_after_backward(ctx.forked)   # a backward that runs on a side stream itself is joined when the pass ends
         unit._after_backward()
         return (dx, None, None, None, None, dx2) + (None,) * len(params)
