@@ -568,11 +568,13 @@ int kp_q8_matmul(const unsigned char* a, long long lda, const unsigned char* sa,
                  long long ldb, const unsigned char* sb, long long ldsb, int fmtb, const float* bias, void* c, long long ldc, float* ws,
                  long long M, long long N, long long K, int dtype, void* stream);
 long long kp_q8_matmul_ws_floats(long long M, long long N, long long K, int dtype);
-/* y T [M][N] = sum_k P(x)[m][k] w[n][k] (+ bias[n]) for a few rows of x T [M][K], P(x) = x's row form in fmtx, formed on the way: what
- * kp_q8_pack + kp_q8_matmul give (up to the order of the fp32 additions), as one launch that streams w once for every 16 rows. */
-int kp_q8_linear_rows(const void* x, long long ldx, int fmtx, const unsigned char* w, long long ldw, const unsigned char* sw, long long ldsw,
-                      int fmtw, const float* bias, void* y, long long ldy, long long M, long long N, long long K, int dtype, void* stream);
-int kp_q8_linear_rows_suits(long long M, long long N, long long K);   /* 1 where that is the faster way (any M < 2^20 is taken) */
+/* y T [M][N] = sum_k P(x)[m][k] w[n][k] (+ bias[n]) for x T [M][K], P(x) = x's row form in fmtx, formed in registers: what kp_q8_pack +
+ * kp_q8_matmul give (up to the order of the fp32 additions) in one launch, for a few rows (w is streamed once for every 16) or a few
+ * columns (N <= 128: x is read once). */
+int kp_q8_linear(const void* x, long long ldx, int fmtx, const unsigned char* w, long long ldw, const unsigned char* sw, long long ldsw,
+                 int fmtw, const float* bias, void* y, long long ldy, long long M, long long N, long long K, int dtype, void* stream);
+/* 1 where that is the faster way (kp_q8_linear takes any shape below 2^20 rows, and 2^31 where N <= 128) */
+int kp_q8_linear_suits(long long M, long long N, long long K);
 
 /* ---- layer norm ----------------------------------------------------------------------------------------------------------------
  * Per row of C elements: y = (x - mean) * rstd * w + b, rstd = 1 / sqrt(mean((x - mean)^2) + eps).  w, b fp32 or NULL (1, 0).  mean, rstd

@@ -53,6 +53,7 @@ template <int DT> __device__ __forceinline__ uint32_t el_pack(float lo, float hi
 typedef unsigned int q8_u32x4_e2 __attribute__((ext_vector_type(4), aligned(2)));
 typedef unsigned int q8_u32x4_e4 __attribute__((ext_vector_type(4), aligned(4)));
 typedef unsigned int q8_u32x2_e1 __attribute__((ext_vector_type(2), aligned(1)));
+typedef unsigned int q8_u32x2_e2 __attribute__((ext_vector_type(2), aligned(2)));
 template <int DT> struct El8 { q8_u32x4 w[DT == KP_F32 ? 2 : 1]; };   // as loaded
 template <int DT> __device__ __forceinline__ El8<DT> el_raw8(const void* p, long long i) {
     El8<DT> r;

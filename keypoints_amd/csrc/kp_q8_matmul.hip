@@ -310,11 +310,73 @@ __global__ __launch_bounds__(64 * WGM * WGN, 2) void q8_mm_k(const MmArgs P) {
     else store_rows(std::integral_constant<int, KP_F16>{});
 }
 
-// Few rows of x in their own type against a packed matrix: y[m][n] = P(x)[m] . W[n] (+ bias).  One launch: a wave packs its own blocks of up
-// to 16 rows of x in registers (the exponent goes straight into the instruction) and streams 16 rows of W past them, 16 x 16 x 128 a
-// block; the 8 waves of a workgroup take every 8th block and join through LDS in wave order.  Bound by the bytes of W and, for a few
-// million of them, by the way to memory and back: every wave has U blocks of loads in flight before its first product.  NT: groups of 16
-// rows of W a wave; two once that still gives every CU a workgroup, which halves the packing of x.
+// ---- x in its own type against a packed matrix: y[m][n] = P(x)[m] . W[n] (+ bias), one launch, no packed x in memory ---------------------
+// A wave packs 16 rows of x in registers, where the 16 x 16 x 128 instruction wants them: lane r16 + 16 quarter holds elements quarter * 16 .. + 15
+// and 64 further of row r16's block; the exponent goes straight into the instruction.
+template <int DT> struct Raw32 { El8<DT> e[4]; };
+template <int DT> __device__ __forceinline__ Raw32<DT> raw_block(const void* x, long long row_at, int k0, int quarter, int K, bool live) {
+    Raw32<DT> r;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        const int k = k0 + (i >> 1) * 64 + quarter * 16 + (i & 1) * 8;
+        r.e[i] = el_raw8_any<DT>(x, row_at + k, live ? K - k : 0);
+    }
+    return r;
+}
+// bytes (into fx) and exponent byte of this lane's row; all lanes of the wave are active
+template <int DT, int FMT> __device__ __forceinline__ uint32_t pack_rows16(const Raw32<DT>& raw, Frag8& fx) {
+    uint32_t m = 0;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) m = q8_raw_max<DT>(m, q8_raw_peak<DT>(raw.e[i]));
+    m = q8_raw_max<DT>(m, (uint32_t)__shfl_xor((int)m, 16, 64));   // the row's four lanes
+    m = q8_raw_max<DT>(m, (uint32_t)__shfl_xor((int)m, 32, 64));
+    if constexpr (DT != KP_F32) m = q8_umax(m & 0xffffu, m >> 16);
+    const uint32_t bits = q8_raw_bits<DT>(m);
+    if (__any(q8_plain<FMT>(bits))) {
+        float v[4][8];
+        uint32_t t = 0;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            el_unpack8<DT>(raw.e[i], v[i]);
+            t = q8_umax(t, q8_mag8(v[i]));
+        }
+        t = q8_umax(t, (uint32_t)__shfl_xor((int)t, 16, 64));
+        t = q8_umax(t, (uint32_t)__shfl_xor((int)t, 32, 64));
+        const uint32_t byte = q8_scale_byte<FMT>(t);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            const q8_u32x2 o = q8_cvt8<FMT>(v[i], q8_down(byte));
+            fx.v[2 * i] = (int)o[0];
+            fx.v[2 * i + 1] = (int)o[1];
+        }
+        return byte;
+    }
+    const uint32_t byte = q8_scale_byte<FMT>(bits);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        const q8_u32x2 o = q8_scaled8<DT, FMT>(raw.e[i], q8_up(byte));
+        fx.v[2 * i] = (int)o[0];
+        fx.v[2 * i + 1] = (int)o[1];
+    }
+    return byte;
+}
+// acc += 16 rows of W (its fragment and exponent byte) times 16 rows of x over a block; F32: exactly, through bfloat16
+template <int FW, int FX, bool F32> __device__ __forceinline__ f32x4 mma16(const Frag8& fw, int ew, const Frag8& fx, uint32_t ex, f32x4 acc) {
+    if constexpr (!F32) return __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(fw.v, fx.v, acc, FW, FX, 0, ew, 0, (int)ex);
+    else {
+        typedef __bf16 bf8 __attribute__((ext_vector_type(8)));
+        const float uw = q8_up((uint32_t)ew & 255u), ux = q8_up(ex);
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+            acc = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf8, q8_bf16x8<FW>(fw.v, i, uw)), __builtin_bit_cast(bf8, q8_bf16x8<FX>(fx.v, i, ux)), acc, 0, 0, 0);
+        return acc;
+    }
+}
+
+// Few rows: 16 rows of W a wave stream past the packed rows, 16 x 16 x 128 a block; the 8 waves of a workgroup take every 8th block and join
+// through LDS in wave order.  Bound by the bytes of W and, for a few million of them, by the way to memory and back: every wave has U blocks
+// of loads in flight before its first product.  NT: groups of 16 rows of W a wave; two once that still gives every CU a workgroup, which
+// halves the packing of x.
 struct RowArgs {
     const void* x;
     long long ldx;
@@ -345,73 +407,25 @@ __global__ __launch_bounds__(512) void q8_rows_k(const RowArgs P) {
     for (int kb0 = wave; kb0 < P.nb; kb0 += NW * U) {
         Frag8 fw[U][NT];
         int es[U][NT];
-        El8<DT> raw[U][4];   // elements quarter * 16 .. + 15 and 64 further, as the fragment of W has them
+        Raw32<DT> raw[U];
 #pragma unroll
         for (int u = 0; u < U; ++u) {
             const int kb = kb0 + u * NW < P.nb ? kb0 + u * NW : P.nb - 1;
-            const bool live = mine && kb0 + u * NW < P.nb;
 #pragma unroll
             for (int t = 0; t < NT; ++t) {
                 fw[u][t].h[0] = *reinterpret_cast<const u32x4*>(w[t] + (long long)kb * 128);
                 fw[u][t].h[1] = *reinterpret_cast<const u32x4*>(w[t] + (long long)kb * 128 + 64);
                 es[u][t] = sw[t][kb];
             }
-#pragma unroll
-            for (int i = 0; i < 4; ++i) {
-                const int k = kb * 128 + (i >> 1) * 64 + quarter * 16 + (i & 1) * 8;
-                raw[u][i] = el_raw8_any<DT>(P.x, xrow + k, live ? P.K - k : 0);
-            }
+            raw[u] = raw_block<DT>(P.x, xrow, kb * 128, quarter, P.K, mine && kb0 + u * NW < P.nb);
         }
 #pragma unroll
         for (int u = 0; u < U; ++u) {
             if (kb0 + u * NW >= P.nb) break;
-            uint32_t m = 0;
-#pragma unroll
-            for (int i = 0; i < 4; ++i) m = q8_raw_max<DT>(m, q8_raw_peak<DT>(raw[u][i]));
-            m = q8_raw_max<DT>(m, (uint32_t)__shfl_xor((int)m, 16, 64));   // the row's four lanes
-            m = q8_raw_max<DT>(m, (uint32_t)__shfl_xor((int)m, 32, 64));
-            if constexpr (DT != KP_F32) m = q8_umax(m & 0xffffu, m >> 16);
-            const uint32_t bits = q8_raw_bits<DT>(m);
             Frag8 fx;
-            uint32_t byte;
-            if (__any(q8_plain<FX + 1>(bits))) {
-                float v[4][8];
-                uint32_t t = 0;
+            const uint32_t byte = pack_rows16<DT, FX + 1>(raw[u], fx);
 #pragma unroll
-                for (int i = 0; i < 4; ++i) {
-                    el_unpack8<DT>(raw[u][i], v[i]);
-                    t = q8_umax(t, q8_mag8(v[i]));
-                }
-                t = q8_umax(t, (uint32_t)__shfl_xor((int)t, 16, 64));
-                t = q8_umax(t, (uint32_t)__shfl_xor((int)t, 32, 64));
-                byte = q8_scale_byte<FX + 1>(t);
-#pragma unroll
-                for (int i = 0; i < 4; ++i) {
-                    const q8_u32x2 o = q8_cvt8<FX + 1>(v[i], q8_down(byte));
-                    fx.v[2 * i] = (int)o[0];
-                    fx.v[2 * i + 1] = (int)o[1];
-                }
-            } else {
-                byte = q8_scale_byte<FX + 1>(bits);
-#pragma unroll
-                for (int i = 0; i < 4; ++i) {
-                    const q8_u32x2 o = q8_scaled8<DT, FX + 1>(raw[u][i], q8_up(byte));
-                    fx.v[2 * i] = (int)o[0];
-                    fx.v[2 * i + 1] = (int)o[1];
-                }
-            }
-#pragma unroll
-            for (int t = 0; t < NT; ++t) {
-                if constexpr (DT != KP_F32) acc[t] = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(fw[u][t].v, fx.v, acc[t], FW, FX, 0, es[u][t], 0, (int)byte);
-                else {
-                    typedef __bf16 bf8 __attribute__((ext_vector_type(8)));
-                    const float uw = q8_up((uint32_t)es[u][t]), ux = q8_up(byte);
-#pragma unroll
-                    for (int i = 0; i < 4; ++i)
-                        acc[t] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf8, q8_bf16x8<FW>(fw[u][t].v, i, uw)),
-                                                                         __builtin_bit_cast(bf8, q8_bf16x8<FX>(fx.v, i, ux)), acc[t], 0, 0, 0);
-                }
-            }
+            for (int t = 0; t < NT; ++t) acc[t] = mma16<FW, FX, DT == KP_F32>(fw[u][t], es[u][t], fx, byte, acc[t]);
         }
     }
 #pragma unroll
@@ -426,6 +440,83 @@ __global__ __launch_bounds__(512) void q8_rows_k(const RowArgs P) {
 #pragma unroll
             for (int k = 0; k < NW; ++k) v += red[k][m][c];
             el_store<DT>(P.y, (long long)(m0 + m) * P.ldy + n0 + c, v);
+        }
+    }
+}
+
+// Few columns (N <= 16 TN), many rows: bound by the bytes of x, which is read once.  A workgroup takes 64 rows, a wave 16 of them; all of W's
+// block (N x 128 bytes) goes through LDS once for the four waves, the next block's on its way in registers, x's two blocks ahead.
+// LDS rows of 128 bytes, the 16-byte piece XOR-swizzled by the row pair as in q8_mm_k.
+template <int DT, int FX, int FW, int TN>
+__global__ __launch_bounds__(256) void q8_narrow_k(const RowArgs P) {
+    constexpr int BN = 16 * TN, PIECES = BN * 8, PER = (PIECES + 255) / 256;   // 16-byte pieces of a block of W, a thread's share
+    __shared__ __attribute__((aligned(16))) uint8_t tile[2][BN * 128];
+    __shared__ uint8_t exps[2][BN];
+    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, r16 = lane & 15, quarter = lane >> 4;
+    const int m0 = blockIdx.x * 64 + wave * 16;
+    const bool mine = m0 + r16 < P.M;
+    const long long xrow = (long long)(m0 + r16) * P.ldx;
+    const int erow = tid < P.N ? tid : P.N - 1;   // (rows of W past the end repeat the last one and are not stored)
+    u32x4 wn[PER];
+    uint32_t en = 0;
+    auto fetch_w = [&](int kb) {
+#pragma unroll
+        for (int i = 0; i < PER; ++i) {
+            const int id = i * 256 + tid, row = (id >> 3) < P.N ? id >> 3 : P.N - 1;
+            if (PIECES % 256 == 0 || id < PIECES) wn[i] = *reinterpret_cast<const u32x4*>(P.w + (long long)row * P.ldw + kb * 128LL + (id & 7) * 16);
+        }
+        if (tid < BN) en = P.sw[(long long)erow * P.ldsw + kb];
+    };
+    f32x4 acc[TN];
+#pragma unroll
+    for (int t = 0; t < TN; ++t) acc[t] = f32x4{0.f, 0.f, 0.f, 0.f};
+    Raw32<DT> r0 = raw_block<DT>(P.x, xrow, 0, quarter, P.K, mine);
+    Raw32<DT> r1 = raw_block<DT>(P.x, xrow, 128, quarter, P.K, mine);
+    fetch_w(0);
+    auto step = [&](int kb, Raw32<DT>& raw) {
+        uint8_t* buf = tile[kb & 1];
+#pragma unroll
+        for (int i = 0; i < PER; ++i) {
+            const int id = i * 256 + tid, row = id >> 3;
+            if (PIECES % 256 == 0 || id < PIECES) *reinterpret_cast<u32x4_a*>(buf + row * 128 + (((id & 7) ^ ((row >> 1) & 7)) << 4)) = wn[i];
+        }
+        if (tid < BN) exps[kb & 1][tid] = (uint8_t)en;
+        if (kb + 1 < P.nb) fetch_w(kb + 1);
+        Frag8 fx;
+        const uint32_t byte = pack_rows16<DT, FX + 1>(raw, fx);
+        raw = raw_block<DT>(P.x, xrow, (kb + 2) * 128, quarter, P.K, mine);   // (past the end: zeros, nothing is read)
+        // one barrier a block: the buffer written here was read two blocks ago, before every wave's previous barrier
+        asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+        __builtin_amdgcn_s_barrier();
+        asm volatile("" ::: "memory");
+#pragma unroll
+        for (int t = 0; t < TN; ++t) {
+            Frag8 fw;
+            const int row = t * 16 + r16;
+#pragma unroll
+            for (int u = 0; u < 2; ++u) fw.h[u] = *reinterpret_cast<const u32x4_a*>(buf + row * 128 + (((u * 4 + quarter) ^ ((row >> 1) & 7)) << 4));
+            acc[t] = mma16<FW, FX, DT == KP_F32>(fw, exps[kb & 1][row], fx, byte, acc[t]);
+        }
+    };
+    for (int kb = 0; kb < P.nb; kb += 2) {
+        step(kb, r0);
+        if (kb + 1 < P.nb) step(kb + 1, r1);
+    }
+    if (!mine) return;
+#pragma unroll
+    for (int t = 0; t < TN; ++t) {   // a lane: row m = r16, columns t * 16 + quarter * 4 .. + 3
+        const int n = t * 16 + quarter * 4;
+        float v[4];
+#pragma unroll
+        for (int e = 0; e < 4; ++e) v[e] = acc[t][e] + (P.bias && n + e < P.N ? P.bias[n + e] : 0.f);
+        const long long at = (long long)(m0 + r16) * P.ldy + n;
+        if (n + 4 <= P.N) {
+            if constexpr (DT == KP_F32) *reinterpret_cast<q8_u32x4_e4*>((float*)P.y + at) = q8_u32x4{__float_as_uint(v[0]), __float_as_uint(v[1]), __float_as_uint(v[2]), __float_as_uint(v[3])};
+            else *reinterpret_cast<q8_u32x2_e2*>((uint16_t*)P.y + at) = q8_u32x2{el_pack<DT>(v[0], v[1]), el_pack<DT>(v[2], v[3])};
+        } else {
+#pragma unroll
+            for (int e = 0; e < 4; ++e)
+                if (n + e < P.N) el_store<DT>(P.y, at + e, v[e]);
         }
     }
 }
@@ -486,7 +577,29 @@ template <int FA, int FB, bool F32> int mm_launch(const MmArgs& P, const Plan& p
     return kp_check_launch("q8_matmul");
 }
 
-template <int DT, int FX> int rows_launch(const RowArgs& P, int fmtw, hipStream_t st) {
+// 1: few rows, 2: few columns, 0: neither -- pack x and take the tiles.
+//
+// Few rows against that (bf16, us): 4096 x 4096: 1 row 6.7 / 11.8, 16 rows 9.2 / 12.6, 32 rows 16.6 / 13.4; 8192 x 8192: 1 row 17.3 / 23.7,
+// 16 rows 20.9 / 24.1; 1024 x 1024, 64 rows 4.4 / 8.1; 4096 x 1000, 32 rows 6.7 / 8.8, 64 rows 12.0 / 9.1; 512 x 8192 (32 workgroups that
+// walk 64 blocks each), 4 rows 10.6 / 11.3, 16 rows 14.8 / 12.2.  So: up to 16 rows, unless few workgroups walk far; more where the walk is
+// short and two rounds of workgroups are enough.
+int linear_way(long long M, long long N, long long K) {
+    if (M <= 4) return 1;
+    if (M <= 16) return K <= 4096 || N >= 4096 ? 1 : 0;
+    if (K <= 1024 && ((N + 15) / 16) * ((M + 15) / 16) <= 512) return 1;
+    return N <= 128 ? 2 : 0;
+}
+
+template <int DT, int FX, int FW> int narrow_launch(const RowArgs& P, hipStream_t st) {
+    const unsigned grid = cdiv(P.M, 64);
+    if (P.N <= 16) q8_narrow_k<DT, FX, FW, 1><<<grid, 256, 0, st>>>(P);
+    else if (P.N <= 32) q8_narrow_k<DT, FX, FW, 2><<<grid, 256, 0, st>>>(P);
+    else if (P.N <= 64) q8_narrow_k<DT, FX, FW, 4><<<grid, 256, 0, st>>>(P);
+    else q8_narrow_k<DT, FX, FW, 8><<<grid, 256, 0, st>>>(P);
+    return kp_check_launch("q8_linear");
+}
+template <int DT, int FX> int linear_launch(const RowArgs& P, int fmtw, hipStream_t st) {
+    if (P.N <= 128 && P.M > 16 && linear_way(P.M, P.N, P.K) != 1) return fmtw == KP_E4M3 ? narrow_launch<DT, FX, 0>(P, st) : narrow_launch<DT, FX, 1>(P, st);
     const bool two = P.N >= 32 * 256;
     const dim3 grid(cdiv(P.N, two ? 32 : 16), cdiv(P.M, 16));
     if (two) {
@@ -496,7 +609,7 @@ template <int DT, int FX> int rows_launch(const RowArgs& P, int fmtw, hipStream_
         if (fmtw == KP_E4M3) q8_rows_k<DT, FX, 0, 1><<<grid, 512, 0, st>>>(P);
         else q8_rows_k<DT, FX, 1, 1><<<grid, 512, 0, st>>>(P);
     }
-    return kp_check_launch("q8_linear_rows");
+    return kp_check_launch("q8_linear");
 }
 
 }  // namespace
@@ -548,31 +661,23 @@ int kp_q8_matmul(const unsigned char* a, long long lda, const unsigned char* sa,
     return kp_check_launch("q8_matmul join");
 }
 
-// Against packing x and the tiles (bf16, us): 4096 x 4096: 1 row 6.7 / 11.8, 16 rows 9.2 / 12.6, 32 rows 16.6 / 13.4; 8192 x 8192: 1 row
-// 17.3 / 23.7, 16 rows 20.9 / 24.1; 1024 x 1024, 64 rows 4.4 / 8.1; 4096 x 1000, 32 rows 6.7 / 8.8, 64 rows 12.0 / 9.1; 512 x 8192 (32
-// workgroups that walk 64 blocks each), 4 rows 10.6 / 11.3, 16 rows 14.8 / 12.2.  So: up to 16 rows, unless few workgroups walk far; more
-// where the walk is short and two rounds of workgroups are enough.
-int kp_q8_linear_rows_suits(long long M, long long N, long long K) {
-    if (M <= 4) return 1;
-    if (M <= 16) return K <= 4096 || N >= 4096;
-    return K <= 1024 && ((N + 15) / 16) * ((M + 15) / 16) <= 512;
-}
+int kp_q8_linear_suits(long long M, long long N, long long K) { return linear_way(M, N, K) != 0; }
 
-int kp_q8_linear_rows(const void* x, long long ldx, int fmtx, const unsigned char* w, long long ldw, const unsigned char* sw, long long ldsw,
+int kp_q8_linear(const void* x, long long ldx, int fmtx, const unsigned char* w, long long ldw, const unsigned char* sw, long long ldsw,
                       int fmtw, const float* bias, void* y, long long ldy, long long M, long long N, long long K, int dtype, void* stream) {
-    KP_REQUIRE(x && w && sw && y && M > 0 && N > 0 && K > 0, "kp_q8_linear_rows: bad args (%lld x %lld x %lld)", M, N, K);
-    KP_REQUIRE((fmtx == KP_E4M3 || fmtx == KP_E5M2) && (fmtw == KP_E4M3 || fmtw == KP_E5M2), "kp_q8_linear_rows: unknown format %d / %d", fmtx, fmtw);
-    KP_REQUIRE(dtype == KP_F32 || dtype == KP_BF16 || dtype == KP_F16, "kp_q8_linear_rows: unknown dtype %d", dtype);
+    KP_REQUIRE(x && w && sw && y && M > 0 && N > 0 && K > 0, "kp_q8_linear: bad args (%lld x %lld x %lld)", M, N, K);
+    KP_REQUIRE((fmtx == KP_E4M3 || fmtx == KP_E5M2) && (fmtw == KP_E4M3 || fmtw == KP_E5M2), "kp_q8_linear: unknown format %d / %d", fmtx, fmtw);
+    KP_REQUIRE(dtype == KP_F32 || dtype == KP_BF16 || dtype == KP_F16, "kp_q8_linear: unknown dtype %d", dtype);
     const long long nb = (K + Q8_BLOCK - 1) / Q8_BLOCK;
-    KP_REQUIRE(M < (1LL << 20) && N <= 0x7fffff00LL && K < (1LL << 30), "kp_q8_linear_rows: %lld x %lld x %lld is more than one call takes", M, N, K);
-    KP_REQUIRE(ldw >= nb * Q8_BLOCK && ldw % 16 == 0 && ((size_t)w & 15) == 0 && ldsw >= nb, "kp_q8_linear_rows: the weight's rows must be padded to whole blocks and start on multiples of 16 bytes (strides %lld, %lld)", ldw, ldsw);
-    KP_REQUIRE((M == 1 || ldx >= K) && ldy >= N, "kp_q8_linear_rows: row strides %lld, %lld for %lld and %lld columns", ldx, ldy, K, N);
+    KP_REQUIRE(M < (1LL << 31) - 64 && (N <= 128 || M < (1LL << 20)) && N <= 0x7fffff00LL && K < (1LL << 30), "kp_q8_linear: %lld x %lld x %lld is more than one call takes", M, N, K);
+    KP_REQUIRE(ldw >= nb * Q8_BLOCK && ldw % 16 == 0 && ((size_t)w & 15) == 0 && ldsw >= nb, "kp_q8_linear: the weight's rows must be padded to whole blocks and start on multiples of 16 bytes (strides %lld, %lld)", ldw, ldsw);
+    KP_REQUIRE((M == 1 || ldx >= K) && ldy >= N, "kp_q8_linear: row strides %lld, %lld for %lld and %lld columns", ldx, ldy, K, N);
     RowArgs P{x, ldx, w, sw, ldw, ldsw, bias, y, ldy, (int)M, (int)N, (int)K, (int)nb};
     const hipStream_t st = (hipStream_t)stream;
     kp_count_bytes((double)N * K + (double)(M * K + M * N) * (dtype == KP_F32 ? 4 : 2));
-    if (dtype == KP_F32) return fmtx == KP_E4M3 ? rows_launch<KP_F32, 0>(P, fmtw, st) : rows_launch<KP_F32, 1>(P, fmtw, st);
-    if (dtype == KP_BF16) return fmtx == KP_E4M3 ? rows_launch<KP_BF16, 0>(P, fmtw, st) : rows_launch<KP_BF16, 1>(P, fmtw, st);
-    return fmtx == KP_E4M3 ? rows_launch<KP_F16, 0>(P, fmtw, st) : rows_launch<KP_F16, 1>(P, fmtw, st);
+    if (dtype == KP_F32) return fmtx == KP_E4M3 ? linear_launch<KP_F32, 0>(P, fmtw, st) : linear_launch<KP_F32, 1>(P, fmtw, st);
+    if (dtype == KP_BF16) return fmtx == KP_E4M3 ? linear_launch<KP_BF16, 0>(P, fmtw, st) : linear_launch<KP_BF16, 1>(P, fmtw, st);
+    return fmtx == KP_E4M3 ? linear_launch<KP_F16, 0>(P, fmtw, st) : linear_launch<KP_F16, 1>(P, fmtw, st);
 }
 
 }  // extern "C"

@@ -118,10 +118,10 @@ def checkpoint8(x: torch.Tensor, fmt: str = 'e4m3') -> Packed8:
     return Packed8(values, scales, x.shape, x.stride(), x.dtype, fmt, True)
 
 
-def _form(rows, width, like):
-    """Empty operand form on `like`'s device: values padded to whole blocks, exponent bytes to whole words."""
+def _sizes(rows, width):
+    """Row strides of an operand form: values padded to whole blocks, exponent bytes to whole words."""
     blocks = (width + BLOCK - 1) // BLOCK
-    return (like.new_empty((rows, blocks * BLOCK), dtype=torch.uint8), like.new_empty((rows, (blocks + 3) // 4 * 4), dtype=torch.uint8))
+    return blocks * BLOCK, (blocks + 3) // 4 * 4
 
 
 def pack8(x: torch.Tensor, fmt: str = 'e4m3') -> Packed8:
@@ -132,36 +132,81 @@ def pack8(x: torch.Tensor, fmt: str = 'e4m3') -> Packed8:
         raise ValueError(f'pack8: the last dimension must hold at least one element, got shape {tuple(x.shape)}')
     m, rows, ld = as_rows(x.detach())
     width = x.shape[-1]
-    values, scales = _form(rows, width, x)
+    ldv, lds = _sizes(rows, width)
+    values, scales = x.new_empty((rows, ldv), dtype=torch.uint8), x.new_empty((rows, lds), dtype=torch.uint8)
     if rows:
         with device_of(x):
-            call('kp_q8_pack', ptr(m), ld, ptr(values), values.shape[1], ptr(scales), scales.shape[1], rows, width, dcode, code, stream_ptr())
+            call('kp_q8_pack', ptr(m), ld, ptr(values), ldv, ptr(scales), lds, rows, width, dcode, code, stream_ptr())
     return Packed8(values, scales, x.shape, None, x.dtype, fmt, False)
 
 
-def _pack_both(m, rows, ld, width, dcode, code, by_rows, by_cols, sums):
-    """kp_q8_pack_both of a matrix: (row form, column form, column sums), each (None, None) / None where not asked for."""
-    if not (by_rows or by_cols or sums):
-        return (None, None), (None, None), None
-    q = _form(rows, width, m) if by_rows else (None, None)
-    qt = _form(width, rows, m) if by_cols else (None, None)
-    colsum = m.new_empty(width, dtype=torch.float32) if sums else None
-    ws = m.new_empty(_lib.lib().kp_q8_pack_both_ws_floats(rows, width), dtype=torch.float32) if sums else None
-    call('kp_q8_pack_both', ptr(m), ld, ptr(q[0]), q[0].shape[1] if by_rows else 0, ptr(q[1]), q[1].shape[1] if by_rows else 0,
-         ptr(qt[0]), qt[0].shape[1] if by_cols else 0, ptr(qt[1]), qt[1].shape[1] if by_cols else 0, ptr(ws), ptr(colsum),
-         rows, width, dcode, code, stream_ptr())
-    return q, qt, colsum
+class _Forms:
+    """Operand forms (and a workspace) of one call in ONE allocation: a linear layer's step has ten of them, and an allocation costs a
+    microsecond of host time, three in a backward.  A form is (address, stride of values, address, stride of exponents, rows, width)."""
+    __slots__ = ('bytes', 'parts', 'memory')
+
+    def __init__(self):
+        self.bytes, self.parts, self.memory = 0, [], None
+
+    def _take(self, n):
+        at = self.bytes
+        self.bytes = at + (n + 255) // 256 * 256
+        return at
+
+    def form(self, rows, width, wanted=True):
+        if not wanted:
+            return None
+        ldv, lds = _sizes(rows, width)
+        f = [self._take(rows * ldv), ldv, self._take(rows * lds), lds, rows, width]
+        self.parts.append(f)
+        return f
+
+    def floats(self, n, wanted=True):
+        if not wanted:
+            return None
+        f = [self._take(4 * n)]
+        self.parts.append(f)
+        return f
+
+    def allocate(self, like):
+        self.memory = like.new_empty(self.bytes, dtype=torch.uint8)
+        self.rebase(self.memory)
+        return self.memory
+
+    def rebase(self, memory):
+        base = memory.data_ptr()
+        for f in self.parts:
+            f[0] += base
+            if len(f) > 1:
+                f[2] += base
 
 
-def _product(a, fmta, b, fmtb, bias, shape, dtype):
-    """kp_q8_matmul of two operand forms (values, scales) into a new tensor of `shape` = [..., rows of b]."""
-    M, N, K = a[0].shape[0], b[0].shape[0], a[0].shape[1]
-    c = a[0].new_empty(shape, dtype=dtype)
-    floats = _lib.lib().kp_q8_matmul_ws_floats(M, N, K, DTYPES[dtype])
-    ws = c.new_empty(floats, dtype=torch.float32) if floats else None
-    call('kp_q8_matmul', ptr(a[0]), K, ptr(a[1]), a[1].shape[1], fmta, ptr(b[0]), K, ptr(b[1]), b[1].shape[1], fmtb, ptr(bias), ptr(c), N,
-         ptr(ws), M, N, K, DTYPES[dtype], stream_ptr())
+_NO_FORM = (None, 0, None, 0)
+
+
+def _pack_both(m, rows, ld, width, dcode, code, q, qt, ws=None, colsum=None):
+    """kp_q8_pack_both of a matrix into a row form, a column form and column sums (each may be None)."""
+    if q is None and qt is None and colsum is None:
+        return
+    v, ldv, s, lds = q[:4] if q is not None else _NO_FORM
+    vt, ldvt, st, ldst = qt[:4] if qt is not None else _NO_FORM
+    call('kp_q8_pack_both', ptr(m), ld, v, ldv, s, lds, vt, ldvt, st, ldst, ws[0] if ws is not None else None, ptr(colsum), rows, width, dcode,
+         code, stream_ptr())
+
+
+def _product(a, fmta, b, fmtb, bias, like, shape, dtype):
+    """kp_q8_matmul of two operand forms into a new tensor of `shape` = [..., rows of b] on `like`'s device."""
+    M, N, K, code = a[4], b[4], a[5], DTYPES[dtype]
+    c = like.new_empty(shape, dtype=dtype)
+    floats = _lib.lib().kp_q8_matmul_ws_floats(M, N, K, code)
+    ws = like.new_empty(floats, dtype=torch.float32) if floats else None
+    call('kp_q8_matmul', a[0], a[1], a[2], a[3], fmta, b[0], b[1], b[2], b[3], fmtb, ptr(bias), ptr(c), N, ptr(ws), M, N, K, code, stream_ptr())
     return c
+
+
+def _form_of(p: Packed8):
+    v, s = p.values, p.scales
+    return ptr(v), v.shape[1], ptr(s), s.shape[1], v.shape[0], p.shape[-1]
 
 
 def _check_bias(bias, width, device):
@@ -171,7 +216,7 @@ def _check_bias(bias, width, device):
 
 def matmul8(a: Packed8, b: Packed8, bias: torch.Tensor = None, dtype: torch.dtype = None) -> torch.Tensor:
     """a @ b.T (+ bias) of two operand forms: a [..., k], b [n, k] -> [..., n] in `dtype` (a's by default), accumulated in fp32 and rounded
-    once.  The formats may differ."""
+    once (16-bit results: with the 8-bit matrix instruction's own cut, include/kp_hip.h).  The formats may differ."""
     for name, p in (('a', a), ('b', b)):
         if not isinstance(p, Packed8) or p.flat:
             raise TypeError(f'matmul8: {name} must be a pack8 operand')
@@ -187,7 +232,7 @@ def matmul8(a: Packed8, b: Packed8, bias: torch.Tensor = None, dtype: torch.dtyp
         return torch.empty(shape, device=a.values.device, dtype=dtype)
     bias = as_vector(bias)
     with device_of(a.values):
-        return _product((a.values, a.scales), FORMATS[a.fmt], (b.values, b.scales), FORMATS[b.fmt], bias, shape, dtype)
+        return _product(_form_of(a), FORMATS[a.fmt], _form_of(b), FORMATS[b.fmt], bias, a.values, shape, dtype)
 
 
 class _Linear8(torch.autograd.Function):
@@ -207,10 +252,15 @@ class _Linear8(torch.autograd.Function):
         need_x, need_w = ctx.needs_input_grad[:2]
         with device_of(x):
             w2, _, wld = as_rows(weight)
-            qx, qxt, _ = _pack_both(m, rows, ld, K, DTYPES[x.dtype], code, True, need_w, False)
-            qw, qwt, _ = _pack_both(w2, N, wld, K, DTYPES[weight.dtype], code, True, need_x, False)
-            ctx.save_for_backward(*qxt, *qwt)
-            return _product(qx, code, qw, code, bias, shape, x.dtype)
+            now, later = _Forms(), _Forms()
+            qx, qw = now.form(rows, K), now.form(N, K)
+            qxt, qwt = later.form(K, rows, need_w), later.form(K, N, need_x)
+            now.allocate(x)
+            if need_x or need_w:
+                ctx.save_for_backward(later.allocate(x))
+            _pack_both(m, rows, ld, K, DTYPES[x.dtype], code, qx, qxt)
+            _pack_both(w2, N, wld, K, DTYPES[weight.dtype], code, qw, qwt)
+            return _product(qx, code, qw, code, bias, x, shape, x.dtype)
 
     @staticmethod
     @once_differentiable
@@ -222,12 +272,20 @@ class _Linear8(torch.autograd.Function):
             return (torch.zeros(xshape, device=dev, dtype=xdtype) if need_x else None,
                     torch.zeros(wshape, device=dev, dtype=wdtype) if need_w else None,
                     torch.zeros(N, device=dev, dtype=torch.float32) if need_b else None, None, None)
-        xv, xs, wv, ws = ctx.saved_tensors
         m, rows, ld = as_rows(dy)
+        K = wshape[1]
         with device_of(dy):
-            qd, qdt, db = _pack_both(m, rows, ld, N, DTYPES[dy.dtype], grad_code, need_x, need_w, need_b)
-            dx = _product(qd, grad_code, (wv, ws), code, None, xshape, xdtype) if need_x else None
-            dw = _product(qdt, grad_code, (xv, xs), code, None, wshape, wdtype) if need_w else None
+            later, now = _Forms(), _Forms()
+            qxt, qwt = later.form(K, rows, need_w), later.form(K, N, need_x)
+            if need_x or need_w:
+                later.rebase(ctx.saved_tensors[0])
+            qd, qdt = now.form(rows, N, need_x), now.form(N, rows, need_w)
+            ws = now.floats(_lib.lib().kp_q8_pack_both_ws_floats(rows, N), need_b)
+            now.allocate(dy)
+            db = dy.new_empty(N, dtype=torch.float32) if need_b else None
+            _pack_both(m, rows, ld, N, DTYPES[dy.dtype], grad_code, qd, qdt, ws, db)
+            dx = _product(qd, grad_code, qwt, code, None, dy, xshape, xdtype) if need_x else None
+            dw = _product(qdt, grad_code, qxt, code, None, dy, wshape, wdtype) if need_w else None
         return dx, dw, db, None, None
 
 
@@ -266,13 +324,14 @@ def linear8(x: torch.Tensor, weight, bias: torch.Tensor = None, fmt: str = 'e4m3
         return torch.empty(shape, device=x.device, dtype=x.dtype)
     K = x.shape[-1]
     with device_of(x):
-        if _lib.lib().kp_q8_linear_rows_suits(rows, N, K):
+        if _lib.lib().kp_q8_linear_suits(rows, N, K):
             y = x.new_empty(shape)
             v, s = weight.values, weight.scales
-            call('kp_q8_linear_rows', ptr(m), ld, code, ptr(v), v.shape[1], ptr(s), s.shape[1], FORMATS[weight.fmt], ptr(bias), ptr(y), N,
+            call('kp_q8_linear', ptr(m), ld, code, ptr(v), v.shape[1], ptr(s), s.shape[1], FORMATS[weight.fmt], ptr(bias), ptr(y), N,
                  rows, N, K, DTYPES[x.dtype], stream_ptr())
             return y
-        form = _form(rows, K, x)
-        call('kp_q8_pack', ptr(m), ld, ptr(form[0]), form[0].shape[1], ptr(form[1]), form[1].shape[1], rows, K, DTYPES[x.dtype], code,
-             stream_ptr())
-        return _product(form, code, (weight.values, weight.scales), FORMATS[weight.fmt], bias, shape, x.dtype)
+        forms = _Forms()
+        q = forms.form(rows, K)
+        forms.allocate(x)
+        call('kp_q8_pack', ptr(m), ld, q[0], q[1], q[2], q[3], rows, K, DTYPES[x.dtype], code, stream_ptr())
+        return _product(q, code, _form_of(weight), FORMATS[weight.fmt], bias, x, shape, x.dtype)

@@ -144,6 +144,27 @@ def test_linear8_serving(M, N, K, dtype):
         close(lowp.linear8(x, packed, bias, fmt=fmt), want, bound, dtype)
 
 
+@pytest.mark.parametrize('dtype', ['fp32', 'bf16', 'fp16'])
+@pytest.mark.parametrize('M,N,K', [(17, 1, 2100), (64, 16, 128), (65, 17, 1300), (300, 33, 4100), (129, 64, 2000), (1000, 65, 520), (2500, 100, 129), (5000, 128, 512)])
+def test_linear8_few_columns(M, N, K, dtype):
+    """The kernel that reads x once (N <= 128), also where the rule would take another, with rows at odd addresses."""
+    from keypoints_amd import _lib, lowp
+    from keypoints_amd.lowp import DTYPES, FORMATS
+    from keypoints_amd._lib import call, ptr
+    from keypoints_amd.runtime import stream_ptr
+    wide = data(M, K + 3, dtype=dtype, seed=3, spread=0.5)
+    x, w, bias = wide[:, 1:1 + K], data(N, K, dtype='fp32', seed=4, spread=0.5) / K ** 0.5, torch.randn(N).cuda()
+    for fmt, wfmt in (('e4m3', 'e4m3'), ('e5m2', 'e4m3'), ('e4m3', 'e5m2')):
+        packed = lowp.pack8(w, wfmt)
+        want, bound = product(quantise(x, fmt)[0], quantise(w, wfmt)[0], dtype, bias)
+        close(lowp.linear8(x, packed, bias, fmt=fmt), want, bound, dtype)
+        y = torch.full((M, N + 2), -7.0, device='cuda', dtype=TYPES[dtype])   # rows further apart than they are long
+        call('kp_q8_linear', ptr(wide) + wide.element_size(), K + 3, FORMATS[fmt], ptr(packed.values), packed.values.shape[1], ptr(packed.scales),
+             packed.scales.shape[1], FORMATS[wfmt], ptr(bias), ptr(y), N + 2, M, N, K, DTYPES[x.dtype], stream_ptr())
+        close(y[:, :N].contiguous(), want, bound, dtype)
+        assert bool((y[:, N:] == -7.0).all())
+
+
 @pytest.mark.parametrize('dtype,wtype', [('fp32', 'fp32'), ('bf16', 'fp32'), ('fp16', 'fp32'), ('bf16', 'bf16')])
 @pytest.mark.parametrize('M,N,K', [(1, 1, 1), (1, 33, 130), (5, 128, 64), (129, 40, 257), (300, 520, 200), (1000, 70, 130)])
 def test_linear8_training(M, N, K, dtype, wtype):

@@ -101,10 +101,10 @@ def test_c_entries_refuse_bad_arguments():
     bad('kp_q8_matmul', *v)                                                                               # rows not on 16 bytes
     assert L.kp_q8_matmul_ws_floats(64, 64, 1 << 16, 1) > 0
     bad('kp_q8_matmul', *mm(M=64, N=64, K=1 << 16, lda=1 << 16, ldb=1 << 16, sa=512, sb=512, ldc=64))     # a workspace is needed
-    bad('kp_q8_linear_rows', p, 8, 1, p, 128, p, 1, 0, None, p, 8, 2, 8, 8, 1, None)
-    bad('kp_q8_linear_rows', p, 4, 1, p, 128, p, 1, 1, None, p, 8, 2, 8, 8, 1, None)
-    bad('kp_q8_linear_rows', p, 8, 1, p, 120, p, 1, 1, None, p, 8, 2, 8, 8, 1, None)
-    bad('kp_q8_linear_rows', p, 8, 1, p, 128, p, 1, 1, None, p, 8, 1 << 20, 8, 8, 1, None)
+    bad('kp_q8_linear', p, 8, 1, p, 128, p, 1, 0, None, p, 8, 2, 8, 8, 1, None)
+    bad('kp_q8_linear', p, 4, 1, p, 128, p, 1, 1, None, p, 8, 2, 8, 8, 1, None)
+    bad('kp_q8_linear', p, 8, 1, p, 120, p, 1, 1, None, p, 8, 2, 8, 8, 1, None)
+    bad('kp_q8_linear', p, 8, 1, p, 128, p, 1, 1, None, p, 200, 1 << 20, 200, 8, 1, None)
     bad('kp_layer_norm_fwd', p, 8, None, None, -1.0, p, 8, None, None, None, None, 0, 2, 8, 1, None)      # negative eps
     bad('kp_layer_norm_fwd', p, 8, None, None, 1e-5, p, 8, p, None, None, None, 0, 2, 8, 1, None)         # mean without rstd
     bad('kp_layer_norm_fwd', p, 8, None, None, 1e-5, p, 8, None, None, p, None, 1, 2, 8, 1, None)
