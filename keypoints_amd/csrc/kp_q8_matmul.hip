@@ -583,11 +583,13 @@ template <int FA, int FB, bool F32> int mm_launch(const MmArgs& P, const Plan& p
 // 16 rows 20.9 / 24.1; 1024 x 1024, 64 rows 4.4 / 8.1; 4096 x 1000, 32 rows 6.7 / 8.8, 64 rows 12.0 / 9.1; 512 x 8192 (32 workgroups that
 // walk 64 blocks each), 4 rows 10.6 / 11.3, 16 rows 14.8 / 12.2.  So: up to 16 rows, unless few workgroups walk far; more where the walk is
 // short and two rounds of workgroups are enough.
+// Few columns (128, bf16): a block takes a workgroup a microsecond, so it wants many rows or few blocks: K = 512: 32768 rows 12.3 / 19.2, 8192
+// rows 8.5 / 9.2, 2048 rows 7.7 / 6.9; K = 4096: 32768 rows 59.5 / 122, 8192 rows 37.9 / 35.2; K = 64: 2048 rows 4.8 / 5.5.
 int linear_way(long long M, long long N, long long K) {
     if (M <= 4) return 1;
     if (M <= 16) return K <= 4096 || N >= 4096 ? 1 : 0;
     if (K <= 1024 && ((N + 15) / 16) * ((M + 15) / 16) <= 512) return 1;
-    return N <= 128 ? 2 : 0;
+    return N <= 128 && (M >= 16384 || (M >= 6144 && K <= 2048) || K <= 256) ? 2 : 0;
 }
 
 template <int DT, int FX, int FW> int narrow_launch(const RowArgs& P, hipStream_t st) {
@@ -599,7 +601,7 @@ template <int DT, int FX, int FW> int narrow_launch(const RowArgs& P, hipStream_
     return kp_check_launch("q8_linear");
 }
 template <int DT, int FX> int linear_launch(const RowArgs& P, int fmtw, hipStream_t st) {
-    if (P.N <= 128 && P.M > 16 && linear_way(P.M, P.N, P.K) != 1) return fmtw == KP_E4M3 ? narrow_launch<DT, FX, 0>(P, st) : narrow_launch<DT, FX, 1>(P, st);
+    if (P.N <= 128 && linear_way(P.M, P.N, P.K) != 1) return fmtw == KP_E4M3 ? narrow_launch<DT, FX, 0>(P, st) : narrow_launch<DT, FX, 1>(P, st);
     const bool two = P.N >= 32 * 256;
     const dim3 grid(cdiv(P.N, two ? 32 : 16), cdiv(P.M, 16));
     if (two) {
