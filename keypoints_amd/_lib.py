@@ -137,7 +137,7 @@ def lib():
 
 def call(name: str, *args):
     """Invoke a kp_* entry point; non-zero return -> KpError with the library's message."""
-    rc = getattr(lib(), name)(*args)
+    rc = getattr(_lib or lib(), name)(*args)
     if rc != 0:
         e = KpError(f'{name} failed ({rc}): {lib().kp_last_error().decode()}')
         e.rc = rc

@@ -44,9 +44,10 @@ def as_rows(x: torch.Tensor):
     """x [..., width] as (tensor, rows, row stride): x itself where its rows lie one stride apart (a column slice of a matrix does), else a
     contiguous copy."""
     width = x.shape[-1]
-    if x.dim() == 2 and (width <= 1 or x.stride(1) == 1) and x.stride(0) >= width:
-        return x, x.shape[0], x.stride(0)
-    x = x.contiguous()
+    if not x.is_contiguous():
+        if x.dim() == 2 and (width <= 1 or x.stride(1) == 1) and x.stride(0) >= width:
+            return x, x.shape[0], x.stride(0)
+        x = x.contiguous()
     return x, x.numel() // width, width
 
 

@@ -19,7 +19,7 @@ def _forward(x, weight, bias, eps, stats, fmt):
     """-> y, x as rows, its row stride, [means | deviations' reciprocals], 8-bit copy, its exponents (each None where not asked for)."""
     m, rows, ld = as_rows(x)
     C = x.shape[-1]
-    y = x.new_empty(x.shape)
+    y = torch.empty_like(m) if m is x and ld == C else x.new_empty(x.shape)
     st = q = s = None
     if stats:
         st = x.new_empty((2, rows), dtype=torch.float32)
@@ -69,19 +69,35 @@ def layer_norm(x: torch.Tensor, weight: torch.Tensor = None, bias: torch.Tensor 
     vectors of x.shape[-1] floats or None.  keep: None -- the backward reads x itself -- or the 8-bit format ('e4m3', 'e5m2'; keypoints_amd.lowp)
     in which a copy of x waits for it: half the memory of a 16-bit x, and the gradients of x and weight are those at the copy's values
     (each off from x by at most 2^-4 / 2^-3 of itself)."""
+    eps = float(eps)
+    C = x.shape[-1] if x.dim() else 0
+    if not (x.is_cuda and C > 0 and x.dtype in DTYPES and 0.0 <= eps < _INF and (keep is None or keep in FORMATS)
+            and _plain_vector(weight, C, x) and _plain_vector(bias, C, x)):
+        weight, bias = _checked(x, weight, bias, eps, keep, C)
+    if torch.is_grad_enabled() and (x.requires_grad or (weight is not None and weight.requires_grad) or (bias is not None and bias.requires_grad)):
+        return _LayerNorm.apply(x, weight, bias, eps, keep)
+    return _forward(x, weight, bias, eps, False, None)[0]
+
+
+_INF = float('inf')
+
+
+def _plain_vector(t, C, x):
+    """None, or a vector as the kernels read it, where x is."""
+    return t is None or (t.dtype is torch.float32 and t.dim() == 1 and t.numel() == C and t.is_cuda and t.is_contiguous() and t.device == x.device)
+
+
+def _checked(x, weight, bias, eps, keep, C):
+    """weight and bias as the kernels read them, or the refusal that says what is wrong (off the path of calls that need neither)."""
     require_device(x, weight, bias)
     dtype_code(x.dtype)
     if keep is not None:
         format_code(keep)
-    if x.dim() < 1 or x.shape[-1] < 1:
+    if C < 1:
         raise ValueError(f'layer_norm: the last dimension must hold at least one element, got shape {tuple(x.shape)}')
-    eps = float(eps)
-    if not 0.0 <= eps < float('inf'):
+    if not 0.0 <= eps < _INF:
         raise ValueError(f'layer_norm: eps must be a number that is not negative, got {eps}')
     for name, t in (('weight', weight), ('bias', bias)):
         if t is not None and (t.shape != x.shape[-1:] or t.dtype not in DTYPES or t.device != x.device):
-            raise ValueError(f'layer_norm: {name} must be a vector of {x.shape[-1]} floats on {x.device}, got {tuple(t.shape)} {t.dtype} on {t.device}')
-    weight, bias = as_vector(weight), as_vector(bias)
-    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (x, weight, bias)):
-        return _LayerNorm.apply(x, weight, bias, eps, keep)
-    return _forward(x, weight, bias, eps, False, None)[0]
+            raise ValueError(f'layer_norm: {name} must be a vector of {C} floats on {x.device}, got {tuple(t.shape)} {t.dtype} on {t.device}')
+    return as_vector(weight), as_vector(bias)
