@@ -80,6 +80,7 @@ class Packed8:
         dtype = self.dtype if dtype is None else dtype
         code = dtype_code(dtype)
         v, s = self.values, self.scales
+        require_device(v, s)
         if self.flat:
             y = torch.empty_strided(self.shape, self.stride, dtype=dtype, device=v.device)
             rows, width, ldq, lds = 1, y.numel(), v.numel(), s.numel()
@@ -170,16 +171,16 @@ class _Forms:
         return f
 
     def allocate(self, like):
-        self.memory = like.new_empty(self.bytes, dtype=torch.uint8)
-        self.rebase(self.memory)
-        return self.memory
+        return self.rebase(like.new_empty(self.bytes, dtype=torch.uint8))
 
     def rebase(self, memory):
+        self.memory = memory   # (held here: what a saved-tensor hook gives back has no other owner)
         base = memory.data_ptr()
         for f in self.parts:
             f[0] += base
             if len(f) > 1:
                 f[2] += base
+        return memory
 
 
 _NO_FORM = (None, 0, None, 0)
@@ -228,6 +229,9 @@ def matmul8(a: Packed8, b: Packed8, bias: torch.Tensor = None, dtype: torch.dtyp
     dtype = a.dtype if dtype is None else dtype
     dtype_code(dtype)
     _check_bias(bias, b.shape[0], a.values.device)
+    if torch.is_grad_enabled() and bias is not None and bias.requires_grad:
+        raise RuntimeError('matmul8: packed operands carry no gradient, and none would reach the bias; run under torch.no_grad()')
+    require_device(a.values, a.scales, b.values, b.scales)
     shape = (*a.shape[:-1], b.shape[0])
     if a.values.shape[0] == 0 or b.shape[0] == 0:
         return torch.empty(shape, device=a.values.device, dtype=dtype)

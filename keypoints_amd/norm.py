@@ -38,17 +38,18 @@ class _LayerNorm(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, weight, bias, eps, keep):
         y, m, ld, st, q, s = _forward(x, weight, bias, eps, True, keep)
-        ctx.args = (keep, ld)
+        ctx.keep = keep
         ctx.save_for_backward(weight, st, q if keep else m, s)
         return y
 
     @staticmethod
     @once_differentiable
     def backward(ctx, dy):
-        keep, ldx = ctx.args
+        keep = ctx.keep
         weight, st, kept, s = ctx.saved_tensors
         need_x, need_w, need_b = ctx.needs_input_grad[:3]
         g, rows, ldg = as_rows(dy)
+        kept, _, ldx = as_rows(kept)   # (a saved-tensor hook may give x back with other strides)
         C = dy.shape[-1]
         make = st.new_empty if rows else st.new_zeros   # (no rows: nothing is launched)
         dx = dy.new_empty(dy.shape) if need_x else None
@@ -58,7 +59,7 @@ class _LayerNorm(torch.autograd.Function):
             ws = st.new_empty(_lib.lib().kp_layer_norm_bwd_ws_floats(rows, C)) if need_w or need_b else None
             at = ptr(st)
             with device_of(dy):
-                call('kp_layer_norm_bwd', ptr(g), ldg, None if keep else ptr(kept), C if keep else ldx, ptr(kept) if keep else None, ptr(s),
+                call('kp_layer_norm_bwd', ptr(g), ldg, None if keep else ptr(kept), ldx, ptr(kept) if keep else None, ptr(s),
                      FORMATS[keep] if keep else 0, ptr(weight), at, at + 4 * rows, ptr(dx), C, ptr(ws), ptr(dw), ptr(db), rows, C,
                      DTYPES[dy.dtype], stream_ptr())
         return dx, dw, db, None, None
@@ -67,8 +68,8 @@ class _LayerNorm(torch.autograd.Function):
 def layer_norm(x: torch.Tensor, weight: torch.Tensor = None, bias: torch.Tensor = None, eps: float = 1e-5, keep: str = None) -> torch.Tensor:
     """(x - mean) / sqrt(variance + eps) * weight + bias over the last dimension, in x's type; statistics in fp32.  weight and bias are
     vectors of x.shape[-1] floats or None.  keep: None -- the backward reads x itself -- or the 8-bit format ('e4m3', 'e5m2'; keypoints_amd.lowp)
-    in which a copy of x waits for it: half the memory of a 16-bit x, and the gradients of x and weight are those at the copy's values
-    (each off from x by at most 2^-4 / 2^-3 of itself)."""
+    in which a copy of x waits for it: half the memory of a 16-bit x, and the gradients of x and weight are taken with
+    the copy's values (each off from x by at most 2^-4 / 2^-3 of itself) and x's own statistics."""
     eps = float(eps)
     C = x.shape[-1] if x.dim() else 0
     if not (x.is_cuda and C > 0 and x.dtype in DTYPES and 0.0 <= eps < _INF and (keep is None or keep in FORMATS)

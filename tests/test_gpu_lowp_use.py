@@ -284,3 +284,22 @@ def test_products_past_two_to_the_thirty_one():
     for r, c in ((slice(0, 70), slice(0, 70)), (slice(-70, None), slice(-70, None)), (slice(-70, None), slice(0, 70)), (slice(20000, 20070), slice(30000, 30070))):
         part = lowp.matmul8(lowp.pack8(a[r]), lowp.pack8(b[c]))
         assert torch.allclose(y[r, c].float(), part.float(), rtol=2.0 ** -7, atol=1e-2)   # (another tile: one rounding apart)
+
+
+@pytest.mark.parametrize('keep', [None, 'e4m3'])
+def test_saved_tensors_that_come_back_with_other_strides(keep):
+    """Saved-tensor hooks (offloading to the host, say) give a strided x back dense."""
+    from keypoints_amd import lowp, norm
+    wide = rnd(37, 400, seed=1)
+    w, weight, dy = rnd(100, seed=2, dtype=torch.float32), rnd(100, 100, seed=3, dtype=torch.float32), rnd(37, 100, seed=4)
+
+    def step():
+        leaves = [wide.clone().requires_grad_(), w.clone().requires_grad_(), weight.clone().requires_grad_()]
+        y = lowp.linear8(norm.layer_norm(leaves[0][:, 200:300], leaves[1], keep=keep), leaves[2])
+        return leaves, y
+
+    leaves, y = step()
+    want = torch.autograd.grad(y, leaves, dy)
+    with torch.autograd.graph.saved_tensors_hooks(lambda t: t.cpu().contiguous(), lambda t: t.cuda()):
+        leaves, y = step()
+    assert all(torch.equal(a, b) for a, b in zip(torch.autograd.grad(y, leaves, dy), want))

@@ -125,3 +125,19 @@ def test_products_plan_covers_every_block():
             n = ws(M, N, K, dtype)
             assert n == 0 or (n % (M * N) == 0 and 2 <= n // (M * N) <= 32)
     assert ws(8192, 8192, 8192, 1) == 0 and ws(0, 4, 4, 1) == 0 and ws(4, 4, 1 << 40, 1) == 0
+
+
+def test_packed_tensors_off_the_device():
+    """A Packed8 that was brought to the CPU (a loaded file) is refused, not launched on."""
+    a, b = packed((4, 200)), packed((6, 200))
+    refuses(RuntimeError, 'HIP device', lowp.matmul8, a, b)
+    refuses(RuntimeError, 'HIP device', a.unpack)
+    refuses(RuntimeError, 'HIP device', packed((1,), flat=True).unpack)
+
+
+def test_matmul8_refuses_a_bias_that_wants_a_gradient():
+    a, b = packed((4, 200)), packed((6, 200))
+    bias = torch.zeros(6, requires_grad=True)
+    refuses(RuntimeError, 'carry no gradient', lowp.matmul8, a, b, bias)
+    with torch.no_grad():
+        refuses(RuntimeError, 'HIP device', lowp.matmul8, a, b, bias)
