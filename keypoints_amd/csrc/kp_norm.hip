@@ -8,7 +8,10 @@
 //             meets, so dw += dy xh and db += dy stay in its registers; one partial row a workgroup, joined by a second launch in a fixed
 //             order (fp64), so equal calls give equal bits
 //
-// Both are bound by memory.  A row is spread over G lanes, 8 consecutive elements (16 bytes of a 16-bit type) each, NJ times: the smallest
+// Both are bound by memory.  Measured (a large copy reaches 5.2 TB/s here): 2097152 rows of 64 in bf16: forward 100 us = 5.4 TB/s,
+// backward 169 us = 4.8 TB/s (it reads two streams and writes a third; join 5 us); 8192 rows of 4096 in fp16 with an 8-bit copy: forward
+// 41 us = 4.1 TB/s, backward 42 us = 4.0 TB/s, join 4 us; 4099 x 1001 in fp32: 9 and 19 us (much of it in the last cache), join 5 us.
+// A row is spread over G lanes, 8 consecutive elements (16 bytes of a 16-bit type) each, NJ times: the smallest
 // power of two that holds it up to a wave (rows of 64 elements: eight rows a wave; a wave takes up to 1024), then 4, 8 or 16 waves with
 // sums through LDS, and beyond 16384 elements a workgroup that walks the row and reads it again.
 #include "kp_q8_dev.h"
@@ -58,8 +61,8 @@ struct LnBwd {
 
 // A row's lanes: sub = thread % G, chunk j of 8 columns at (j * G + sub) * 8.  The next row's loads are in flight during this row's sums
 // (not in the backward of the widest rows, two chunks a lane in workgroups of 1024: the 128 registers a lane has there go to the sums).
-// A workgroup has 256 threads; past a wave, G in the forward and 1024 in the backward, so that the four rows of 256 lanes that are taken at once share one partial row of the
-// weight's gradient.
+// A workgroup has 256 threads; past a wave, G in the forward and 1024 in the backward, so that the four rows of 256 lanes that are taken at
+// once share one partial row of the weight's gradient.
 template <int G> constexpr int ln_tpb = G > 64 ? 1024 : 256;
 template <int G> constexpr int ln_fwd_tpb = G > 64 ? G : 256;
 

@@ -198,8 +198,9 @@ template <int G, bool PAIRS> __device__ __forceinline__ uint32_t q8_group_max(ui
 }
 
 // ---- a block from its elements as loaded.  The largest magnitude is taken over the type's own bits as integers (two at a time in 16 bits)
-// and the elements are converted by the scaling conversions of gfx950, 2 operations an element in all instead of 7.  Blocks that hold an infinity or a not-a-number, or whose
-// scale is the smallest one, take the plain sequence: the maximum over finite elements, a multiplication and a conversion.
+// and the elements are converted by the scaling conversions of gfx950, 2 operations an element in all instead of 7.  Blocks that hold an
+// infinity or a not-a-number, or whose scale is the smallest one, take the plain sequence: the maximum over finite elements, a
+// multiplication and a conversion.
 template <int DT> __device__ __forceinline__ uint32_t q8_raw_mag(uint32_t w) { return w & (DT == KP_F32 ? 0x7fffffffu : 0x7fff7fffu); }
 template <int DT> __device__ __forceinline__ uint32_t q8_raw_max(uint32_t a, uint32_t b) { return DT == KP_F32 ? q8_umax(a, b) : q8_umax16(a, b); }
 template <int DT> __device__ __forceinline__ uint32_t q8_raw_peak(const El8<DT>& r) {

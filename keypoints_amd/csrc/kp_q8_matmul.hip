@@ -10,6 +10,10 @@
 //                    converted on the way from LDS (exponent and all) and multiplied by the bfloat16 instruction, whose sums are fp32
 //                    sums (measured 6e-9 .. 4e-7 of the norm), at half its partner's rate.  Weight gradients go this way.
 //
+// Measured (bf16 / fp32 results; the library's 8-bit product reaches 2.75 PFLOP/s on the first): 8192^3 490 us = 2.25 PFLOP/s / 815 us =
+// 1.35, 4096^3 68 / 125 us = 2.0 / 1.1, 16384 x 2048 x 4096 119 / 204 us = 2.3 / 1.35.  The largest are bound by the power cap: at 8192^3 the clock falls
+// to 1.6 GHz with the matrix cores 62 % busy, at 4096^3 it stays at 2.2 GHz with 43 %.
+//
 // Any order of the elements inside a block serves, as long as A and B agree: the fragments are read as the swizzle likes them.
 #include <math.h>
 #include "kp_mfma_util.h"
@@ -445,7 +449,8 @@ __global__ __launch_bounds__(512) void q8_rows_k(const RowArgs P) {
 }
 
 // Few columns (N <= 16 TN), many rows: bound by the bytes of x, which is read once.  A workgroup takes 64 rows, a wave 16 of them; all of W's
-// block (N x 128 bytes) goes through LDS once for the four waves, the next block's on its way in registers, x's two blocks ahead.
+// block (N x 128 bytes) goes through LDS once for the four waves; W's and x's next two blocks are on their way in registers (W's one
+// ahead: 8192 x 4096 -> 128 in fp32 95.9 us instead of 58.7, in bf16 37.1 instead of 35.2).
 // LDS rows of 128 bytes, the 16-byte piece XOR-swizzled by the row pair as in q8_mm_k.
 template <int DT, int FX, int FW, int TN>
 __global__ __launch_bounds__(256) void q8_narrow_k(const RowArgs P) {
@@ -457,34 +462,35 @@ __global__ __launch_bounds__(256) void q8_narrow_k(const RowArgs P) {
     const bool mine = m0 + r16 < P.M;
     const long long xrow = (long long)(m0 + r16) * P.ldx;
     const int erow = tid < P.N ? tid : P.N - 1;   // (rows of W past the end repeat the last one and are not stored)
-    u32x4 wn[PER];
-    uint32_t en = 0;
-    auto fetch_w = [&](int kb) {
+    struct Rest { u32x4 w[PER]; uint32_t e; Raw32<DT> x; };   // a thread's part of a block
+    auto fetch_w = [&](Rest& r, int kb) {
 #pragma unroll
         for (int i = 0; i < PER; ++i) {
             const int id = i * 256 + tid, row = (id >> 3) < P.N ? id >> 3 : P.N - 1;
-            if (PIECES % 256 == 0 || id < PIECES) wn[i] = *reinterpret_cast<const u32x4*>(P.w + (long long)row * P.ldw + kb * 128LL + (id & 7) * 16);
+            if (PIECES % 256 == 0 || id < PIECES) r.w[i] = *reinterpret_cast<const u32x4*>(P.w + (long long)row * P.ldw + kb * 128LL + (id & 7) * 16);
         }
-        if (tid < BN) en = P.sw[(long long)erow * P.ldsw + kb];
+        if (tid < BN) r.e = P.sw[(long long)erow * P.ldsw + kb];
     };
     f32x4 acc[TN];
 #pragma unroll
     for (int t = 0; t < TN; ++t) acc[t] = f32x4{0.f, 0.f, 0.f, 0.f};
-    Raw32<DT> r0 = raw_block<DT>(P.x, xrow, 0, quarter, P.K, mine);
-    Raw32<DT> r1 = raw_block<DT>(P.x, xrow, 128, quarter, P.K, mine);
-    fetch_w(0);
-    auto step = [&](int kb, Raw32<DT>& raw) {
+    Rest r0, r1;
+    fetch_w(r0, 0);
+    r0.x = raw_block<DT>(P.x, xrow, 0, quarter, P.K, mine);
+    if (P.nb > 1) fetch_w(r1, 1);
+    r1.x = raw_block<DT>(P.x, xrow, 128, quarter, P.K, mine);   // (past the end: zeros, nothing is read)
+    auto step = [&](int kb, Rest& r) {
         uint8_t* buf = tile[kb & 1];
 #pragma unroll
         for (int i = 0; i < PER; ++i) {
             const int id = i * 256 + tid, row = id >> 3;
-            if (PIECES % 256 == 0 || id < PIECES) *reinterpret_cast<u32x4_a*>(buf + row * 128 + (((id & 7) ^ ((row >> 1) & 7)) << 4)) = wn[i];
+            if (PIECES % 256 == 0 || id < PIECES) *reinterpret_cast<u32x4_a*>(buf + row * 128 + (((id & 7) ^ ((row >> 1) & 7)) << 4)) = r.w[i];
         }
-        if (tid < BN) exps[kb & 1][tid] = (uint8_t)en;
-        if (kb + 1 < P.nb) fetch_w(kb + 1);
+        if (tid < BN) exps[kb & 1][tid] = (uint8_t)r.e;
+        if (kb + 2 < P.nb) fetch_w(r, kb + 2);
         Frag8 fx;
-        const uint32_t byte = pack_rows16<DT, FX + 1>(raw, fx);
-        raw = raw_block<DT>(P.x, xrow, (kb + 2) * 128, quarter, P.K, mine);   // (past the end: zeros, nothing is read)
+        const uint32_t byte = pack_rows16<DT, FX + 1>(r.x, fx);
+        r.x = raw_block<DT>(P.x, xrow, (kb + 2) * 128, quarter, P.K, mine);
         // one barrier a block: the buffer written here was read two blocks ago, before every wave's previous barrier
         asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
         __builtin_amdgcn_s_barrier();
@@ -635,7 +641,7 @@ int kp_q8_matmul(const unsigned char* a, long long lda, const unsigned char* sa,
     KP_REQUIRE((fmta == KP_E4M3 || fmta == KP_E5M2) && (fmtb == KP_E4M3 || fmtb == KP_E5M2), "kp_q8_matmul: unknown format %d / %d", fmta, fmtb);
     KP_REQUIRE(dtype == KP_F32 || dtype == KP_BF16 || dtype == KP_F16, "kp_q8_matmul: unknown dtype %d", dtype);
     const long long nb = (K + Q8_BLOCK - 1) / Q8_BLOCK, words = (nb + 3) / 4 * 4;
-    KP_REQUIRE(mm_sizes_ok(M, N, K) && lda < (1LL << 23) && ldb < (1LL << 23),
+    KP_REQUIRE(mm_sizes_ok(M, N, K) && lda < (1LL << 23) && ldb < (1LL << 23) && ldsa < (1LL << 23) && ldsb < (1LL << 23),
                "kp_q8_matmul: %lld x %lld x %lld is more than one call takes (2^23 along the product, 2^31 and 2^29 rows)", M, N, K);
     KP_REQUIRE(lda >= nb * Q8_BLOCK && ldb >= nb * Q8_BLOCK && lda % 16 == 0 && ldb % 16 == 0 && ((size_t)a & 15) == 0 && ((size_t)b & 15) == 0,
                "kp_q8_matmul: operand rows must be padded to whole blocks and start on multiples of 16 bytes (strides %lld, %lld)", lda, ldb);
@@ -666,12 +672,12 @@ int kp_q8_matmul(const unsigned char* a, long long lda, const unsigned char* sa,
 int kp_q8_linear_suits(long long M, long long N, long long K) { return linear_way(M, N, K) != 0; }
 
 int kp_q8_linear(const void* x, long long ldx, int fmtx, const unsigned char* w, long long ldw, const unsigned char* sw, long long ldsw,
-                      int fmtw, const float* bias, void* y, long long ldy, long long M, long long N, long long K, int dtype, void* stream) {
+                 int fmtw, const float* bias, void* y, long long ldy, long long M, long long N, long long K, int dtype, void* stream) {
     KP_REQUIRE(x && w && sw && y && M > 0 && N > 0 && K > 0, "kp_q8_linear: bad args (%lld x %lld x %lld)", M, N, K);
     KP_REQUIRE((fmtx == KP_E4M3 || fmtx == KP_E5M2) && (fmtw == KP_E4M3 || fmtw == KP_E5M2), "kp_q8_linear: unknown format %d / %d", fmtx, fmtw);
     KP_REQUIRE(dtype == KP_F32 || dtype == KP_BF16 || dtype == KP_F16, "kp_q8_linear: unknown dtype %d", dtype);
     const long long nb = (K + Q8_BLOCK - 1) / Q8_BLOCK;
-    KP_REQUIRE(M < (1LL << 31) - 64 && (N <= 128 || M < (1LL << 20)) && N <= 0x7fffff00LL && K < (1LL << 30), "kp_q8_linear: %lld x %lld x %lld is more than one call takes", M, N, K);
+    KP_REQUIRE(M < (1LL << 31) - 64 && (N <= 128 || M <= 65535LL * 16) && N <= 0x7fffff00LL && K < (1LL << 30), "kp_q8_linear: %lld x %lld x %lld is more than one call takes", M, N, K);
     KP_REQUIRE(ldw >= nb * Q8_BLOCK && ldw % 16 == 0 && ((size_t)w & 15) == 0 && ldsw >= nb, "kp_q8_linear: the weight's rows must be padded to whole blocks and start on multiples of 16 bytes (strides %lld, %lld)", ldw, ldsw);
     KP_REQUIRE((M == 1 || ldx >= K) && ldy >= N, "kp_q8_linear: row strides %lld, %lld for %lld and %lld columns", ldx, ldy, K, N);
     RowArgs P{x, ldx, w, sw, ldw, ldsw, bias, y, ldy, (int)M, (int)N, (int)K, (int)nb};
