@@ -577,7 +577,7 @@ long long kp_q8_matmul_ws_floats(long long M, long long N, long long K, int dtyp
 int kp_q8_linear(const void* x, long long ldx, int fmtx, const unsigned char* w, long long ldw, const unsigned char* sw, long long ldsw,
                  int fmtw, const float* bias, void* y, long long ldy, long long M, long long N, long long K, int dtype, void* stream);
 /* 1 where that is the faster way (kp_q8_linear takes up to 16 * 65535 rows, and about 2^31 where N <= 128) */
-int kp_q8_linear_suits(long long M, long long N, long long K);
+int kp_q8_linear_suits(long long M, long long N, long long K, int dtype);
 
 /* ---- layer norm ----------------------------------------------------------------------------------------------------------------
  * Per row of C elements: y = (x - mean) * rstd * w + b, rstd = 1 / sqrt(mean((x - mean)^2) + eps).  w, b fp32 or NULL (1, 0).  mean, rstd

@@ -203,6 +203,13 @@ template <int G, bool PAIRS> __device__ __forceinline__ uint32_t q8_group_max(ui
 // multiplication and a conversion.
 template <int DT> __device__ __forceinline__ uint32_t q8_raw_mag(uint32_t w) { return w & (DT == KP_F32 ? 0x7fffffffu : 0x7fff7fffu); }
 template <int DT> __device__ __forceinline__ uint32_t q8_raw_max(uint32_t a, uint32_t b) { return DT == KP_F32 ? q8_umax(a, b) : q8_umax16(a, b); }
+// over lanes l, l ^ 16, l ^ 32, l ^ 48 (all lanes of the wave are active): the row swaps of gfx950 instead of two ways through LDS
+template <int DT> __device__ __forceinline__ uint32_t q8_raw_max4(uint32_t m) {
+    const auto a = __builtin_amdgcn_permlane16_swap(m, m, false, false);
+    m = q8_raw_max<DT>(a[0], a[1]);
+    const auto b = __builtin_amdgcn_permlane32_swap(m, m, false, false);
+    return q8_raw_max<DT>(b[0], b[1]);
+}
 template <int DT> __device__ __forceinline__ uint32_t q8_raw_peak(const El8<DT>& r) {
     uint32_t m = q8_raw_mag<DT>(r.w[0][0]);
 #pragma unroll

@@ -332,8 +332,7 @@ template <int DT, int FMT> __device__ __forceinline__ uint32_t pack_rows16(const
     uint32_t m = 0;
 #pragma unroll
     for (int i = 0; i < 4; ++i) m = q8_raw_max<DT>(m, q8_raw_peak<DT>(raw.e[i]));
-    m = q8_raw_max<DT>(m, (uint32_t)__shfl_xor((int)m, 16, 64));   // the row's four lanes
-    m = q8_raw_max<DT>(m, (uint32_t)__shfl_xor((int)m, 32, 64));
+    m = q8_raw_max4<DT>(m);   // the row's four lanes
     if constexpr (DT != KP_F32) m = q8_umax(m & 0xffffu, m >> 16);
     const uint32_t bits = q8_raw_bits<DT>(m);
     if (__any(q8_plain<FMT>(bits))) {
@@ -344,8 +343,7 @@ template <int DT, int FMT> __device__ __forceinline__ uint32_t pack_rows16(const
             el_unpack8<DT>(raw.e[i], v[i]);
             t = q8_umax(t, q8_mag8(v[i]));
         }
-        t = q8_umax(t, (uint32_t)__shfl_xor((int)t, 16, 64));
-        t = q8_umax(t, (uint32_t)__shfl_xor((int)t, 32, 64));
+        t = q8_raw_max4<KP_F32>(t);
         const uint32_t byte = q8_scale_byte<FMT>(t);
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
@@ -449,64 +447,110 @@ __global__ __launch_bounds__(512) void q8_rows_k(const RowArgs P) {
 }
 
 // Few columns (N <= 16 TN), many rows: bound by the bytes of x, which is read once.  A workgroup takes 64 rows, a wave 16 of them; all of W's
-// block (N x 128 bytes) goes through LDS once for the four waves; W's and x's next two blocks are on their way in registers (W's one
-// ahead: 8192 x 4096 -> 128 in fp32 95.9 us instead of 58.7, in bf16 37.1 instead of 35.2).
-// LDS rows of 128 bytes, the 16-byte piece XOR-swizzled by the row pair as in q8_mm_k.
+// block (N x 128 bytes) goes through LDS once for the four waves.  One barrier a block: while a block's fragments of W come from LDS, the
+// next block of W goes there and the next 128 elements of x are packed; two more blocks of both are on their way in registers.  The loads
+// stand in no branch (rows past the end repeat the last one, for blocks past the end all lanes read one address): behind a branch that may
+// have issued none, the compiler waits for all that are on their way.  A short last block comes after the others.
+// Measured (bf16): 32768 x 512 -> 128 12.5 us = 3.4 TB/s, 32768 x 4096 -> 64 46 us = 5.9 TB/s; against loads one block ahead behind branches:
+// 8192 x 8192 -> 32 43 us instead of 72, 8192 x 4096 -> 128 28.9 instead of 37, 16384 x 2048 -> 16 12.1 instead of 18.3.
+// LDS rows of 128 bytes, the 16-byte piece XOR-swizzled by the row pair as in q8_mm_k; the exponent bytes of rows r16, 16 + r16, ... side by side.
 template <int DT, int FX, int FW, int TN>
-__global__ __launch_bounds__(256) void q8_narrow_k(const RowArgs P) {
+__global__ __launch_bounds__(256, 2) void q8_narrow_k(const RowArgs P) {
     constexpr int BN = 16 * TN, PIECES = BN * 8, PER = (PIECES + 255) / 256;   // 16-byte pieces of a block of W, a thread's share
     __shared__ __attribute__((aligned(16))) uint8_t tile[2][BN * 128];
-    __shared__ uint8_t exps[2][BN];
+    __shared__ __attribute__((aligned(16))) uint8_t exps[2][16 * 8];
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, r16 = lane & 15, quarter = lane >> 4;
     const int m0 = blockIdx.x * 64 + wave * 16;
     const bool mine = m0 + r16 < P.M;
-    const long long xrow = (long long)(m0 + r16) * P.ldx;
-    const int erow = tid < P.N ? tid : P.N - 1;   // (rows of W past the end repeat the last one and are not stored)
-    struct Rest { u32x4 w[PER]; uint32_t e; Raw32<DT> x; };   // a thread's part of a block
-    auto fetch_w = [&](Rest& r, int kb) {
+    const long long xrow = (long long)(mine ? m0 + r16 : P.M - 1) * P.ldx;
+    const int erow = tid < P.N ? tid : P.N - 1, full = P.K / Q8_BLOCK;
+    struct Ahead { u32x4 w[PER]; uint32_t e; Raw32<DT> x; };   // a thread's part of a block on its way
+    auto fetch_w = [&](Ahead& r, int kb, bool in) {
 #pragma unroll
         for (int i = 0; i < PER; ++i) {
             const int id = i * 256 + tid, row = (id >> 3) < P.N ? id >> 3 : P.N - 1;
-            if (PIECES % 256 == 0 || id < PIECES) r.w[i] = *reinterpret_cast<const u32x4*>(P.w + (long long)row * P.ldw + kb * 128LL + (id & 7) * 16);
+            r.w[i] = *reinterpret_cast<const u32x4*>(P.w + (in ? (long long)row * P.ldw + kb * 128LL + (id & 7) * 16 : 0));
         }
-        if (tid < BN) r.e = P.sw[(long long)erow * P.ldsw + kb];
+        r.e = P.sw[in ? (long long)erow * P.ldsw + kb : 0];
+    };
+    auto fetch = [&](Ahead& r, int kb) {
+        const bool in = kb < full;
+        fetch_w(r, kb, in);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) r.x.e[i] = el_raw8<DT>(P.x, in ? xrow + kb * 128 + (i >> 1) * 64 + quarter * 16 + (i & 1) * 8 : 0);
+    };
+    auto put = [&](const Ahead& r, int buf) {
+#pragma unroll
+        for (int i = 0; i < PER; ++i) {
+            const int id = i * 256 + tid, row = id >> 3;
+            if (PIECES % 256 == 0 || id < PIECES) *reinterpret_cast<u32x4_a*>(tile[buf] + row * 128 + (((id & 7) ^ ((row >> 1) & 7)) << 4)) = r.w[i];
+        }
+        if (tid < BN) exps[buf][(tid & 15) * 8 + (tid >> 4)] = (uint8_t)r.e;
+    };
+    auto meet = [&]() {   // this wave's reads of a buffer have returned and its part of the other one is written
+        asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+        __builtin_amdgcn_s_barrier();
+        asm volatile("" ::: "memory");
     };
     f32x4 acc[TN];
 #pragma unroll
     for (int t = 0; t < TN; ++t) acc[t] = f32x4{0.f, 0.f, 0.f, 0.f};
-    Rest r0, r1;
-    fetch_w(r0, 0);
-    r0.x = raw_block<DT>(P.x, xrow, 0, quarter, P.K, mine);
-    if (P.nb > 1) fetch_w(r1, 1);
-    r1.x = raw_block<DT>(P.x, xrow, 128, quarter, P.K, mine);   // (past the end: zeros, nothing is read)
-    auto step = [&](int kb, Rest& r) {
-        uint8_t* buf = tile[kb & 1];
+    Ahead r0, r1;
+    constexpr int TW = TN < 4 ? TN : 4;   // tiles of W whose fragments are held at once
+    Frag8 fx, fw[TW];
+    uint32_t byte;
+    q8_u32x2 ew;
+    auto read_w = [&](int buf, int t0) {
 #pragma unroll
-        for (int i = 0; i < PER; ++i) {
-            const int id = i * 256 + tid, row = id >> 3;
-            if (PIECES % 256 == 0 || id < PIECES) *reinterpret_cast<u32x4_a*>(buf + row * 128 + (((id & 7) ^ ((row >> 1) & 7)) << 4)) = r.w[i];
-        }
-        if (tid < BN) exps[kb & 1][tid] = (uint8_t)r.e;
-        if (kb + 2 < P.nb) fetch_w(r, kb + 2);
-        Frag8 fx;
-        const uint32_t byte = pack_rows16<DT, FX + 1>(r.x, fx);
-        r.x = raw_block<DT>(P.x, xrow, (kb + 2) * 128, quarter, P.K, mine);
-        // one barrier a block: the buffer written here was read two blocks ago, before every wave's previous barrier
-        asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
-        __builtin_amdgcn_s_barrier();
-        asm volatile("" ::: "memory");
+        for (int t = 0; t < TW; ++t)
 #pragma unroll
-        for (int t = 0; t < TN; ++t) {
-            Frag8 fw;
-            const int row = t * 16 + r16;
+            for (int u = 0; u < 2; ++u) {
+                const int row = (t0 + t) * 16 + r16;
+                fw[t].h[u] = *reinterpret_cast<const u32x4_a*>(tile[buf] + row * 128 + (((u * 4 + quarter) ^ ((row >> 1) & 7)) << 4));
+            }
+        ew = *reinterpret_cast<const u32x2_a*>(exps[buf] + r16 * 8);
+    };
+    auto products = [&](int buf) {
 #pragma unroll
-            for (int u = 0; u < 2; ++u) fw.h[u] = *reinterpret_cast<const u32x4_a*>(buf + row * 128 + (((u * 4 + quarter) ^ ((row >> 1) & 7)) << 4));
-            acc[t] = mma16<FW, FX, DT == KP_F32>(fw, exps[kb & 1][row], fx, byte, acc[t]);
+        for (int t0 = 0; t0 < TN; t0 += TW) {
+            if (t0) read_w(buf, t0);
+#pragma unroll
+            for (int t = 0; t < TW; ++t) acc[t0 + t] = mma16<FW, FX, DT == KP_F32>(fw[t], (int)(ew[t0 >> 2] >> (8 * t)), fx, byte, acc[t0 + t]);
         }
     };
-    for (int kb = 0; kb < P.nb; kb += 2) {
-        step(kb, r0);
-        if (kb + 1 < P.nb) step(kb + 1, r1);
+    auto step = [&](int kb, Ahead& r) {   // r: block kb + 1
+        Frag8 fxn;
+        put(r, (kb & 1) ^ 1);
+        const uint32_t byten = pack_rows16<DT, FX + 1>(r.x, fxn);
+        fetch(r, kb + 3);
+        __builtin_amdgcn_sched_barrier(0);
+        read_w(kb & 1, 0);
+        products(kb & 1);
+        fx = fxn;
+        byte = byten;
+        meet();
+    };
+    if (full) {
+        fetch(r0, 0);
+        fetch(r1, 1);
+        put(r0, 0);
+        byte = pack_rows16<DT, FX + 1>(r0.x, fx);
+        fetch(r0, 2);
+        meet();
+        for (int kb = 0; kb + 1 < full; kb += 2) {
+            step(kb, r1);
+            step(kb + 1, r0);
+        }
+        if (full & 1) step(full - 1, r1);
+    }
+    if (full < P.nb) {
+        fetch_w(r0, full, true);
+        r0.x = raw_block<DT>(P.x, xrow, full * 128, quarter, P.K, true);
+        put(r0, 0);
+        byte = pack_rows16<DT, FX + 1>(r0.x, fx);
+        meet();
+        read_w(0, 0);
+        products(0);
     }
     if (!mine) return;
 #pragma unroll
@@ -589,13 +633,16 @@ template <int FA, int FB, bool F32> int mm_launch(const MmArgs& P, const Plan& p
 // 16 rows 20.9 / 24.1; 1024 x 1024, 64 rows 4.4 / 8.1; 4096 x 1000, 32 rows 6.7 / 8.8, 64 rows 12.0 / 9.1; 512 x 8192 (32 workgroups that
 // walk 64 blocks each), 4 rows 10.6 / 11.3, 16 rows 14.8 / 12.2.  So: up to 16 rows, unless few workgroups walk far; more where the walk is
 // short and two rounds of workgroups are enough.
-// Few columns (128, bf16): a block takes a workgroup a microsecond, so it wants many rows or few blocks: K = 512: 32768 rows 12.3 / 19.2, 8192
-// rows 8.5 / 9.2, 2048 rows 7.7 / 6.9; K = 4096: 32768 rows 59.5 / 122, 8192 rows 37.9 / 35.2; K = 64: 2048 rows 4.8 / 5.5.
-int linear_way(long long M, long long N, long long K) {
+// Few columns (bf16): a block takes a workgroup 0.9 us (128 columns) or 0.6 (64), whatever the number of workgroups, so it wants many rows, or
+// few blocks and not all 128 columns.  128 columns: K = 512: 32768 rows 12.5 / 19.2, 8192 rows 7.9 / 9.3, 4096 rows 7.4 / 7.2; K = 4096: 32768 rows
+// 57.8 / 116, 8192 rows 30.3 / 35.5, 4096 rows 28.8 / 24.2; K = 200: 2048 rows 5.5 / 5.7.  64 columns: K = 512: 2048 rows 5.0 / 6.6; K = 2048:
+// 2048 rows 12.6 / 14.3; K = 4096: 2048 rows 22.2 / 18.2.  In fp32 a block takes nearly twice as long and packing does not: twice the rows.
+int linear_way(long long M, long long N, long long K, bool f32) {
     if (M <= 4) return 1;
     if (M <= 16) return K <= 4096 || N >= 4096 ? 1 : 0;
     if (K <= 1024 && ((N + 15) / 16) * ((M + 15) / 16) <= 512) return 1;
-    return N <= 128 && (M >= 16384 || (M >= 6144 && K <= 2048) || K <= 256) ? 2 : 0;
+    const long long rows = f32 ? M / 2 : M;
+    return N <= 128 && (rows >= 6144 || (N <= 64 && rows >= 2048 && K <= 2048) || K <= 256) ? 2 : 0;
 }
 
 template <int DT, int FX, int FW> int narrow_launch(const RowArgs& P, hipStream_t st) {
@@ -607,7 +654,7 @@ template <int DT, int FX, int FW> int narrow_launch(const RowArgs& P, hipStream_
     return kp_check_launch("q8_linear");
 }
 template <int DT, int FX> int linear_launch(const RowArgs& P, int fmtw, hipStream_t st) {
-    if (P.N <= 128 && linear_way(P.M, P.N, P.K) != 1) return fmtw == KP_E4M3 ? narrow_launch<DT, FX, 0>(P, st) : narrow_launch<DT, FX, 1>(P, st);
+    if (P.N <= 128 && linear_way(P.M, P.N, P.K, DT == KP_F32) != 1) return fmtw == KP_E4M3 ? narrow_launch<DT, FX, 0>(P, st) : narrow_launch<DT, FX, 1>(P, st);
     const bool two = P.N >= 32 * 256;
     const dim3 grid(cdiv(P.N, two ? 32 : 16), cdiv(P.M, 16));
     if (two) {
@@ -669,7 +716,7 @@ int kp_q8_matmul(const unsigned char* a, long long lda, const unsigned char* sa,
     return kp_check_launch("q8_matmul join");
 }
 
-int kp_q8_linear_suits(long long M, long long N, long long K) { return linear_way(M, N, K) != 0; }
+int kp_q8_linear_suits(long long M, long long N, long long K, int dtype) { return linear_way(M, N, K, dtype == KP_F32) != 0; }
 
 int kp_q8_linear(const void* x, long long ldx, int fmtx, const unsigned char* w, long long ldw, const unsigned char* sw, long long ldsw,
                  int fmtw, const float* bias, void* y, long long ldy, long long M, long long N, long long K, int dtype, void* stream) {

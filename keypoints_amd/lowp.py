@@ -329,7 +329,7 @@ def linear8(x: torch.Tensor, weight, bias: torch.Tensor = None, fmt: str = 'e4m3
         return torch.empty(shape, device=x.device, dtype=x.dtype)
     K = x.shape[-1]
     with device_of(x):
-        if _lib.lib().kp_q8_linear_suits(rows, N, K):
+        if _lib.lib().kp_q8_linear_suits(rows, N, K, DTYPES[x.dtype]):
             y = x.new_empty(shape)
             v, s = weight.values, weight.scales
             call('kp_q8_linear', ptr(m), ld, code, ptr(v), v.shape[1], ptr(s), s.shape[1], FORMATS[weight.fmt], ptr(bias), ptr(y), N,

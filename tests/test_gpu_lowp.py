@@ -165,6 +165,17 @@ def test_linear8_few_columns(M, N, K, dtype):
         assert bool((y[:, N:] == -7.0).all())
 
 
+@pytest.mark.parametrize('dtype', ['fp32', 'bf16', 'fp16'])
+@pytest.mark.parametrize('M,N,K', [(12301, 1, 1), (12300, 17, 100), (12500, 128, 128), (13000, 70, 255), (12289, 33, 384), (12290, 16, 520), (12400, 100, 1024)])
+def test_linear8_few_columns_many_rows(M, N, K, dtype):
+    """From no whole block to eight of them, each at a count of rows that takes the kernel by its rule."""
+    from keypoints_amd import _lib, lowp
+    assert _lib.lib().kp_q8_linear_suits(M, N, K, lowp.DTYPES[TYPES[dtype]]) and not (K <= 1024 and ((N + 15) // 16) * ((M + 15) // 16) <= 512)
+    x, w, bias = data(M, K, dtype=dtype, seed=3, spread=0.5), data(N, K, dtype='fp32', seed=4, spread=0.5) / K ** 0.5, torch.randn(N).cuda()
+    want, bound = product(quantise(x, 'e4m3')[0], quantise(w, 'e4m3')[0], dtype, bias)
+    close(lowp.linear8(x, lowp.pack8(w), bias), want, bound, dtype)
+
+
 @pytest.mark.parametrize('dtype,wtype', [('fp32', 'fp32'), ('bf16', 'fp32'), ('fp16', 'fp32'), ('bf16', 'bf16')])
 @pytest.mark.parametrize('M,N,K', [(1, 1, 1), (1, 33, 130), (5, 128, 64), (129, 40, 257), (300, 520, 200), (1000, 70, 130)])
 def test_linear8_training(M, N, K, dtype, wtype):
