@@ -8,9 +8,9 @@
 //             meets, so dw += dy xh and db += dy stay in its registers; one partial row a workgroup, joined by a second launch in a fixed
 //             order (fp64), so equal calls give equal bits
 //
-// Both are bound by memory.  Measured (a large copy reaches 5.2 TB/s here): 2097152 rows of 64 in bf16: forward 100 us = 5.4 TB/s,
-// backward 169 us = 4.8 TB/s (it reads two streams and writes a third; join 5 us); 8192 rows of 4096 in fp16 with an 8-bit copy: forward
-// 41 us = 4.1 TB/s, backward 42 us = 4.0 TB/s, join 4 us; 4099 x 1001 in fp32: 9 and 19 us (much of it in the last cache), join 5 us.
+// Both are bound by memory.  Measured (a large copy reaches 5.2 TB/s here): 2097152 rows of 64 in bf16: forward 112 us = 4.8 TB/s, backward with
+// join 157 us = 5.1 TB/s; 8192 rows of 4096 in fp16: forward 25.7 us = 5.2 TB/s, backward 43.7 us = 4.6 TB/s, with an 8-bit copy 38.4 and 38.1 us
+// = 4.4 TB/s (a pass of 170 MB: its start and end count); 4096 x 16384 in bf16 51 and 98 us = 5.3 and 4.1 TB/s.
 // A row is spread over G lanes, 8 consecutive elements (16 bytes of a 16-bit type) each, NJ times: the smallest
 // power of two that holds it up to a wave (rows of 64 elements: eight rows a wave; a wave takes up to 1024), then 4, 8 or 16 waves with
 // sums through LDS, and beyond 16384 elements a workgroup that walks the row and reads it again.
@@ -62,7 +62,8 @@ struct LnBwd {
 // How a row's last chunks are read.  FULL: rows of exactly 8 G NJ elements.  OVERLAP: a chunk that would reach past the end starts 8 elements
 // before it and counts those that no other lane has counted (it computes and stores the others as their lanes do): loads and stores stand in
 // no branch, behind which the compiler would wait for everything on its way, stores too.  Against PARTS, element by element, the backward
-// takes (bf16, us): 8192 x 4096 43.7 / 50.3, 32768 x 1024 45.6 / 53.1, 8192 x 8192 86.1 / 95.4, 2097152 x 64 157 / 159.
+// takes (bf16, us): 8192 x 4096 43.7 / 50.3, 32768 x 1024 45.6 / 53.1, 8192 x 8192 86.1 / 95.4, 2097152 x 64 157 / 159; the forward 32768 x 1024
+// 26.2 / 28.6, 32768 x 1000 27.9 / 30.5, 4096 x 16384 51.0 / 57.1, with an 8-bit copy 2097152 x 64 144 / 151.
 // PARTS stays for rows of less than 8 elements, and for kept rows whose overlapping chunk could lie in two blocks.
 enum LnEnds { LN_FULL, LN_OVERLAP, LN_PARTS };
 
@@ -74,30 +75,47 @@ template <int G> constexpr int ln_tpb = G > 64 ? 1024 : 256;
 template <int G> constexpr int ln_fwd_tpb = G > 64 ? G : 256;
 
 // KEEP: 0, or KP_E4M3 / KP_E5M2: the row leaves in 8 bits too
-template <int DT, int G, int NJ, int KEEP>
+template <int DT, int G, int NJ, int KEEP, int ENDS>
 __global__ __launch_bounds__(ln_fwd_tpb<G>) void ln_fwd_k(const LnFwd P) {
     constexpr int TPB = ln_fwd_tpb<G>, R = TPB / G;
     __shared__ float red[G > 64 ? 64 : 1];   // four sets of 16: two sums a row, alternating rows
     const int sub = threadIdx.x & (G - 1);
     const float inv = 1.f / (float)P.C;
-    int n[NJ];
+    int col[NJ], n[NJ], skip[NJ];   // as in the backward; lanes past the last block of 128 do what the last block's lanes do
     float w[NJ][8], b[NJ][8];
 #pragma unroll
     for (int j = 0; j < NJ; ++j) {
-        const int c = (j * G + sub) * 8, left = P.C - c;
-        n[j] = left < 0 ? 0 : (left < 8 ? left : 8);
+        int c = (j * G + sub) * 8;
+        const int left = P.C - c;
+        if (ENDS == LN_OVERLAP && KEEP != 0 && c >= P.nb * Q8_BLOCK) c = (P.nb - 1) * Q8_BLOCK + (c & (Q8_BLOCK - 1));
+        col[j] = ENDS == LN_OVERLAP && c > P.C - 8 ? P.C - 8 : c;
+        n[j] = ENDS != LN_PARTS || left >= 8 ? 8 : (left < 0 ? 0 : left);
+        skip[j] = ENDS == LN_OVERLAP && left < 8 ? (left < 0 ? 8 : 8 - left) : 0;
 #pragma unroll
         for (int k = 0; k < 8; ++k) { w[j][k] = 1.f; b[j][k] = 0.f; }
-        if (P.w) el_load8<KP_F32>(P.w, c, n[j], w[j]);
-        if (P.b) el_load8<KP_F32>(P.b, c, n[j], b[j]);
+        if (P.w) el_load8<KP_F32>(P.w, col[j], n[j], w[j]);
+        if (P.b) el_load8<KP_F32>(P.b, col[j], n[j], b[j]);
     }
-    const long long step = (long long)gridDim.x * R;
-    long long row = (long long)blockIdx.x * R + threadIdx.x / G;
     El8<DT> next[NJ];
+    auto fetch = [&](long long row) {
 #pragma unroll
-    for (int j = 0; j < NJ; ++j) next[j] = el_raw8_any<DT>(P.x, row * P.ldx + (j * G + sub) * 8, row < P.rows ? n[j] : 0);
-    for (long long r0 = (long long)blockIdx.x * R, odd = 0; r0 < P.rows; r0 += step, row += step, odd ^= 1) {
-        const bool live = row < P.rows;
+        for (int j = 0; j < NJ; ++j) {
+            if constexpr (ENDS != LN_PARTS) next[j] = el_raw8<DT>(P.x, row < P.rows ? row * P.ldx + col[j] : 0);
+            else next[j] = el_raw8_any<DT>(P.x, row * P.ldx + col[j], row < P.rows ? n[j] : 0);
+        }
+    };
+    const long long step = (long long)gridDim.x * R;
+    long long row = (long long)blockIdx.x * R + threadIdx.x / G, r0 = (long long)blockIdx.x * R, odd = 0;
+    float mean = 0.f, rstd = 0.f;
+    auto stats = [&](long long at) {
+        if (P.mean && sub == 0 && at >= 0 && at < P.rows) {
+            P.mean[at] = mean;
+            P.rstd[at] = rstd;
+        }
+    };
+    fetch(row);
+    auto turn = [&](auto ALL) {   // ALL: every row of the workgroup's turn is there
+        const bool live = decltype(ALL)::value || row < P.rows;
         float v[NJ][8];
         float sum[1] = {0.f}, sq[1] = {0.f};
         El8<DT> raw[KEEP ? NJ : 1];
@@ -106,43 +124,48 @@ __global__ __launch_bounds__(ln_fwd_tpb<G>) void ln_fwd_k(const LnFwd P) {
             if constexpr (KEEP != 0) raw[j] = next[j];
             el_unpack8<DT>(next[j], v[j]);
 #pragma unroll
-            for (int k = 0; k < 8; ++k) sum[0] += v[j][k];
+            for (int k = 0; k < 8; ++k) sum[0] += ENDS != LN_OVERLAP || k >= skip[j] ? v[j][k] : 0.f;
         }
-#pragma unroll
-        for (int j = 0; j < NJ; ++j) next[j] = el_raw8_any<DT>(P.x, (row + step) * P.ldx + (j * G + sub) * 8, row + step < P.rows ? n[j] : 0);
+        stats(row - step);   // (the row before's: behind the loads, these stores in a branch would make the next turn wait for this turn's)
+        fetch(row + step);
         float* slot = red + (G > 64 ? (odd ? 32 : 0) : 0);
         ln_sums<G, 1>(sum, slot);
-        const float mean = sum[0] * inv;
+        mean = sum[0] * inv;
 #pragma unroll
         for (int j = 0; j < NJ; ++j)
 #pragma unroll
             for (int k = 0; k < 8; ++k) {
-                v[j][k] = k < n[j] ? v[j][k] - mean : 0.f;
-                sq[0] = __builtin_fmaf(v[j][k], v[j][k], sq[0]);
+                v[j][k] = ENDS != LN_PARTS || k < n[j] ? v[j][k] - mean : 0.f;
+                const float once = ENDS != LN_OVERLAP || k >= skip[j] ? v[j][k] : 0.f;
+                sq[0] = __builtin_fmaf(once, once, sq[0]);
             }
         ln_sums<G, 1>(sq, slot + (G > 64 ? 16 : 0));
-        const float rstd = 1.f / sqrtf(sq[0] * inv + P.eps);
+        rstd = 1.f / sqrtf(sq[0] * inv + P.eps);
 #pragma unroll
         for (int j = 0; j < NJ; ++j) {
-            const int c = (j * G + sub) * 8;
             if constexpr (KEEP != 0) {
                 q8_u32x2 out;
                 const uint32_t byte = q8_pack_block<DT, KEEP, (G < 16 ? G : 16)>(raw[j], out);
                 if (live && n[j] > 0) {
-                    q8_store8(P.q + row * P.C + c, n[j], out);
-                    if ((c & (Q8_BLOCK - 1)) == 0) P.s[row * P.nb + c / Q8_BLOCK] = (uint8_t)byte;
+                    q8_store8(P.q + row * P.C + col[j], n[j], out);
+                    if (ENDS != LN_PARTS || (col[j] & (Q8_BLOCK - 1)) == 0) P.s[row * P.nb + col[j] / Q8_BLOCK] = (uint8_t)byte;   // (all of a block's lanes: no branch)
                 }
             }
             float o[8];
 #pragma unroll
             for (int k = 0; k < 8; ++k) o[k] = __builtin_fmaf(v[j][k] * rstd, w[j][k], b[j][k]);
-            if (live) el_store8<DT>(P.y, row * P.ldy + c, n[j], o);
+            if (live) el_store8<DT>(P.y, row * P.ldy + col[j], n[j], o);
         }
-        if (P.mean && sub == 0 && live) {
-            P.mean[row] = mean;
-            P.rstd[row] = rstd;
-        }
-    }
+        r0 += step;
+        row += step;
+        odd ^= 1;
+    };
+    if constexpr (ENDS != LN_PARTS) {
+        while (r0 + R <= P.rows) turn(std::true_type{});
+        if (r0 < P.rows) turn(std::false_type{});
+    } else
+        while (r0 < P.rows) turn(std::false_type{});
+    stats(row - step);
 }
 
 template <int DT, int G, int NJ, int KEEP, int ENDS>
@@ -404,7 +427,12 @@ template <int DT, int KEEP> int fwd_launch(const LnFwd& P, hipStream_t st) {
     const int g = ln_group(P.C), per = g > 64 ? 1 : 256 / g;
     const long long want = (P.rows + per - 1) / per, cap = g > 64 ? 1024 * 512 / g : 2048;
     const unsigned grid = (unsigned)(want < cap ? want : cap);
-#define LN_FWD(G, NJ) ln_fwd_k<DT, G, NJ, KEEP><<<grid, ln_fwd_tpb<G>, 0, st>>>(P)
+#define LN_FWD(G, NJ)                                                                                                    \
+    do {                                                                                                                 \
+        if (P.C == 8 * G * NJ) ln_fwd_k<DT, G, NJ, KEEP, LN_FULL><<<grid, ln_fwd_tpb<G>, 0, st>>>(P);                    \
+        else if (KEEP ? P.C % 8 == 0 : G > 1) ln_fwd_k<DT, G, NJ, KEEP, LN_OVERLAP><<<grid, ln_fwd_tpb<G>, 0, st>>>(P);  \
+        else ln_fwd_k<DT, KEEP ? G : 1, KEEP ? NJ : 1, KEEP, LN_PARTS><<<grid, ln_fwd_tpb<KEEP ? G : 1>, 0, st>>>(P);    \
+    } while (0)
     switch (g) {
         case 1: LN_FWD(1, 1); break;
         case 2: LN_FWD(2, 1); break;

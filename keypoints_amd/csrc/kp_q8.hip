@@ -1,8 +1,8 @@
 // The 8-bit block format of kp_q8_dev.h: rows to 8 bits, back, and both ways at once (rows and columns) with the column sums.
 // All of it is bound by memory: 2 (4) bytes of input and 1 byte per form an element.  Measured in bf16 (a large copy: 5.2 TB/s): 2^27 elements
-// in memory order 88 us to 8 bits = 4.6 TB/s and 64 us back = 6.3 TB/s (the bytes come partly out of the last cache, just written); both
-// ways at once 16384 x 2048 31 us (both forms), 16384 x 4096 62 us (both forms and column sums) = 4.3 TB/s.  More blocks of a thread in flight and
-// fewer operations an element changed none of these.
+// in memory order 74 us to 8 bits = 5.4 TB/s (88 where the card's memory was slower) and 64 us back = 6.3 TB/s (the bytes come partly out of
+// the last cache, just written); both ways at once 16384 x 2048 31 us (both forms), 16384 x 4096 62 us (both forms and column sums) = 4.3 TB/s.
+// More blocks of a thread in flight, loads a turn ahead in no branch and fewer operations an element changed none of these.
 #include "kp_q8_dev.h"
 
 namespace {
