@@ -187,8 +187,10 @@ _NO_FORM = (None, 0, None, 0)
 
 
 def _pack_both(m, rows, ld, width, dcode, code, q, qt, ws=None, colsum=None):
-    """kp_q8_pack_both of a matrix into a row form, a column form and column sums (each may be None)."""
-    if q is None and qt is None and colsum is None:
+    """A matrix into a row form, a column form and column sums (each may be None): kp_q8_pack_both, or kp_q8_pack for rows alone."""
+    if qt is None and colsum is None:
+        if q is not None:
+            call('kp_q8_pack', ptr(m), ld, q[0], q[1], q[2], q[3], rows, width, dcode, code, stream_ptr())
         return
     v, ldv, s, lds = q[:4] if q is not None else _NO_FORM
     vt, ldvt, st, ldst = qt[:4] if qt is not None else _NO_FORM
@@ -338,5 +340,5 @@ def linear8(x: torch.Tensor, weight, bias: torch.Tensor = None, fmt: str = 'e4m3
         forms = _Forms()
         q = forms.form(rows, K)
         forms.allocate(x)
-        call('kp_q8_pack', ptr(m), ld, q[0], q[1], q[2], q[3], rows, K, DTYPES[x.dtype], code, stream_ptr())
+        _pack_both(m, rows, ld, K, DTYPES[x.dtype], code, q, None)
         return _product(q, code, _form_of(weight), FORMATS[weight.fmt], bias, x, shape, x.dtype)
