@@ -226,7 +226,8 @@ __global__ __launch_bounds__(ln_tpb<G>) void ln_bwd_k(const LnBwd P) {
         constexpr bool all = decltype(ALL)::value;
         if constexpr (!PRE) fetch(next, row);
         float g[NJ][8], xh[NJ][8];
-        const float mean = next.mean, rstd = next.rstd;
+        const bool here = all || row < P.rows;   // (rows past the end were read at the first one's start)
+        const float mean = here ? next.mean : 0.f, rstd = here ? next.rstd : 0.f;
 #pragma unroll
         for (int j = 0; j < NJ; ++j) {
             if constexpr (KEEP != 0) q8_values8<KEEP>(next.q[j], q8_up(next.s[j]), xh[j]);
@@ -234,7 +235,10 @@ __global__ __launch_bounds__(ln_tpb<G>) void ln_bwd_k(const LnBwd P) {
             el_unpack8<DT>(next.dy[j], g[j]);
             if constexpr (ENDS != LN_PARTS && !all)
 #pragma unroll
-                for (int k = 0; k < 8; ++k) g[j][k] = row < P.rows ? g[j][k] : 0.f;
+                for (int k = 0; k < 8; ++k) {
+                    g[j][k] = here ? g[j][k] : 0.f;
+                    xh[j][k] = here ? xh[j][k] : 0.f;
+                }
         }
         if constexpr (PRE) fetch(next, row + step);
         float ab[2] = {0.f, 0.f};   // sums of g and of g xh; past the row's end g is zero
@@ -256,7 +260,7 @@ __global__ __launch_bounds__(ln_tpb<G>) void ln_bwd_k(const LnBwd P) {
         if (P.dx) {
             ln_sums<G, 2>(ab, red + (G > 64 ? (odd ? 32 : 0) : 0));
             const float a = ab[0] * inv, b = ab[1] * inv;
-            if (all || row < P.rows) {
+            if (here) {
 #pragma unroll
                 for (int j = 0; j < NJ; ++j) {
                     float o[8];

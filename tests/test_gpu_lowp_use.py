@@ -162,6 +162,24 @@ def test_not_a_numbers_stay_in_their_rows():
     assert bool(dw[:, 7].isnan().all()) and bool(dw[:, 8].isfinite().all())
 
 
+@pytest.mark.parametrize('keep', [None, 'e4m3'])
+def test_an_overflow_stays_in_its_column(keep):
+    """Row 0's element 0 is further from the mean than fp32 reaches: its normalised value is no number, every other one of the row is 0."""
+    from keypoints_amd import norm
+    x = rnd(3, 16, seed=1, dtype=torch.float32)
+    x[0] = -4e37
+    x[0, 0] = 3.4e38
+    w = rnd(16, seed=2, dtype=torch.float32)
+    dy = rnd(3, 16, seed=3, dtype=torch.float32)
+
+    def grads(rows):
+        leaves = [x[rows].clone().requires_grad_(), w.clone().requires_grad_(), w.clone().requires_grad_()]
+        return torch.autograd.grad(norm.layer_norm(*leaves, keep=keep), leaves, dy[rows])
+    dx, dw, db = grads(slice(0, 3))
+    _, want, _ = grads(slice(1, 3))
+    assert not dw[0].isfinite() and torch.equal(dw[1:], want[1:]) and bool(db.isfinite().all()) and bool(dx[1:].isfinite().all())
+
+
 def test_equal_calls_give_equal_bits_on_any_stream():
     from keypoints_amd import lowp, norm
     x, w, b = rnd(5000, 384, seed=1), rnd(384, seed=2, dtype=torch.float32), rnd(384, seed=3, dtype=torch.float32)
