@@ -11,8 +11,9 @@
 //                    sums (measured 6e-9 .. 4e-7 of the norm), at half its partner's rate.  Weight gradients go this way.
 //
 // Measured (bf16 / fp32 results; the library's 8-bit product reaches 2.75 PFLOP/s on the first): 8192^3 490 us = 2.25 PFLOP/s / 815 us =
-// 1.35, 4096^3 68 / 125 us = 2.0 / 1.1, 16384 x 2048 x 4096 119 / 204 us = 2.3 / 1.35.  The largest are bound by the power cap: at 8192^3 the clock falls
-// to 1.6 GHz with the matrix cores 62 % busy, at 4096^3 it stays at 2.2 GHz with 43 %.
+// 1.35 (555 / 840 on the slowest card), 4096^3 67 / 111 us = 2.0 / 1.25, 16384 x 2048 x 4096 119 / 204 us = 2.3 / 1.35, 2048^3 14 / 24 us.  The
+// largest are bound by the power cap: at 8192^3 the clock falls to 1.6 GHz with the matrix cores 62 % busy, at 4096^3 it stays at 2.2 GHz with
+// 43 %.  Raising the waves' priority around the products changes nothing.
 //
 // Any order of the elements inside a block serves, as long as A and B agree: the fragments are read as the swizzle likes them.
 #include <math.h>
