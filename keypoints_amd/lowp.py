@@ -40,6 +40,15 @@ def dtype_code(dtype: torch.dtype) -> int:
     return DTYPES[dtype]
 
 
+def real(t):
+    """t itself, or the tensor behind a map that a network returned unmade (models.functional.LazyNCHW): the wrapper carries no graph, so an
+    autograd Function that was handed it would pass no gradient on.  (Plain tensors leave by their type, without the import.)"""
+    if t is None or type(t) is torch.Tensor or type(t) is torch.nn.Parameter:
+        return t
+    from .models.functional import unlazy
+    return unlazy(t)
+
+
 def as_rows(x: torch.Tensor):
     """x [..., width] as (tensor, rows, row stride): x itself where its rows lie one stride apart (a column slice of a matrix does), else a
     contiguous copy."""
@@ -108,6 +117,7 @@ def _dense(x: torch.Tensor) -> bool:
 def checkpoint8(x: torch.Tensor, fmt: str = 'e4m3') -> Packed8:
     """x in 8 bits, to be kept between a forward and its backward: `.unpack()` gives it back with its shape, strides and type.  The blocks
     run over the elements in memory order, across rows, whatever the shape; no gradient flows through it."""
+    x = real(x)
     code, dcode = format_code(fmt), dtype_code(x.dtype)
     require_device(x)
     if not _dense(x):
@@ -128,6 +138,7 @@ def _sizes(rows, width):
 
 def pack8(x: torch.Tensor, fmt: str = 'e4m3') -> Packed8:
     """x [..., width] as a product's operand, blocks along the last dimension.  No gradient flows through it (linear8 has its own)."""
+    x = real(x)
     code, dcode = format_code(fmt), dtype_code(x.dtype)
     require_device(x)
     if x.dim() < 1 or x.shape[-1] < 1:
@@ -221,6 +232,7 @@ def _check_bias(bias, width, device):
 def matmul8(a: Packed8, b: Packed8, bias: torch.Tensor = None, dtype: torch.dtype = None) -> torch.Tensor:
     """a @ b.T (+ bias) of two operand forms: a [..., k], b [n, k] -> [..., n] in `dtype` (a's by default), accumulated in fp32 and rounded
     once (16-bit results: with the 8-bit matrix instruction's own cut, include/kp_hip.h).  The formats may differ."""
+    bias = real(bias)
     for name, p in (('a', a), ('b', b)):
         if not isinstance(p, Packed8) or p.flat:
             raise TypeError(f'matmul8: {name} must be a pack8 operand')
@@ -303,6 +315,7 @@ def linear8(x: torch.Tensor, weight, bias: torch.Tensor = None, fmt: str = 'e4m3
     bias.  The backward packs the output gradient in `grad_fmt` and takes dx and dw from two more 8-bit products; between the passes only
     8-bit forms wait (a byte an element of x and of the weight).  Gradients come in the types of what they belong to.
     weight a Packed8 (pack8): serving.  `fmt` is x's format; no gradient."""
+    x, weight, bias = real(x), real(weight), real(bias)
     require_device(x, bias)
     code = format_code(fmt)
     format_code(grad_fmt)

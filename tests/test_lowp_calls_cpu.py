@@ -1,0 +1,63 @@
+"""CPU: the calls that keypoints_amd.lowp and norm make of a user's calls, with the launches noted instead of made (tests/launch_stub.py)."""
+import pytest
+import torch
+
+from launch_stub import stub
+
+from keypoints_amd import _lib, lowp, norm
+
+
+@pytest.fixture
+def made(monkeypatch):
+    return stub(monkeypatch)
+
+
+def lazy(requires_grad=True):
+    """(source, the map a network returns): the fp32 image of a padded bf16 tensor, made when somebody looks at it."""
+    from keypoints_amd.models.functional import LazyNCHW
+    source = torch.zeros(1, 6, 10, 3, dtype=torch.bfloat16, requires_grad=requires_grad)
+    return source, LazyNCHW(source * 1, 1, _lib.KP_BF16)
+
+
+@pytest.mark.parametrize('op', ['norm', 'kept', 'linear'])
+def test_a_lazy_map_passes_its_gradient_on(made, op):
+    """TransporterNet.forward returns its blend as a wrapper that carries no graph itself: the operators run on the tensor behind it."""
+    source, x = lazy()
+    w = torch.zeros(5, 8, requires_grad=True)
+    y = lowp.linear8(x, w) if op == 'linear' else norm.layer_norm(x, keep='e4m3' if op == 'kept' else None)
+    assert y.requires_grad
+    y.sum().backward()
+    assert source.grad is not None and source.grad.shape == source.shape
+
+
+def test_lazy_weights_and_biases(made):
+    source, m = lazy()
+    x = torch.zeros(2, 8)
+    for fn in (lambda t: norm.layer_norm(x, t), lambda t: norm.layer_norm(x, None, t), lambda t: lowp.linear8(x, torch.zeros(8, 8), t)):
+        from keypoints_amd.models.functional import LazyNCHW
+
+        class Row(LazyNCHW):
+            """A lazy tensor of the shape these arguments have."""
+            @staticmethod
+            def __new__(cls):
+                return torch.Tensor._make_wrapper_subclass(cls, (8,), dtype=torch.float32)
+
+            def __init__(self):
+                pass
+
+            def materialize(self):
+                return source.float()[0, 1, 1:9, 0]
+
+        source.grad = None
+        fn(Row()).sum().backward()
+        assert source.grad is not None
+    with pytest.raises(RuntimeError, match='carries no gradient'):
+        lowp.linear8(m, lowp.pack8(torch.zeros(5, 8)))
+
+
+def test_packing_a_lazy_map_reads_the_map(made):
+    _, x = lazy()
+    for fn in (lowp.checkpoint8, lowp.pack8):
+        made.clear()
+        fn(x)
+        assert made[-1][0] == 'kp_q8_pack' and made[-1][1][0] == x.materialize().data_ptr() != 0
