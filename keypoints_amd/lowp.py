@@ -17,6 +17,7 @@ more, down to zero).  Not-a-numbers stay what they are, so an overflowing fp16 s
 from __future__ import annotations
 
 import torch
+from torch.autograd import forward_ad
 from torch.autograd.function import once_differentiable
 
 from . import _lib
@@ -47,6 +48,13 @@ def real(t):
         return t
     from .models.functional import unlazy
     return unlazy(t)
+
+
+def no_tangents(op, *tensors):
+    """Refuses inputs of forward-mode differentiation: the operators have no formula for it, and a result without a tangent would read as a
+    derivative of zero."""
+    if forward_ad._current_level >= 0 and any(isinstance(t, torch.Tensor) and forward_ad.unpack_dual(t).tangent is not None for t in tensors):
+        raise RuntimeError(f'{op}: no forward-mode derivative; take the reverse one, or hand over the primal tensors')
 
 
 def as_rows(x: torch.Tensor):
@@ -233,6 +241,7 @@ def matmul8(a: Packed8, b: Packed8, bias: torch.Tensor = None, dtype: torch.dtyp
     """a @ b.T (+ bias) of two operand forms: a [..., k], b [n, k] -> [..., n] in `dtype` (a's by default), accumulated in fp32 and rounded
     once (16-bit results: with the 8-bit matrix instruction's own cut, include/kp_hip.h).  The formats may differ."""
     bias = real(bias)
+    no_tangents('matmul8', bias)
     for name, p in (('a', a), ('b', b)):
         if not isinstance(p, Packed8) or p.flat:
             raise TypeError(f'matmul8: {name} must be a pack8 operand')
@@ -316,6 +325,7 @@ def linear8(x: torch.Tensor, weight, bias: torch.Tensor = None, fmt: str = 'e4m3
     8-bit forms wait (a byte an element of x and of the weight).  Gradients come in the types of what they belong to.
     weight a Packed8 (pack8): serving.  `fmt` is x's format; no gradient."""
     x, weight, bias = real(x), real(weight), real(bias)
+    no_tangents('linear8', x, weight, bias)
     require_device(x, bias)
     code = format_code(fmt)
     format_code(grad_fmt)

@@ -11,7 +11,7 @@ from torch.autograd.function import once_differentiable
 
 from . import _lib
 from ._lib import call, ptr
-from .lowp import BLOCK, DTYPES, FORMATS, as_rows, as_vector, dtype_code, format_code, real
+from .lowp import BLOCK, DTYPES, FORMATS, as_rows, as_vector, dtype_code, format_code, no_tangents, real
 from .runtime import device_of, require_device, stream_ptr
 
 
@@ -71,6 +71,7 @@ def layer_norm(x: torch.Tensor, weight: torch.Tensor = None, bias: torch.Tensor 
     in which a copy of x waits for it: half the memory of a 16-bit x, and the gradients of x and weight are taken with
     the copy's values (each off from x by at most 2^-4 / 2^-3 of itself) and x's own statistics."""
     x, weight, bias, eps = real(x), real(weight), real(bias), float(eps)
+    no_tangents('layer_norm', x, weight, bias)
     C = x.shape[-1] if x.dim() else 0
     if not (x.is_cuda and C > 0 and x.dtype in DTYPES and 0.0 <= eps < _INF and (keep is None or keep in FORMATS)
             and _plain_vector(weight, C, x) and _plain_vector(bias, C, x)):

@@ -61,3 +61,28 @@ def test_packing_a_lazy_map_reads_the_map(made):
         made.clear()
         fn(x)
         assert made[-1][0] == 'kp_q8_pack' and made[-1][1][0] == x.materialize().data_ptr() != 0
+
+
+def test_forward_mode_is_refused_not_lost(made):
+    """A dual tensor's tangent goes through none of the operators: a call that would return its result without one says so."""
+    import torch.autograd.forward_ad as fwd
+    x, w, v = torch.zeros(3, 8), torch.zeros(5, 8), torch.zeros(8)
+    packed = lowp.pack8(w)
+    with fwd.dual_level():
+        dual = lambda t: fwd.make_dual(t, torch.ones_like(t))
+        calls = [lambda: norm.layer_norm(dual(x)), lambda: norm.layer_norm(x, dual(v)), lambda: norm.layer_norm(x, None, dual(v)),
+                 lambda: norm.layer_norm(dual(x), keep='e4m3'), lambda: lowp.linear8(dual(x), w), lambda: lowp.linear8(x, dual(w)),
+                 lambda: lowp.linear8(x, w, dual(torch.zeros(5))), lambda: lowp.linear8(dual(x), packed),
+                 lambda: lowp.linear8(x, packed, dual(torch.zeros(5))), lambda: lowp.matmul8(packed, packed, dual(torch.zeros(5)))]
+        for grad in (True, False):
+            for fn in calls:
+                made.clear()
+                with torch.set_grad_enabled(grad), pytest.raises(RuntimeError):
+                    fn()
+                assert not any(name != 'kp_q8_pack' for name, _ in made)
+        for plain in (lambda: norm.layer_norm(x, v, v), lambda: lowp.linear8(x, packed), lambda: lowp.linear8(x, w), lambda: lowp.matmul8(packed, packed)):
+            plain()   # (nothing carries a tangent)
+    for transform in (lambda f: torch.func.jvp(f, (x,), (torch.ones_like(x),)), lambda f: torch.func.grad(lambda t: f(t).sum())(x)):
+        for f in (norm.layer_norm, lambda t: lowp.linear8(t, w), lambda t: lowp.linear8(t, packed)):
+            with pytest.raises(RuntimeError):
+                transform(f)
