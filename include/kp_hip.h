@@ -582,16 +582,16 @@ int kp_q8_linear_suits(long long M, long long N, long long K, int dtype);
 /* ---- layer norm ----------------------------------------------------------------------------------------------------------------
  * Per row of C elements: y = (x - mean) * rstd * w + b, rstd = 1 / sqrt(mean((x - mean)^2) + eps).  w, b fp32 or NULL (1, 0).  mean, rstd
  * [rows] fp32 are written when not NULL (both or none).  q, s (both or none): x in the 8-bit format as well, q [rows][C] back to back,
- * s [rows][ceil(C / 128)]: what the backward may read instead of x. */
+ * s [rows][ceil(C / 128)]: what the backward may read instead of x.  C up to 2^30. */
 int kp_layer_norm_fwd(const void* x, long long ldx, const float* w, const float* b, float eps, void* y, long long ldy, float* mean,
-                      float* rstd, unsigned char* q, unsigned char* s, int fmt, long long rows, int C, int dtype, void* stream);
+                      float* rstd, unsigned char* q, unsigned char* s, int fmt, long long rows, long long C, int dtype, void* stream);
 /* dx = rstd (g - mean(g) - xh mean(g xh)) with g = dy w, xh = (x - mean) rstd (x, or the values q, s stand for); dw = sum dy xh, db = sum
  * dy, fp32, overwritten; each of dx, dw, db may be NULL.  ws: kp_layer_norm_bwd_ws_floats floats when dw or db is asked for.  Sums are
  * taken in a fixed order. */
 int kp_layer_norm_bwd(const void* dy, long long lddy, const void* x, long long ldx, const unsigned char* q, const unsigned char* s, int fmt,
                       const float* w, const float* mean, const float* rstd, void* dx, long long lddx, float* ws, float* dw, float* db,
-                      long long rows, int C, int dtype, void* stream);
-long long kp_layer_norm_bwd_ws_floats(long long rows, int C);
+                      long long rows, long long C, int dtype, void* stream);
+long long kp_layer_norm_bwd_ws_floats(long long rows, long long C);
 
 /* ---- loss and optimiser -------------------------------------------------- */
 /* l2_reconstruction_loss (transporter.py:56-60): loss_sum[0] += sum (x-t)^2*mask (fp64, zeroed by caller);

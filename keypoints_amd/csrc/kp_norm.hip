@@ -408,6 +408,7 @@ __global__ __launch_bounds__(256) void ln_cols_long_k(const LnBwd P) {
 
 // ---- which kernel -----------------------------------------------------------------------------------------------------------------
 constexpr int LONG = 16384;
+constexpr long long MOST = 1LL << 30;   // columns are counted in 32 bits, a partial row of 2 C floats and a walk's last step past its end included
 int ln_group(int C) {   // lanes of a row
     if (C > 1024) return C > 4096 ? 1024 : C > 2048 ? 512 : 256;
     int g = 1;
@@ -495,35 +496,37 @@ template <int DT> int bwd_type(const LnBwd& P, int fmt, int parts, hipStream_t s
 extern "C" {
 
 int kp_layer_norm_fwd(const void* x, long long ldx, const float* w, const float* b, float eps, void* y, long long ldy, float* mean,
-                      float* rstd, unsigned char* q, unsigned char* s, int fmt, long long rows, int C, int dtype, void* stream) {
+                      float* rstd, unsigned char* q, unsigned char* s, int fmt, long long rows, long long C, int dtype, void* stream) {
     KP_REQUIRE(dtype == KP_F32 || dtype == KP_BF16 || dtype == KP_F16, "kp_layer_norm_fwd: unknown dtype %d", dtype);
-    KP_REQUIRE(x && y && rows > 0 && C > 0 && (rows == 1 || (ldx >= C && ldy >= C)), "kp_layer_norm_fwd: bad args (%lld x %d, strides %lld, %lld)", rows, C, ldx, ldy);
+    KP_REQUIRE(x && y && rows > 0 && C > 0 && (rows == 1 || (ldx >= C && ldy >= C)), "kp_layer_norm_fwd: bad args (%lld x %lld, strides %lld, %lld)", rows, C, ldx, ldy);
+    KP_REQUIRE(C <= MOST, "kp_layer_norm_fwd: %lld columns are more than one call takes (2^30)", C);
     KP_REQUIRE(eps >= 0.f && !mean == !rstd && !q == !s && (!q || fmt == KP_E4M3 || fmt == KP_E5M2), "kp_layer_norm_fwd: mean with rstd, q with s, a known format, eps >= 0");
-    LnFwd P{x, w, b, y, mean, rstd, q, s, ldx, ldy, rows, C, (C + Q8_BLOCK - 1) / Q8_BLOCK, eps};
+    LnFwd P{x, w, b, y, mean, rstd, q, s, ldx, ldy, rows, (int)C, (int)((C + Q8_BLOCK - 1) / Q8_BLOCK), eps};
     const hipStream_t st = (hipStream_t)stream;
     kp_count_bytes((double)rows * C * (2 * (dtype == KP_F32 ? 4 : 2) + (q ? 1 : 0)));
     return dtype == KP_F32 ? fwd_type<KP_F32>(P, fmt, st) : dtype == KP_BF16 ? fwd_type<KP_BF16>(P, fmt, st) : fwd_type<KP_F16>(P, fmt, st);
 }
 
-long long kp_layer_norm_bwd_ws_floats(long long rows, int C) {
-    return rows > 0 && C > 0 ? (long long)ln_parts(rows, C) * 2 * C : 0;
+long long kp_layer_norm_bwd_ws_floats(long long rows, long long C) {
+    return rows > 0 && C > 0 && C <= MOST ? ln_parts(rows, (int)C) * 2 * C : 0;
 }
 
 int kp_layer_norm_bwd(const void* dy, long long lddy, const void* x, long long ldx, const unsigned char* q, const unsigned char* s, int fmt,
                       const float* w, const float* mean, const float* rstd, void* dx, long long lddx, float* ws, float* dw, float* db,
-                      long long rows, int C, int dtype, void* stream) {
+                      long long rows, long long C, int dtype, void* stream) {
     KP_REQUIRE(dtype == KP_F32 || dtype == KP_BF16 || dtype == KP_F16, "kp_layer_norm_bwd: unknown dtype %d", dtype);
-    KP_REQUIRE(dy && mean && rstd && (dx || dw || db) && rows > 0 && C > 0, "kp_layer_norm_bwd: bad args (%lld x %d)", rows, C);
-    KP_REQUIRE(rows == 1 || (lddy >= C && (!dx || lddx >= C) && (!x || ldx >= C)), "kp_layer_norm_bwd: row strides %lld, %lld, %lld for %d columns", lddy, ldx, lddx, C);
+    KP_REQUIRE(dy && mean && rstd && (dx || dw || db) && rows > 0 && C > 0, "kp_layer_norm_bwd: bad args (%lld x %lld)", rows, C);
+    KP_REQUIRE(C <= MOST, "kp_layer_norm_bwd: %lld columns are more than one call takes (2^30)", C);
+    KP_REQUIRE(rows == 1 || (lddy >= C && (!dx || lddx >= C) && (!x || ldx >= C)), "kp_layer_norm_bwd: row strides %lld, %lld, %lld for %lld columns", lddy, ldx, lddx, C);
     KP_REQUIRE((x != nullptr) != (q != nullptr) && !q == !s && (!q || fmt == KP_E4M3 || fmt == KP_E5M2), "kp_layer_norm_bwd: either x or its 8-bit form");
     KP_REQUIRE(ws || !(dw || db), "kp_layer_norm_bwd: the weight's gradient needs a workspace (kp_layer_norm_bwd_ws_floats)");
-    const int parts = ln_parts(rows, C);
-    LnBwd P{dy, x, q, s, w, mean, rstd, dx, (dw || db) ? ws : nullptr, lddy, ldx, lddx, rows, C, (C + Q8_BLOCK - 1) / Q8_BLOCK};
+    const int parts = ln_parts(rows, (int)C);
+    LnBwd P{dy, x, q, s, w, mean, rstd, dx, (dw || db) ? ws : nullptr, lddy, ldx, lddx, rows, (int)C, (int)((C + Q8_BLOCK - 1) / Q8_BLOCK)};
     const hipStream_t st = (hipStream_t)stream;
     kp_count_bytes((double)rows * C * (2 * (dtype == KP_F32 ? 4 : 2) + (q ? 1 : (dtype == KP_F32 ? 4 : 2))));
     const int rc = dtype == KP_F32 ? bwd_type<KP_F32>(P, fmt, parts, st) : dtype == KP_BF16 ? bwd_type<KP_BF16>(P, fmt, parts, st) : bwd_type<KP_F16>(P, fmt, parts, st);
     if (rc != KP_OK || !(dw || db)) return rc;
-    q8_join_k<<<cdiv(2LL * C, 16), 1024, 0, st>>>(ws, parts, 2LL * C, dw, C, db);
+    q8_join_k<<<cdiv(2 * C, 16), 1024, 0, st>>>(ws, parts, 2 * C, dw, C, db);
     return kp_check_launch("layer_norm_bwd join");
 }
 

@@ -73,7 +73,7 @@ def layer_norm(x: torch.Tensor, weight: torch.Tensor = None, bias: torch.Tensor 
     x, weight, bias, eps = real(x), real(weight), real(bias), float(eps)
     no_tangents('layer_norm', x, weight, bias)
     C = x.shape[-1] if x.dim() else 0
-    if not (x.is_cuda and C > 0 and x.dtype in DTYPES and 0.0 <= eps < _INF and (keep is None or keep in FORMATS)
+    if not (x.is_cuda and 0 < C <= MOST and x.dtype in DTYPES and 0.0 <= eps < _INF and (keep is None or keep in FORMATS)
             and _plain_vector(weight, C, x) and _plain_vector(bias, C, x)):
         weight, bias = _checked(x, weight, bias, eps, keep, C)
     if torch.is_grad_enabled() and (x.requires_grad or (weight is not None and weight.requires_grad) or (bias is not None and bias.requires_grad)):
@@ -82,6 +82,7 @@ def layer_norm(x: torch.Tensor, weight: torch.Tensor = None, bias: torch.Tensor 
 
 
 _INF = float('inf')
+MOST = 1 << 30   # columns
 
 
 def _plain_vector(t, C, x):
@@ -95,8 +96,8 @@ def _checked(x, weight, bias, eps, keep, C):
     dtype_code(x.dtype)
     if keep is not None:
         format_code(keep)
-    if C < 1:
-        raise ValueError(f'layer_norm: the last dimension must hold at least one element, got shape {tuple(x.shape)}')
+    if not 1 <= C <= MOST:
+        raise ValueError(f'layer_norm: the last dimension must hold at least one element and at most 2^30, got shape {tuple(x.shape)}')
     if not 0.0 <= eps < _INF:
         raise ValueError(f'layer_norm: eps must be a number that is not negative, got {eps}')
     for name, t in (('weight', weight), ('bias', bias)):

@@ -86,3 +86,23 @@ def test_forward_mode_is_refused_not_lost(made):
         for f in (norm.layer_norm, lambda t: lowp.linear8(t, w), lambda t: lowp.linear8(t, packed)):
             with pytest.raises(RuntimeError):
                 transform(f)
+
+
+def test_rows_longer_than_the_kernels_count(made):
+    """Sizes that 32 bits do not hold arrive whole and are refused (2^32 + 8 columns are not 8); the largest row that is taken has 2^30."""
+    import ctypes
+    L, p = _lib.lib(), ctypes.c_void_p(256)   # a non-null address that nothing reads
+
+    def bad(name, *args):
+        assert getattr(L, name)(*args) == -1 and name in L.kp_last_error().decode()
+    for C in ((1 << 30) + 1, (1 << 31) - 8, (1 << 31) + 8, (1 << 32) + 8):
+        bad('kp_layer_norm_fwd', p, C, None, None, 1e-5, p, C, None, None, None, None, 0, 2, C, 1, None)
+        bad('kp_layer_norm_bwd', p, C, p, C, None, None, 0, None, p, p, p, C, p, p, p, 2, C, 1, None)
+        assert L.kp_layer_norm_bwd_ws_floats(2, C) == 0
+        long = torch.zeros(1).expand(1, C)   # (no memory behind it)
+        made.clear()
+        for call in (lambda: norm.layer_norm(long), lambda: norm.layer_norm(long, keep='e4m3')):
+            with pytest.raises(ValueError, match='last dimension'):
+                call()
+        assert not made
+    assert L.kp_layer_norm_bwd_ws_floats(2, 1 << 30) == 2 * 2 * (1 << 30)
