@@ -263,6 +263,25 @@ def matmul8(a: Packed8, b: Packed8, bias: torch.Tensor = None, dtype: torch.dtyp
         return _product(_form_of(a), FORMATS[a.fmt], _form_of(b), FORMATS[b.fmt], bias, a.values, shape, dtype)
 
 
+def _forward(x, weight, bias, code, need_x, need_w):
+    """-> y = P(x) P(w)^T + b and what a backward reads: P'(x) where the weight's gradient is wanted, P'(w) where x's is (None: neither)."""
+    m, rows, ld = as_rows(x)
+    N, K = weight.shape
+    shape = (*x.shape[:-1], N)
+    if rows == 0 or N == 0:
+        return torch.empty(shape, device=x.device, dtype=x.dtype), None
+    with device_of(x):
+        w2, _, wld = as_rows(weight)
+        now, later = _Forms(), _Forms()
+        qx, qw = now.form(rows, K), now.form(N, K)
+        qxt, qwt = later.form(K, rows, need_w), later.form(K, N, need_x)
+        now.allocate(x)
+        kept = later.allocate(x) if need_x or need_w else None
+        _pack_both(m, rows, ld, K, DTYPES[x.dtype], code, qx, qxt)
+        _pack_both(w2, N, wld, K, DTYPES[weight.dtype], code, qw, qwt)
+        return _product(qx, code, qw, code, bias, x, shape, x.dtype), kept
+
+
 class _Linear8(torch.autograd.Function):
     """y = P(x) P(w)^T + b;  dx = P(dy) P'(w),  dw = P'(dy)^T P'(x),  db = column sums of dy.  P: blocks along the product's inner index, P':
     along the other one (w along its rows, x and dy along the batch), so that every product's operands have their blocks along its own
@@ -270,25 +289,11 @@ class _Linear8(torch.autograd.Function):
 
     @staticmethod
     def forward(ctx, x, weight, bias, fmt, grad_fmt):
-        code, grad_code = FORMATS[fmt], FORMATS[grad_fmt]
-        m, rows, ld = as_rows(x)
-        N, K = weight.shape
-        shape = (*x.shape[:-1], N)
-        ctx.args = (x.shape, x.dtype, (N, K), weight.dtype, code, grad_code)
-        if rows == 0 or N == 0:
-            return torch.empty(shape, device=x.device, dtype=x.dtype)
-        need_x, need_w = ctx.needs_input_grad[:2]
-        with device_of(x):
-            w2, _, wld = as_rows(weight)
-            now, later = _Forms(), _Forms()
-            qx, qw = now.form(rows, K), now.form(N, K)
-            qxt, qwt = later.form(K, rows, need_w), later.form(K, N, need_x)
-            now.allocate(x)
-            if need_x or need_w:
-                ctx.save_for_backward(later.allocate(x))
-            _pack_both(m, rows, ld, K, DTYPES[x.dtype], code, qx, qxt)
-            _pack_both(w2, N, wld, K, DTYPES[weight.dtype], code, qw, qwt)
-            return _product(qx, code, qw, code, bias, x, shape, x.dtype)
+        ctx.args = (x.shape, x.dtype, weight.shape, weight.dtype, FORMATS[fmt], FORMATS[grad_fmt])
+        y, kept = _forward(x, weight, bias, FORMATS[fmt], *ctx.needs_input_grad[:2])
+        if kept is not None:
+            ctx.save_for_backward(kept)
+        return y
 
     @staticmethod
     @once_differentiable
@@ -344,9 +349,10 @@ def linear8(x: torch.Tensor, weight, bias: torch.Tensor = None, fmt: str = 'e4m3
     N = weight.shape[0]
     _check_bias(bias, N, x.device)
     bias = as_vector(bias)
+    grad = torch.is_grad_enabled() and (x.requires_grad or (bias is not None and bias.requires_grad) or (not packed and weight.requires_grad))
     if not packed:
-        return _Linear8.apply(x, weight, bias, fmt, grad_fmt)
-    if torch.is_grad_enabled() and (x.requires_grad or (bias is not None and bias.requires_grad)):
+        return _Linear8.apply(x, weight, bias, fmt, grad_fmt) if grad else _forward(x, weight, bias, code, False, False)[0]
+    if grad:
         raise RuntimeError('linear8: a packed weight carries no gradient; pass the weight itself, or run under torch.no_grad()')
     shape = (*x.shape[:-1], N)
     m, rows, ld = as_rows(x)

@@ -106,3 +106,28 @@ def test_rows_longer_than_the_kernels_count(made):
                 call()
         assert not made
     assert L.kp_layer_norm_bwd_ws_floats(2, 1 << 30) == 2 * 2 * (1 << 30)
+
+
+def names(made):
+    return [name for name, _ in made]
+
+
+def test_a_layer_evaluated_without_gradients_packs_rows_only(made):
+    """torch.no_grad() around a layer whose weight is a Parameter: no column form, nothing kept, and any number of rows."""
+    x, b = torch.zeros(300, 64), torch.nn.Parameter(torch.zeros(40))
+    w = torch.nn.Parameter(torch.zeros(40, 64))
+    with torch.no_grad():
+        for leaf in (x, x.clone().requires_grad_()):
+            made.clear()
+            y = lowp.linear8(leaf, w, b)
+            assert names(made) == ['kp_q8_pack', 'kp_q8_pack', 'kp_q8_matmul'] and not y.requires_grad
+    made.clear()
+    assert not lowp.linear8(x, w.detach(), b.detach()).requires_grad and names(made) == ['kp_q8_pack', 'kp_q8_pack', 'kp_q8_matmul']
+    made.clear()
+    y = lowp.linear8(x, w, b)
+    assert names(made) == ['kp_q8_pack_both', 'kp_q8_pack', 'kp_q8_matmul']
+    y.sum().backward()
+    assert w.grad is not None and b.grad is not None
+    with torch.inference_mode():
+        made.clear()
+        assert lowp.linear8(x[:0], w, b).shape == (0, 40) and not made
