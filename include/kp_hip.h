@@ -556,7 +556,7 @@ int kp_q8_unpack(const unsigned char* q, long long ldq, const unsigned char* s, 
  * blocks), the column form (qt, st: row c holds column c of x, blocks along the rows, padded alike; qt on a multiple of 16 bytes) and the
  * fp32 column sums colsum[cols] (fixed order; ws: kp_q8_pack_both_ws_floats floats).  The forward of a linear layer packs its input both
  * ways -- rows for its own product, columns for the weight gradient's, which is the activation checkpoint -- and the backward its output
- * gradient, with the bias gradient as column sums. */
+ * gradient, with the bias gradient as column sums.  Up to 8388480 rows (65535 tiles of 128). */
 int kp_q8_pack_both(const void* x, long long ldx, unsigned char* q, long long ldq, unsigned char* s, long long lds, unsigned char* qt,
                     long long ldqt, unsigned char* st, long long ldst, float* ws, float* colsum, long long rows, long long cols, int dtype,
                     int fmt, void* stream);

@@ -26,6 +26,7 @@ from .runtime import device_of, require_device, stream_ptr
 
 BLOCK = 128
 FORMATS = {'e4m3': _lib.KP_E4M3, 'e5m2': _lib.KP_E5M2}
+MOST = 65535 * BLOCK   # elements a product's sum runs over (kp_q8_matmul, and the rows that kp_q8_pack_both turns): 8388480
 DTYPES = {torch.float32: _lib.KP_F32, torch.bfloat16: _lib.KP_BF16, torch.float16: _lib.KP_F16}
 
 
@@ -237,6 +238,15 @@ def _check_bias(bias, width, device):
         raise ValueError(f'the bias must be a vector of {width} floats on {device}, got {tuple(bias.shape)} {bias.dtype} on {bias.device}')
 
 
+def _check_sizes(op, rows, columns, *sums):
+    """What kp_q8_matmul and kp_q8_pack_both take in one call; `sums`: (name, length) of every sum that a product of this call runs over."""
+    for name, n in sums:
+        if n > MOST:
+            raise ValueError(f'{op}: the sum over {n} {name} is longer than one product takes ({MOST}): split it')
+    if rows > 0x7fffff00 or columns > 0x1fffff00:
+        raise ValueError(f'{op}: {rows} x {columns} results are more than one product takes (2^31 - 256 rows, 2^29 - 256 columns)')
+
+
 def matmul8(a: Packed8, b: Packed8, bias: torch.Tensor = None, dtype: torch.dtype = None) -> torch.Tensor:
     """a @ b.T (+ bias) of two operand forms: a [..., k], b [n, k] -> [..., n] in `dtype` (a's by default), accumulated in fp32 and rounded
     once (16-bit results: with the 8-bit matrix instruction's own cut, include/kp_hip.h).  The formats may differ."""
@@ -252,6 +262,7 @@ def matmul8(a: Packed8, b: Packed8, bias: torch.Tensor = None, dtype: torch.dtyp
     dtype = a.dtype if dtype is None else dtype
     dtype_code(dtype)
     _check_bias(bias, b.shape[0], a.values.device)
+    _check_sizes('matmul8', a.values.shape[0], b.shape[0], ('inner elements', b.shape[1]))
     if torch.is_grad_enabled() and bias is not None and bias.requires_grad:
         raise RuntimeError('matmul8: packed operands carry no gradient, and none would reach the bias; run under torch.no_grad()')
     require_device(a.values, a.scales, b.values, b.scales)
@@ -322,12 +333,18 @@ class _Linear8(torch.autograd.Function):
         return dx, dw, db, None, None
 
 
+def _suits(rows, N, K, code):
+    """Whether x goes to the product as it is (kp_q8_linear)."""
+    return _lib.lib().kp_q8_linear_suits(rows, N, K, code) != 0
+
+
 def linear8(x: torch.Tensor, weight, bias: torch.Tensor = None, fmt: str = 'e4m3', grad_fmt: str = 'e4m3') -> torch.Tensor:
     """x [..., k] @ weight.T (+ bias) in 8-bit products: [..., n] in x's type.
 
     weight a tensor [n, k] (fp32 master weights, or 16 bits): every call packs x and the weight in `fmt`; differentiable in x, weight and
     bias.  The backward packs the output gradient in `grad_fmt` and takes dx and dw from two more 8-bit products; between the passes only
-    8-bit forms wait (a byte an element of x and of the weight).  Gradients come in the types of what they belong to.
+    8-bit forms wait (a byte an element of x and of the weight).  Gradients come in the types of what they belong to.  A product sums over at
+    most 8388480 elements: rows, where the weight's or bias's gradient is asked for (larger batches in parts, whose gradients add up).
     weight a Packed8 (pack8): serving.  `fmt` is x's format; no gradient."""
     x, weight, bias = real(x), real(weight), real(bias)
     no_tangents('linear8', x, weight, bias)
@@ -351,16 +368,27 @@ def linear8(x: torch.Tensor, weight, bias: torch.Tensor = None, fmt: str = 'e4m3
     bias = as_vector(bias)
     grad = torch.is_grad_enabled() and (x.requires_grad or (bias is not None and bias.requires_grad) or (not packed and weight.requires_grad))
     if not packed:
+        sums = [('inner elements', x.shape[-1])]
+        if grad:
+            if x.requires_grad:
+                sums.append(("outputs (x's gradient)", N))
+            if weight.requires_grad or (bias is not None and bias.requires_grad):
+                sums.append(("rows (the weight's and bias's gradients)", x.numel() // x.shape[-1]))
+        _check_sizes('linear8', x.numel() // x.shape[-1], N, *sums)
         return _Linear8.apply(x, weight, bias, fmt, grad_fmt) if grad else _forward(x, weight, bias, code, False, False)[0]
     if grad:
         raise RuntimeError('linear8: a packed weight carries no gradient; pass the weight itself, or run under torch.no_grad()')
     shape = (*x.shape[:-1], N)
-    m, rows, ld = as_rows(x)
+    K = x.shape[-1]
+    rows = x.numel() // K
     if rows == 0 or N == 0:
         return torch.empty(shape, device=x.device, dtype=x.dtype)
-    K = x.shape[-1]
+    suits = _suits(rows, N, K, DTYPES[x.dtype])
+    if not suits:
+        _check_sizes('linear8', rows, N, ('inner elements', K))
+    m, _, ld = as_rows(x)
     with device_of(x):
-        if _lib.lib().kp_q8_linear_suits(rows, N, K, DTYPES[x.dtype]):
+        if suits:
             y = x.new_empty(shape)
             v, s = weight.values, weight.scales
             call('kp_q8_linear', ptr(m), ld, code, ptr(v), v.shape[1], ptr(s), s.shape[1], FORMATS[weight.fmt], ptr(bias), ptr(y), N,

@@ -131,3 +131,43 @@ def test_a_layer_evaluated_without_gradients_packs_rows_only(made):
     with torch.inference_mode():
         made.clear()
         assert lowp.linear8(x[:0], w, b).shape == (0, 40) and not made
+
+
+@pytest.mark.parametrize('rows,width,inner,wants', [(8388481, 3, 4, 'w'), (8388481, 3, 4, 'b'), (8388608, 3, 4, 'xwb'), (3, 8388481, 4, 'x'),
+                                                    (5, 3, 8388481, ''), (5, 3, 8388481, 'w'), (40, 1 << 29, 1, '')])
+def test_products_longer_than_one_call_takes(made, rows, width, inner, wants):
+    """A sum over more than 8388480 elements -- the rows are the weight gradient's -- is refused by the call itself, not between its launches or
+    in the backward; where no such sum is asked for, any number of rows passes."""
+    x = torch.zeros(1, dtype=torch.bfloat16).expand(rows, inner).requires_grad_('x' in wants)   # (no memory behind it)
+    w = torch.zeros(1).expand(width, inner).requires_grad_('w' in wants)
+    b = torch.zeros(width).requires_grad_('b' in wants) if width < 10 else None
+    with pytest.raises(ValueError, match='8388480|2\\^29'):
+        lowp.linear8(x, w, b)
+    assert not made
+
+
+def test_many_rows_without_the_weights_gradient(made, monkeypatch):
+    monkeypatch.setattr(lowp, 'MOST', 256)
+    x, w, b = torch.zeros(300, 8), torch.zeros(5, 8), torch.zeros(5)
+    leaf = lambda t: t.clone().requires_grad_()
+    lowp.linear8(leaf(x), w, b).sum().backward()
+    lowp.linear8(x, w, b)
+    with torch.no_grad():
+        lowp.linear8(x, leaf(w), leaf(b))
+    for args in ((x, leaf(w), b), (x, w, leaf(b)), (leaf(torch.zeros(3, 8)), torch.zeros(300, 8), None), (torch.zeros(3, 300), torch.zeros(5, 300), None)):
+        made.clear()
+        with pytest.raises(ValueError, match='256'):
+            lowp.linear8(*args)
+        assert not made
+    for rows, kind in ((4, None), (20, ValueError)):   # serving: a few rows are summed by a kernel without that limit
+        x, packed = torch.zeros(rows, 600, dtype=torch.bfloat16), lowp.pack8(torch.zeros(300, 600))
+        monkeypatch.setattr(lowp, '_suits', lambda M, N, K, code: M <= 4)
+        made.clear()
+        if kind is None:
+            lowp.linear8(x, packed)
+        else:
+            with pytest.raises(kind, match='256'):
+                lowp.linear8(x, packed)
+            assert not made
+    with pytest.raises(ValueError, match='256'):
+        lowp.matmul8(packed, packed)
