@@ -76,6 +76,14 @@ def as_vector(t):
     return t.to(torch.float32).contiguous()
 
 
+def saved(t: torch.Tensor, shape, dtype, device):
+    """A saved tensor as the backward got it.  Saved-tensor hooks (offloading, compression) may give back another one: with other strides,
+    which is fine, or of another size, type or place, of which the kernels would read past the end."""
+    if t.shape != shape or t.dtype is not dtype or t.device != device:
+        raise RuntimeError(f'a saved tensor of shape {tuple(shape)}, {dtype}, on {device} came back from its hook as {tuple(t.shape)}, {t.dtype}, on {t.device}')
+    return t
+
+
 class Packed8:
     """A tensor in the 8-bit block format: `values` (bytes), `scales` (exponent bytes), the `shape` and `dtype` it stands for.
 
@@ -322,7 +330,8 @@ class _Linear8(torch.autograd.Function):
             later, now = _Forms(), _Forms()
             qxt, qwt = later.form(K, rows, need_w), later.form(K, N, need_x)
             if need_x or need_w:
-                later.rebase(ctx.saved_tensors[0])
+                kept = saved(ctx.saved_tensors[0], (later.bytes,), torch.uint8, dev).contiguous()
+                later.rebase(kept if kept.data_ptr() % 16 == 0 else kept.clone())   # (what the products take)
             qd, qdt = now.form(rows, N, need_x), now.form(N, rows, need_w)
             ws = now.floats(_lib.lib().kp_q8_pack_both_ws_floats(rows, N), need_b)
             now.allocate(dy)

@@ -11,7 +11,7 @@ from torch.autograd.function import once_differentiable
 
 from . import _lib
 from ._lib import call, ptr
-from .lowp import BLOCK, DTYPES, FORMATS, as_rows, as_vector, dtype_code, format_code, no_tangents, real
+from .lowp import BLOCK, DTYPES, FORMATS, as_rows, as_vector, dtype_code, format_code, no_tangents, real, saved
 from .runtime import device_of, require_device, stream_ptr
 
 
@@ -49,8 +49,16 @@ class _LayerNorm(torch.autograd.Function):
         weight, st, kept, s = ctx.saved_tensors
         need_x, need_w, need_b = ctx.needs_input_grad[:3]
         g, rows, ldg = as_rows(dy)
-        kept, _, ldx = as_rows(kept)   # (a saved-tensor hook may give x back with other strides)
-        C = dy.shape[-1]
+        C, dev, f32 = dy.shape[-1], dy.device, torch.float32
+        st = saved(st, (2, rows), f32, dev).contiguous()
+        if weight is not None:
+            weight = saved(weight, (C,), f32, dev).contiguous()
+        if keep:
+            kept = saved(kept, (rows, C), torch.uint8, dev).contiguous()
+            s = saved(s, (rows, (C + BLOCK - 1) // BLOCK), torch.uint8, dev).contiguous()
+            ldx = C
+        else:
+            kept, _, ldx = as_rows(saved(kept, dy.shape, dy.dtype, dev))
         make = st.new_empty if rows else st.new_zeros   # (no rows: nothing is launched)
         dx = dy.new_empty(dy.shape) if need_x else None
         dw = make(C) if need_w else None

@@ -1,4 +1,6 @@
 """CPU: the calls that keypoints_amd.lowp and norm make of a user's calls, with the launches noted instead of made (tests/launch_stub.py)."""
+import ctypes
+
 import pytest
 import torch
 
@@ -90,7 +92,6 @@ def test_forward_mode_is_refused_not_lost(made):
 
 def test_rows_longer_than_the_kernels_count(made):
     """Sizes that 32 bits do not hold arrive whole and are refused (2^32 + 8 columns are not 8); the largest row that is taken has 2^30."""
-    import ctypes
     L, p = _lib.lib(), ctypes.c_void_p(256)   # a non-null address that nothing reads
 
     def bad(name, *args):
@@ -171,3 +172,60 @@ def test_many_rows_without_the_weights_gradient(made, monkeypatch):
             assert not made
     with pytest.raises(ValueError, match='256'):
         lowp.matmul8(packed, packed)
+
+
+HOOKS = {   # what a saved tensor may come back as: (still the same numbers, or refused)
+    'columns of a wider one': (True, lambda t: torch.cat([t, t], -1)[..., :t.shape[-1]]),
+    'every second row': (True, lambda t: torch.stack([t, t], 1).flatten(0, 1)[::2]),
+    'transposed': (True, lambda t: t.t().contiguous().t() if t.dim() == 2 else t.clone()),
+    'another type': (False, lambda t: t.to(torch.float64)),
+    'fewer elements': (False, lambda t: t[..., :-1].contiguous()),
+    'off the device': (False, lambda t: t.to('meta')),
+}
+
+
+@pytest.mark.parametrize('how', HOOKS)
+@pytest.mark.parametrize('op', ['norm', 'kept', 'linear'])
+def test_saved_tensors_as_hooks_give_them_back(made, monkeypatch, op, how):
+    """Saved-tensor hooks may hand a backward any tensor: it reads what has the right numbers where they lie, and refuses the rest."""
+    same, change = HOOKS[how]
+    x, w = torch.randn(6, 140, requires_grad=True), torch.randn(140, requires_grad=True)
+    weight = torch.randn(5, 140, requires_grad=True)
+    given = []
+    keep = lambda t: t.detach().clone().random_(1, 100) if t.dtype == torch.uint8 or t.shape == (2, 6) else t.detach().clone()   # (not written: no launch)
+    with torch.autograd.graph.saved_tensors_hooks(keep, lambda t: given.append((t, change(t))) or given[-1][1]):
+        y = lowp.linear8(x, weight) if op == 'linear' else norm.layer_norm(x, w, keep='e4m3' if op == 'kept' else None)
+    made.clear()
+    if not same:
+        with pytest.raises(RuntimeError, match='saved'):
+            y.sum().backward()
+        assert not made
+        return
+    by = lambda shape, dtype: next(t for t, _ in given if tuple(t.shape) == shape and t.dtype == dtype)
+
+    def numbers(address, shape, dtype, stride=None):
+        rows, width = shape if len(shape) == 2 else (1, shape[0])
+        flat = torch.frombuffer(bytearray((ctypes.c_char * (((rows - 1) * (stride or width) + width) * dtype.itemsize)).from_address(address)), dtype=dtype)
+        return flat.as_strided((rows, width), (stride or width, 1)).reshape(shape)
+
+    def look(name, *a):   # (while the call's own copies live)
+        made.append((name, a))
+        if name == 'kp_layer_norm_bwd':
+            _, _, xp, ldx, q, s, _, wp, mean, rstd = a[:10]
+            if op == 'kept':
+                assert torch.equal(numbers(q, (6, 140), torch.uint8), by((6, 140), torch.uint8)) and torch.equal(numbers(s, (6, 2), torch.uint8), by((6, 2), torch.uint8))
+            else:
+                assert torch.equal(numbers(xp, (6, 140), torch.float32, ldx), x)
+            st = by((2, 6), torch.float32)
+            assert torch.equal(numbers(wp, (140,), torch.float32), w)
+            assert torch.equal(numbers(mean, (6,), torch.float32), st[0]) and torch.equal(numbers(rstd, (6,), torch.float32), st[1])
+        if name == 'kp_q8_matmul':   # dx = P(dy) P'(w), dw = P'(dy)^T P'(x): the second operand is what was kept
+            blob = given[0][0]
+            first = len([m for m in made if m[0] == 'kp_q8_matmul']) == 1   # (x's column form lies first: 140 rows of 128 bytes and their exponents)
+            at = 140 * 128 + 768 if first else 0
+            assert torch.equal(numbers(a[5], (140 * 128,), torch.uint8), blob[at:at + 140 * 128]) and a[5] % 16 == 0
+
+    for module in (lowp, norm):
+        monkeypatch.setattr(module, 'call', look)
+    y.sum().backward()
+    assert names(made) == (['kp_q8_pack_both', 'kp_q8_matmul', 'kp_q8_matmul'] if op == 'linear' else ['kp_layer_norm_bwd'])
