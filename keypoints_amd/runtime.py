@@ -70,6 +70,7 @@ _side_streams = {}     # (device index, parent stream id, role) -> torch.cuda.St
 # runs on: torch hands streams out of a pool of 32 in turn, so a stream an application (or a graph capture) gets may be one that was once
 # taken as a side stream here
 _FORKED = contextvars.ContextVar('keypoints_amd_forked_from', default=None)
+_forks = {}            # side stream -> the stream of its last side block's fork (for forwards that a backward runs again, forked_from)
 _used = set()          # side streams with work their parent has not waited for yet
 
 
@@ -106,8 +107,17 @@ def side_stream(role: str) -> torch.cuda.Stream:
 
 def forked_from():
     """The stream this code's side block was forked from (None outside a side block).  A forward notes it for its backward, which the autograd
-    engine runs on the same stream in no block."""
-    return _FORKED.get()
+    engine runs on the same stream in no block.  A forward that a backward runs again (torch.utils.checkpoint) is in no block either: there the
+    stream decides, unless only one of the two is being captured -- then it is one that the pool handed out anew."""
+    stream = _FORKED.get()
+    if stream is None and torch._C._current_graph_task_id() != -1:
+        stream = _forks.get(torch.cuda.current_stream())
+        if stream is not None:
+            here = torch.cuda.is_current_stream_capturing()
+            with torch.cuda.stream(stream):
+                if torch.cuda.is_current_stream_capturing() != here:
+                    return None
+    return stream
 
 
 def nested_fork_under_capture(forked) -> bool:
@@ -163,6 +173,7 @@ class fork:
             self._cur = torch.cuda.current_stream()
             self._stream = side_stream(self._role)
             self._stream.wait_stream(self._cur)
+            _forks[self._stream] = self._cur
             _held.pop(self._stream, None)   # the parent's readers of the previous outputs are behind this wait
         return _SideBlock(self)
 
