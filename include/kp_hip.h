@@ -571,6 +571,8 @@ int kp_q8_matmul(const unsigned char* a, long long lda, const unsigned char* sa,
                  long long ldb, const unsigned char* sb, long long ldsb, int fmtb, const float* bias, void* c, long long ldc, float* ws,
                  long long M, long long N, long long K, int dtype, void* stream);
 long long kp_q8_matmul_ws_floats(long long M, long long N, long long K, int dtype);
+/* edge of the output tiles that it takes for these sizes: 64, 128 or 256 (0: sizes it refuses) */
+int kp_q8_matmul_tile(long long M, long long N, long long K, int dtype);
 /* y T [M][N] = sum_k P(x)[m][k] w[n][k] (+ bias[n]) for x T [M][K], P(x) = x's row form in fmtx, formed in registers: what kp_q8_pack +
  * kp_q8_matmul give (up to the order of the fp32 additions) in one launch, for a few rows (w is streamed once for every 16) or a few
  * columns (N <= 128: x is read once). */

@@ -682,6 +682,10 @@ long long kp_q8_matmul_ws_floats(long long M, long long N, long long K, int dtyp
     return p.splits > 1 ? p.splits * M * N : 0;
 }
 
+int kp_q8_matmul_tile(long long M, long long N, long long K, int dtype) {
+    return mm_sizes_ok(M, N, K) ? plan_of(M, N, (int)((K + Q8_BLOCK - 1) / Q8_BLOCK), dtype == KP_F32).tile : 0;
+}
+
 int kp_q8_matmul(const unsigned char* a, long long lda, const unsigned char* sa, long long ldsa, int fmta, const unsigned char* b,
                  long long ldb, const unsigned char* sb, long long ldsb, int fmtb, const float* bias, void* c, long long ldc, float* ws,
                  long long M, long long N, long long K, int dtype, void* stream) {
