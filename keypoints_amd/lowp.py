@@ -45,16 +45,16 @@ def dtype_code(dtype: torch.dtype) -> int:
 def real(t):
     """t itself, or the tensor behind a map that a network returned unmade (models.functional.LazyNCHW): the wrapper carries no graph, so an
     autograd Function that was handed it would pass no gradient on.  (Plain tensors leave by their type, without the import.)"""
-    if t is None or type(t) is torch.Tensor or type(t) is torch.nn.Parameter:
+    if type(t) in PLAIN:
         return t
     from .models.functional import unlazy
     return unlazy(t)
 
 
 def no_tangents(op, *tensors):
-    """Refuses inputs of forward-mode differentiation: the operators have no formula for it, and a result without a tangent would read as a
+    """(Inside a level of forward-mode differentiation: forward_ad._current_level >= 0.)  Refuses inputs of forward-mode differentiation: the operators have no formula for it, and a result without a tangent would read as a
     derivative of zero."""
-    if forward_ad._current_level >= 0 and any(isinstance(t, torch.Tensor) and forward_ad.unpack_dual(t).tangent is not None for t in tensors):
+    if any(isinstance(t, torch.Tensor) and forward_ad.unpack_dual(t).tangent is not None for t in tensors):
         raise RuntimeError(f'{op}: no forward-mode derivative; take the reverse one, or hand over the primal tensors')
 
 
@@ -117,6 +117,9 @@ class Packed8:
             with device_of(v):
                 call('kp_q8_unpack', ptr(v), ldq, ptr(s), lds, ptr(y), width, rows, width, code, FORMATS[self.fmt], stream_ptr())
         return y
+
+
+PLAIN = frozenset((torch.Tensor, torch.nn.Parameter, type(None), Packed8))
 
 
 def _dense(x: torch.Tensor) -> bool:
@@ -259,7 +262,8 @@ def matmul8(a: Packed8, b: Packed8, bias: torch.Tensor = None, dtype: torch.dtyp
     """a @ b.T (+ bias) of two operand forms: a [..., k], b [n, k] -> [..., n] in `dtype` (a's by default), accumulated in fp32 and rounded
     once (16-bit results: with the 8-bit matrix instruction's own cut, include/kp_hip.h).  The formats may differ."""
     bias = real(bias)
-    no_tangents('matmul8', bias)
+    if forward_ad._current_level >= 0:
+        no_tangents('matmul8', bias)
     for name, p in (('a', a), ('b', b)):
         if not isinstance(p, Packed8) or p.flat:
             raise TypeError(f'matmul8: {name} must be a pack8 operand')
@@ -355,8 +359,10 @@ def linear8(x: torch.Tensor, weight, bias: torch.Tensor = None, fmt: str = 'e4m3
     8-bit forms wait (a byte an element of x and of the weight).  Gradients come in the types of what they belong to.  A product sums over at
     most 8388480 elements: rows, where the weight's or bias's gradient is asked for (larger batches in parts, whose gradients add up).
     weight a Packed8 (pack8): serving.  `fmt` is x's format; no gradient."""
-    x, weight, bias = real(x), real(weight), real(bias)
-    no_tangents('linear8', x, weight, bias)
+    if not (type(x) in PLAIN and type(weight) in PLAIN and type(bias) in PLAIN):
+        x, weight, bias = real(x), real(weight), real(bias)
+    if forward_ad._current_level >= 0:
+        no_tangents('linear8', x, weight, bias)
     require_device(x, bias)
     code = format_code(fmt)
     format_code(grad_fmt)
@@ -377,13 +383,11 @@ def linear8(x: torch.Tensor, weight, bias: torch.Tensor = None, fmt: str = 'e4m3
     bias = as_vector(bias)
     grad = torch.is_grad_enabled() and (x.requires_grad or (bias is not None and bias.requires_grad) or (not packed and weight.requires_grad))
     if not packed:
-        sums = [('inner elements', x.shape[-1])]
-        if grad:
-            if x.requires_grad:
-                sums.append(("outputs (x's gradient)", N))
-            if weight.requires_grad or (bias is not None and bias.requires_grad):
-                sums.append(("rows (the weight's and bias's gradients)", x.numel() // x.shape[-1]))
-        _check_sizes('linear8', x.numel() // x.shape[-1], N, *sums)
+        K = weight.shape[1]
+        rows = x.numel() // K
+        if rows > MOST or N > MOST or K > MOST:
+            _check_sizes('linear8', rows, N, ('inner elements', K), ("outputs (x's gradient)", N if grad and x.requires_grad else 0),
+                         ("rows (the weight's and bias's gradients)", rows if grad and (weight.requires_grad or (bias is not None and bias.requires_grad)) else 0))
         return _Linear8.apply(x, weight, bias, fmt, grad_fmt) if grad else _forward(x, weight, bias, code, False, False)[0]
     if grad:
         raise RuntimeError('linear8: a packed weight carries no gradient; pass the weight itself, or run under torch.no_grad()')
@@ -393,7 +397,7 @@ def linear8(x: torch.Tensor, weight, bias: torch.Tensor = None, fmt: str = 'e4m3
     if rows == 0 or N == 0:
         return torch.empty(shape, device=x.device, dtype=x.dtype)
     suits = _suits(rows, N, K, DTYPES[x.dtype])
-    if not suits:
+    if not suits and (rows > MOST or N > MOST or K > MOST):
         _check_sizes('linear8', rows, N, ('inner elements', K))
     m, _, ld = as_rows(x)
     with device_of(x):

@@ -7,11 +7,12 @@ the same in training and inference, no running statistics, nothing to synchronis
 from __future__ import annotations
 
 import torch
+from torch.autograd import forward_ad
 from torch.autograd.function import once_differentiable
 
 from . import _lib
 from ._lib import call, ptr
-from .lowp import BLOCK, DTYPES, FORMATS, as_rows, as_vector, dtype_code, format_code, no_tangents, real, saved
+from .lowp import BLOCK, DTYPES, FORMATS, PLAIN, as_rows, as_vector, dtype_code, format_code, no_tangents, real, saved
 from .runtime import device_of, require_device, stream_ptr
 
 
@@ -78,8 +79,11 @@ def layer_norm(x: torch.Tensor, weight: torch.Tensor = None, bias: torch.Tensor 
     vectors of x.shape[-1] floats or None.  keep: None -- the backward reads x itself -- or the 8-bit format ('e4m3', 'e5m2'; keypoints_amd.lowp)
     in which a copy of x waits for it: half the memory of a 16-bit x, and the gradients of x and weight are taken with
     the copy's values (each off from x by at most 2^-4 / 2^-3 of itself) and x's own statistics."""
-    x, weight, bias, eps = real(x), real(weight), real(bias), float(eps)
-    no_tangents('layer_norm', x, weight, bias)
+    if not (type(x) in PLAIN and type(weight) in PLAIN and type(bias) in PLAIN):
+        x, weight, bias = real(x), real(weight), real(bias)
+    if forward_ad._current_level >= 0:
+        no_tangents('layer_norm', x, weight, bias)
+    eps = float(eps)
     C = x.shape[-1] if x.dim() else 0
     if not (x.is_cuda and 0 < C <= MOST and x.dtype in DTYPES and 0.0 <= eps < _INF and (keep is None or keep in FORMATS)
             and _plain_vector(weight, C, x) and _plain_vector(bias, C, x)):
