@@ -564,7 +564,8 @@ long long kp_q8_pack_both_ws_floats(long long rows, long long cols);
 /* c T [M][N] = sum_k a[m][k] b[n][k] (+ bias[n], fp32, may be NULL), fp32 accumulation, rounded once.  Results in fp32 are sums of exact
  * products.  Results in 16 bits come from the 8-bit matrix instruction, which aligns the products of 8 neighbouring k to the largest of them
  * and cuts them below 2^-13 of it: before the rounding they are off by less than 7 * 2^-13 of the sum of those largest products (measured:
- * 1e-5 .. 7e-5 of the result's norm).  a, b: row forms along k padded to whole blocks, rows on multiples of 16 bytes; rows of exponent
+ * 1e-5 .. 7e-5 of the result's norm; a result whose products cancel can be off by more than its last place).  In fp32 elements below 2^-126
+ * may be lost, and one that the format rounded up to 2^128 is an infinity.  a, b: row forms along k padded to whole blocks, rows on multiples of 16 bytes; rows of exponent
  * bytes on multiples of 4 bytes with whole words readable (lds % 4 == 0).  K, lda, ldb, ldsa, ldsb below 2^23.
  * ws: kp_q8_matmul_ws_floats floats (0 for most shapes: then NULL), used when few tiles split the sum; joined in a fixed order. */
 int kp_q8_matmul(const unsigned char* a, long long lda, const unsigned char* sa, long long ldsa, int fmta, const unsigned char* b,
