@@ -323,7 +323,9 @@ __device__ __forceinline__ float ln_total(float v, float* red) {   // over a wor
     return t[0];
 }
 
-// Rows past 16384 elements: a workgroup walks the row, element by element and thread, and reads it again for each pass.
+// Rows past 16384 elements: a workgroup walks the row, element by element and thread, and reads it again for each pass (three times forward;
+// twice backward and once more for the columns).  Right for any length, not made fast: 4096 x 20000 in bf16 174 us forward and 311 backward,
+// 2.7 and 3.3 times what their bytes take (4096 x 16384 above: 1.0 and 1.3).
 template <int DT, int KEEP>
 __global__ __launch_bounds__(1024) void ln_fwd_long_k(const LnFwd P) {
     __shared__ float red[32];

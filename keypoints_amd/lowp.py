@@ -135,8 +135,8 @@ def _dense(x: torch.Tensor) -> bool:
 
 
 def checkpoint8(x: torch.Tensor, fmt: str = 'e4m3') -> Packed8:
-    """x in 8 bits, to be kept between a forward and its backward: `.unpack()` gives it back with its shape, strides and type.  The blocks
-    run over the elements in memory order, across rows, whatever the shape; no gradient flows through it."""
+    """x in 8 bits, to be kept between a forward and its backward: `.unpack()` gives it back with its shape, strides (a tensor with gaps or
+    repeated elements: dense ones) and type.  The blocks run over the elements in memory order, across rows, whatever the shape; no gradient flows through it."""
     x = real(x)
     code, dcode = format_code(fmt), dtype_code(x.dtype)
     require_device(x)
@@ -385,7 +385,6 @@ def linear8(x: torch.Tensor, weight, bias: torch.Tensor = None, fmt: str = 'e4m3
         raise ValueError(f'linear8: x on {x.device}, the weight on {dev}')
     N = weight.shape[0]
     _check_bias(bias, N, x.device)
-    bias = as_vector(bias)
     grad = torch.is_grad_enabled() and (x.requires_grad or (bias is not None and bias.requires_grad) or (not packed and weight.requires_grad))
     if not packed:
         K = weight.shape[1]
@@ -393,6 +392,7 @@ def linear8(x: torch.Tensor, weight, bias: torch.Tensor = None, fmt: str = 'e4m3
         if rows > MOST or N > MOST or K > MOST:
             _check_sizes('linear8', rows, N, ('inner elements', K), ("outputs (x's gradient)", N if grad and x.requires_grad else 0),
                          ("rows (the weight's and bias's gradients)", rows if grad and (weight.requires_grad or (bias is not None and bias.requires_grad)) else 0))
+        bias = as_vector(bias)
         return _Linear8.apply(x, weight, bias, fmt, grad_fmt) if grad else _forward(x, weight, bias, code, False, False)[0]
     if grad:
         raise RuntimeError('linear8: a packed weight carries no gradient; pass the weight itself, or run under torch.no_grad()')
@@ -404,6 +404,7 @@ def linear8(x: torch.Tensor, weight, bias: torch.Tensor = None, fmt: str = 'e4m3
     suits = _suits(rows, N, K, DTYPES[x.dtype])
     if not suits and (rows > MOST or N > MOST or K > MOST):
         _check_sizes('linear8', rows, N, ('inner elements', K))
+    bias = as_vector(bias)
     m, _, ld = as_rows(x)
     with device_of(x):
         if suits:
