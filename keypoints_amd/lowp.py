@@ -289,6 +289,22 @@ def matmul8(a: Packed8, b: Packed8, bias: torch.Tensor = None, dtype: torch.dtyp
         return _product(_form_of(a), FORMATS[a.fmt], _form_of(b), FORMATS[b.fmt], bias, a.values, shape, dtype)
 
 
+def _parts(rows):
+    """(first row, rows) of the parts in which a batch is packed along itself: one, but past MOST rows.  They begin on whole blocks, so the blocks
+    are the whole batch's; the weight's and bias's gradients add up over the parts."""
+    return ((0, rows),) if rows <= MOST else tuple((at, min(MOST, rows - at)) for at in range(0, rows, MOST))
+
+
+def _pack_rows_and_columns(m, rows, ld, width, dcode, code, q, qts, wss=None, colsums=None):
+    """_pack_both for a batch whose column forms, workspaces and column sums come by its parts (each list may hold None, q may be None)."""
+    if len(qts) == 1 or (qts[0] is None and colsums is None):   # (rows alone: any number of them)
+        return _pack_both(m, rows, ld, width, dcode, code, q, qts[0], wss and wss[0], colsums and colsums[0])
+    m = m if m.dim() == 2 else m.view(rows, width)
+    for i, (at, n) in enumerate(_parts(rows)):
+        part = None if q is None else (q[0] + at * q[1], q[1], q[2] + at * q[3], q[3])
+        _pack_both(m[at:at + n], n, ld, width, dcode, code, part, qts[i], wss and wss[i], colsums and colsums[i])
+
+
 def _forward(x, weight, bias, code, need_x, need_w):
     """-> y = P(x) P(w)^T + b and what a backward reads: P'(x) where the weight's gradient is wanted, P'(w) where x's is (None: neither)."""
     m, rows, ld = as_rows(x)
@@ -300,10 +316,10 @@ def _forward(x, weight, bias, code, need_x, need_w):
         w2, _, wld = as_rows(weight)
         now, later = _Forms(), _Forms()
         qx, qw = now.form(rows, K), now.form(N, K)
-        qxt, qwt = later.form(K, rows, need_w), later.form(K, N, need_x)
+        qxts, qwt = [later.form(K, n, need_w) for _, n in _parts(rows)], later.form(K, N, need_x)
         now.allocate(x)
         kept = later.allocate(x) if need_x or need_w else None
-        _pack_both(m, rows, ld, K, DTYPES[x.dtype], code, qx, qxt)
+        _pack_rows_and_columns(m, rows, ld, K, DTYPES[x.dtype], code, qx, qxts)
         _pack_both(w2, N, wld, K, DTYPES[weight.dtype], code, qw, qwt)
         return _product(qx, code, qw, code, bias, x, shape, x.dtype), kept
 
@@ -333,20 +349,35 @@ class _Linear8(torch.autograd.Function):
                     torch.zeros(N, device=dev, dtype=torch.float32) if need_b else None, None, None)
         m, rows, ld = as_rows(dy)
         K = wshape[1]
+        parts = _parts(rows)
         with device_of(dy):
             later, now = _Forms(), _Forms()
-            qxt, qwt = later.form(K, rows, need_w), later.form(K, N, need_x)
+            qxts, qwt = [later.form(K, n, need_w) for _, n in parts], later.form(K, N, need_x)
             if need_x or need_w:
                 kept = saved(ctx.saved_tensors[0], (later.bytes,), torch.uint8, dev).contiguous()
                 later.rebase(kept if kept.data_ptr() % 16 == 0 else kept.clone())   # (what the products take)
-            qd, qdt = now.form(rows, N, need_x), now.form(N, rows, need_w)
-            ws = now.floats(_lib.lib().kp_q8_pack_both_ws_floats(rows, N), need_b)
+            qd, qdts = now.form(rows, N, need_x), [now.form(N, n, need_w) for _, n in parts]
+            wss = dbs = None
+            if need_b:
+                wss = [now.floats(_lib.lib().kp_q8_pack_both_ws_floats(n, N)) for _, n in parts]
+                dbs = [dy.new_empty(N, dtype=torch.float32) for _ in parts]
             now.allocate(dy)
-            db = dy.new_empty(N, dtype=torch.float32) if need_b else None
-            _pack_both(m, rows, ld, N, DTYPES[dy.dtype], grad_code, qd, qdt, ws, db)
+            _pack_rows_and_columns(m, rows, ld, N, DTYPES[dy.dtype], grad_code, qd, qdts, wss, dbs)
             dx = _product(qd, grad_code, qwt, code, None, dy, xshape, xdtype) if need_x else None
-            dw = _product(qdt, grad_code, qxt, code, None, dy, wshape, wdtype) if need_w else None
+            if len(parts) == 1:
+                dw = _product(qdts[0], grad_code, qxts[0], code, None, dy, wshape, wdtype) if need_w else None
+                db = dbs[0] if need_b else None
+            else:   # (sums of the parts in fp32, in their order, rounded once)
+                dw = _total(_product(a, grad_code, b, code, None, dy, wshape, torch.float32) for a, b in zip(qdts, qxts)).to(wdtype) if need_w else None
+                db = _total(iter(dbs)) if need_b else None
         return dx, dw, db, None, None
+
+
+def _total(tensors):
+    total = next(tensors)
+    for t in tensors:
+        total += t
+    return total
 
 
 def _suits(rows, N, K, code):
@@ -360,7 +391,7 @@ def linear8(x: torch.Tensor, weight, bias: torch.Tensor = None, fmt: str = 'e4m3
     weight a tensor [n, k] (fp32 master weights, or 16 bits): every call packs x and the weight in `fmt`; differentiable in x, weight and
     bias.  The backward packs the output gradient in `grad_fmt` and takes dx and dw from two more 8-bit products; between the passes only
     8-bit forms wait (a byte an element of x and of the weight).  Gradients come in the types of what they belong to.  A product sums over at
-    most 8388480 elements: rows, where the weight's or bias's gradient is asked for (larger batches in parts, whose gradients add up).
+    most 8388480 elements; the weight's gradient of more rows is the sum of such parts.
     weight a Packed8 (pack8): serving.  `fmt` is x's format; no gradient.
 
     Each product is matmul8's: y and dx as x's type has it, dw as the weight's has it.  A float32 x takes the exact sums."""
@@ -390,8 +421,7 @@ def linear8(x: torch.Tensor, weight, bias: torch.Tensor = None, fmt: str = 'e4m3
         K = weight.shape[1]
         rows = x.numel() // K
         if rows > MOST or N > MOST or K > MOST:
-            _check_sizes('linear8', rows, N, ('inner elements', K), ("outputs (x's gradient)", N if grad and x.requires_grad else 0),
-                         ("rows (the weight's and bias's gradients)", rows if grad and (weight.requires_grad or (bias is not None and bias.requires_grad)) else 0))
+            _check_sizes('linear8', rows, N, ('inner elements', K), ("outputs (x's gradient)", N if grad and x.requires_grad else 0))
         bias = as_vector(bias)
         return _Linear8.apply(x, weight, bias, fmt, grad_fmt) if grad else _forward(x, weight, bias, code, False, False)[0]
     if grad:

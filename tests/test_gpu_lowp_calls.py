@@ -43,7 +43,7 @@ def test_a_layer_with_and_without_gradients():
 
 
 def test_many_rows_without_gradients():
-    """More rows than a training step takes, with a Parameter as weight."""
+    """More rows than one sum takes, with a Parameter as weight."""
     from keypoints_amd import lowp
     rows = lowp.MOST + 200
     x = torch.randn(rows, 8, device='cuda', dtype=torch.bfloat16)
@@ -51,8 +51,57 @@ def test_many_rows_without_gradients():
     with torch.no_grad():
         y = lowp.linear8(x, w)
         assert torch.equal(y[-300:], lowp.linear8(x[-300:].contiguous(), w)) and torch.equal(y[:300], lowp.linear8(x[:300].contiguous(), w))
-    with pytest.raises(ValueError, match='8388480'):
-        lowp.linear8(x, w)
+
+
+@pytest.mark.parametrize('wtype', [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize('most', [256, 1024, 1920])
+def test_a_batch_in_parts_is_the_whole_batch(monkeypatch, most, wtype):
+    """Whole numbers, whose sums are exact in any grouping: a step that packs its batch in parts gives what one part gives, bit for bit."""
+    from keypoints_amd import lowp
+    g = torch.Generator().manual_seed(8)
+    numbers = lambda *s: torch.randint(-7, 8, s, generator=g).float()
+    wide = numbers(2049, 150).bfloat16().cuda()
+    for x in (wide[:, 3:133], wide[:2048, :130].contiguous().view(2, 1024, 130)):
+        leaves = [x.detach().clone().requires_grad_() if x.dim() == 3 else x.detach().requires_grad_(), numbers(70, 130).to(wtype).cuda().requires_grad_(),
+                  numbers(70).cuda().requires_grad_()]
+        dy = numbers(x.numel() // 130, 70).bfloat16().cuda().view(*x.shape[:-1], 70)
+        got = []
+        for n in (lowp.MOST, most):
+            monkeypatch.setattr(lowp, 'MOST', n)
+            y = lowp.linear8(*leaves)
+            got.append([y.detach(), *torch.autograd.grad(y, leaves, dy)])
+            for i in range(3):   # ... and each gradient by itself
+                alone = [t.detach().requires_grad_(i == k) for k, t in enumerate(leaves)]
+                one, = torch.autograd.grad(lowp.linear8(*alone), alone[i], dy)
+                assert torch.equal(one, got[-1][1 + i])
+            for t in leaves:
+                t.requires_grad_()
+        assert all(torch.equal(a, b) for a, b in zip(*got))
+        assert torch.equal(got[1][2], (dy.reshape(-1, 70).double().t().contiguous() @ x.reshape(-1, 130).double()).float().to(wtype))
+        monkeypatch.undo()
+
+
+@pytest.mark.parametrize('N,K', [(16, 8), (300, 260)])
+def test_a_training_step_of_more_rows_than_one_sum_takes(N, K):
+    """128 frames of 256 x 256 and some more, as rows of -1, 0 and 1: sums stay far below 2^24 and are exact."""
+    from keypoints_amd import lowp
+    rows = 128 * 256 * 256 + 77
+    g = torch.Generator(device='cuda').manual_seed(9)
+    few = lambda *s: torch.randint(-1, 2, s, generator=g, device='cuda', dtype=torch.int8)
+    x, w, b, dy = few(rows, K).bfloat16().requires_grad_(), few(N, K).float().requires_grad_(), few(N).float().requires_grad_(), few(rows, N).bfloat16()
+    y = lowp.linear8(x, w, b)
+    dx, dw, db = torch.autograd.grad(y, (x, w, b), dy)
+    want = torch.zeros(N, K, device='cuda', dtype=torch.float64)
+    sums = torch.zeros(N, device='cuda', dtype=torch.float64)
+    with torch.no_grad():
+        for at in range(0, rows, 1 << 20):
+            part = slice(at, at + (1 << 20))
+            xd, dyd = x[part].double(), dy[part].double()
+            want += torch.mm(dyd.t().contiguous(), xd)
+            sums += dyd.sum(0)
+            assert torch.equal(y[part], (torch.mm(xd, w.double().t().contiguous()) + b.double()).bfloat16())
+            assert torch.equal(dx[part], torch.mm(dyd, w.double()).bfloat16())
+    assert want.abs().max() < 1 << 20 and torch.equal(dw, want.float()) and torch.equal(db, sums.float())
 
 
 def test_saved_forms_given_back_strided():

@@ -134,11 +134,9 @@ def test_a_layer_evaluated_without_gradients_packs_rows_only(made):
         assert lowp.linear8(x[:0], w, b).shape == (0, 40) and not made
 
 
-@pytest.mark.parametrize('rows,width,inner,wants', [(8388481, 3, 4, 'w'), (8388481, 3, 4, 'b'), (8388608, 3, 4, 'xwb'), (3, 8388481, 4, 'x'),
-                                                    (5, 3, 8388481, ''), (5, 3, 8388481, 'w'), (40, 1 << 29, 1, '')])
+@pytest.mark.parametrize('rows,width,inner,wants', [(3, 8388481, 4, 'x'), (5, 3, 8388481, ''), (5, 3, 8388481, 'w'), (40, 1 << 29, 1, '')])
 def test_products_longer_than_one_call_takes(made, rows, width, inner, wants):
-    """A sum over more than 8388480 elements -- the rows are the weight gradient's -- is refused by the call itself, not between its launches or
-    in the backward; where no such sum is asked for, any number of rows passes."""
+    """A sum over more than 8388480 elements is refused by the call itself, not between its launches or in the backward."""
     x = torch.zeros(1, dtype=torch.bfloat16).expand(rows, inner).requires_grad_('x' in wants)   # (no memory behind it)
     w = torch.zeros(1).expand(width, inner).requires_grad_('w' in wants)
     b = torch.zeros(width).requires_grad_('b' in wants) if width < 10 else None
@@ -147,27 +145,53 @@ def test_products_longer_than_one_call_takes(made, rows, width, inner, wants):
     assert not made
 
 
-def test_many_rows_without_the_weights_gradient(made, monkeypatch):
+@pytest.mark.parametrize('shape', [(300,), (2, 3, 50), (512,), (513,)])
+@pytest.mark.parametrize('wants', ['x', 'w', 'b', 'xb', 'xwb'])
+def test_more_rows_than_one_sum_takes(made, monkeypatch, shape, wants):
+    """A training step of more rows than a product sums over packs the batch along itself in parts that begin on whole blocks; the parts' gradients
+    are added.  Every byte of the forms is written by exactly one part."""
     monkeypatch.setattr(lowp, 'MOST', 256)
-    x, w, b = torch.zeros(300, 8), torch.zeros(5, 8), torch.zeros(5)
+    rows = torch.Size(shape).numel()
+    sizes = [256] * (rows // 256) + ([rows % 256] if rows % 256 else [])
+    x, w, b = torch.zeros(*shape, 140), torch.zeros(5, 140), torch.zeros(5)
+    leaves = [t.requires_grad_(k in wants) for t, k in ((x, 'x'), (w, 'w'), (b, 'b'))]
+    y = lowp.linear8(*leaves)
+    if 'w' in wants:
+        calls = [a for name, a in made if name == 'kp_q8_pack_both' and a[12] != 5]
+        assert [a[12] for a in calls] == sizes and all(a[13] == 140 for a in calls)
+        at = 0
+        for a in calls:   # x, ldx, q, ldq, s, lds, qt, ldqt, ...
+            assert a[0] == x.data_ptr() + at * 140 * 4 and a[2] == calls[0][2] + at * 256 and a[4] == calls[0][4] + at * 4 and a[7] % 128 == 0 and a[7] >= a[12]
+            at += a[12]
+        spans = sorted((a[6], a[6] + 140 * a[7]) for a in calls)
+        assert all(e <= b for (_, e), (b, _) in zip(spans, spans[1:]))
+    else:
+        assert [(name, a[6]) for name, a in made if name == 'kp_q8_pack'][0] == ('kp_q8_pack', rows)
+    made.clear()
+    g = torch.autograd.grad(y, [t for t in leaves if t.requires_grad], torch.zeros_like(y))
+    both = [a for name, a in made if name == 'kp_q8_pack_both']
+    if 'w' in wants or 'b' in wants:
+        assert [a[12] for a in both] == sizes
+    assert [a[14:17] for name, a in made if name == 'kp_q8_matmul'] == ([(rows, 140, 5)] if 'x' in wants else []) + ([(5, 140, n) for n in sizes] if 'w' in wants else [])
+    assert [t.shape for t in g] == [t.shape for t in leaves if t.requires_grad]
+
+
+def test_lengths_that_are_refused(made, monkeypatch):
+    monkeypatch.setattr(lowp, 'MOST', 256)
     leaf = lambda t: t.clone().requires_grad_()
-    lowp.linear8(leaf(x), w, b).sum().backward()
-    lowp.linear8(x, w, b)
-    with torch.no_grad():
-        lowp.linear8(x, leaf(w), leaf(b))
-    for args in ((x, leaf(w), b), (x, w, leaf(b)), (leaf(torch.zeros(3, 8)), torch.zeros(300, 8), None), (torch.zeros(3, 300), torch.zeros(5, 300), None)):
+    for args in ((leaf(torch.zeros(3, 8)), torch.zeros(300, 8), None), (torch.zeros(3, 300), torch.zeros(5, 300), None)):
         made.clear()
         with pytest.raises(ValueError, match='256'):
             lowp.linear8(*args)
         assert not made
-    for rows, kind in ((4, None), (20, ValueError)):   # serving: a few rows are summed by a kernel without that limit
+    for rows, refused in ((4, False), (20, True)):   # serving: a few rows are summed by a kernel without that limit
         x, packed = torch.zeros(rows, 600, dtype=torch.bfloat16), lowp.pack8(torch.zeros(300, 600))
         monkeypatch.setattr(lowp, '_suits', lambda M, N, K, code: M <= 4)
         made.clear()
-        if kind is None:
+        if not refused:
             lowp.linear8(x, packed)
         else:
-            with pytest.raises(kind, match='256'):
+            with pytest.raises(ValueError, match='256'):
                 lowp.linear8(x, packed)
             assert not made
     with pytest.raises(ValueError, match='256'):
