@@ -290,19 +290,26 @@ def matmul8(a: Packed8, b: Packed8, bias: torch.Tensor = None, dtype: torch.dtyp
 
 
 def _parts(rows):
-    """(first row, rows) of the parts in which a batch is packed along itself: one, but past MOST rows.  They begin on whole blocks, so the blocks
-    are the whole batch's; the weight's and bias's gradients add up over the parts."""
-    return ((0, rows),) if rows <= MOST else tuple((at, min(MOST, rows - at)) for at in range(0, rows, MOST))
+    """(first row, rows) of the parts in which a batch of more than MOST rows is packed along itself.  They begin on whole blocks, so the blocks are
+    the whole batch's; the weight's and bias's gradients add up over the parts."""
+    return [(at, min(MOST, rows - at)) for at in range(0, rows, MOST)]
 
 
-def _pack_rows_and_columns(m, rows, ld, width, dcode, code, q, qts, wss=None, colsums=None):
-    """_pack_both for a batch whose column forms, workspaces and column sums come by its parts (each list may hold None, q may be None)."""
-    if len(qts) == 1 or (qts[0] is None and colsums is None):   # (rows alone: any number of them)
-        return _pack_both(m, rows, ld, width, dcode, code, q, qts[0], wss and wss[0], colsums and colsums[0])
+def _pack_parts(m, rows, ld, width, dcode, code, q, qts, wss=None, colsums=None):
+    """_pack_both for such a batch: a column form, workspace and column sums for each part (q, and whole lists, may be None)."""
     m = m if m.dim() == 2 else m.view(rows, width)
     for i, (at, n) in enumerate(_parts(rows)):
         part = None if q is None else (q[0] + at * q[1], q[1], q[2] + at * q[3], q[3])
-        _pack_both(m[at:at + n], n, ld, width, dcode, code, part, qts[i], wss and wss[i], colsums and colsums[i])
+        _pack_both(m[at:at + n], n, ld, width, dcode, code, part, qts and qts[i], wss and wss[i], colsums and colsums[i])
+
+
+def _total(tensors):
+    """Their sum, in their order (into the first)."""
+    tensors = iter(tensors)
+    total = next(tensors)
+    for t in tensors:
+        total += t
+    return total
 
 
 def _forward(x, weight, bias, code, need_x, need_w):
@@ -316,10 +323,12 @@ def _forward(x, weight, bias, code, need_x, need_w):
         w2, _, wld = as_rows(weight)
         now, later = _Forms(), _Forms()
         qx, qw = now.form(rows, K), now.form(N, K)
-        qxts, qwt = [later.form(K, n, need_w) for _, n in _parts(rows)], later.form(K, N, need_x)
+        long = need_w and rows > MOST
+        qxt = [later.form(K, n) for _, n in _parts(rows)] if long else later.form(K, rows, need_w)
+        qwt = later.form(K, N, need_x)
         now.allocate(x)
         kept = later.allocate(x) if need_x or need_w else None
-        _pack_rows_and_columns(m, rows, ld, K, DTYPES[x.dtype], code, qx, qxts)
+        (_pack_parts if long else _pack_both)(m, rows, ld, K, DTYPES[x.dtype], code, qx, qxt)
         _pack_both(w2, N, wld, K, DTYPES[weight.dtype], code, qw, qwt)
         return _product(qx, code, qw, code, bias, x, shape, x.dtype), kept
 
@@ -349,35 +358,38 @@ class _Linear8(torch.autograd.Function):
                     torch.zeros(N, device=dev, dtype=torch.float32) if need_b else None, None, None)
         m, rows, ld = as_rows(dy)
         K = wshape[1]
-        parts = _parts(rows)
         with device_of(dy):
             later, now = _Forms(), _Forms()
-            qxts, qwt = [later.form(K, n, need_w) for _, n in parts], later.form(K, N, need_x)
+            parts = _parts(rows) if rows > MOST else None
+            qxt = later.form(K, rows, need_w) if parts is None or not need_w else [later.form(K, n) for _, n in parts]
+            qwt = later.form(K, N, need_x)
             if need_x or need_w:
                 kept = saved(ctx.saved_tensors[0], (later.bytes,), torch.uint8, dev).contiguous()
                 later.rebase(kept if kept.data_ptr() % 16 == 0 else kept.clone())   # (what the products take)
-            qd, qdts = now.form(rows, N, need_x), [now.form(N, n, need_w) for _, n in parts]
-            wss = dbs = None
-            if need_b:
-                wss = [now.floats(_lib.lib().kp_q8_pack_both_ws_floats(n, N)) for _, n in parts]
-                dbs = [dy.new_empty(N, dtype=torch.float32) for _ in parts]
-            now.allocate(dy)
-            _pack_rows_and_columns(m, rows, ld, N, DTYPES[dy.dtype], grad_code, qd, qdts, wss, dbs)
+            qd, dw = now.form(rows, N, need_x), None
+            ws_floats, dcode = _lib.lib().kp_q8_pack_both_ws_floats, DTYPES[dy.dtype]
+            if parts is None:
+                qdt = now.form(N, rows, need_w)
+                ws = now.floats(ws_floats(rows, N), need_b)
+                now.allocate(dy)
+                db = dy.new_empty(N, dtype=torch.float32) if need_b else None
+                _pack_both(m, rows, ld, N, dcode, grad_code, qd, qdt, ws, db)
+            else:
+                qdt = [now.form(N, n) for _, n in parts] if need_w else None
+                wss = [now.floats(ws_floats(n, N)) for _, n in parts] if need_b else None
+                now.allocate(dy)
+                dbs = [dy.new_empty(N, dtype=torch.float32) for _ in parts] if need_b else None
+                if need_w or need_b:
+                    _pack_parts(m, rows, ld, N, dcode, grad_code, qd, qdt, wss, dbs)
+                else:
+                    _pack_both(m, rows, ld, N, dcode, grad_code, qd, None)
+                db = _total(dbs) if need_b else None
             dx = _product(qd, grad_code, qwt, code, None, dy, xshape, xdtype) if need_x else None
-            if len(parts) == 1:
-                dw = _product(qdts[0], grad_code, qxts[0], code, None, dy, wshape, wdtype) if need_w else None
-                db = dbs[0] if need_b else None
-            else:   # (sums of the parts in fp32, in their order, rounded once)
-                dw = _total(_product(a, grad_code, b, code, None, dy, wshape, torch.float32) for a, b in zip(qdts, qxts)).to(wdtype) if need_w else None
-                db = _total(iter(dbs)) if need_b else None
+            if need_w and parts is None:
+                dw = _product(qdt, grad_code, qxt, code, None, dy, wshape, wdtype)
+            elif need_w:   # (added in fp32, rounded once)
+                dw = _total(_product(a, grad_code, b, code, None, dy, wshape, torch.float32) for a, b in zip(qdt, qxt)).to(wdtype)
         return dx, dw, db, None, None
-
-
-def _total(tensors):
-    total = next(tensors)
-    for t in tensors:
-        total += t
-    return total
 
 
 def _suits(rows, N, K, code):
